@@ -253,6 +253,151 @@ SKV_API int skv_schedule_phases(const uint64_t* demand, int n_src, int n_dst, sk
 SKV_API int skv_slice_segments(const skv_segment* segs, int n_segs, uint64_t lo, uint64_t hi, skv_segment* out,
                                int out_cap, int* n_out);
 
+/* ------------------------------------------------------------------ operators on a cache and a state row
+ * What a prefill role runs to fill the storage this library moves, and a decode role to go on from it.  No counterpart
+ * in the reference's path (its model kernels are elsewhere); the page address rule, the int8 format and the state-row
+ * sizes are the ones above.  All of them run on the current device, on `stream`, read their lengths and tables on the
+ * device, allocate nothing and can be captured into a CUDA graph (after one call outside of capture has set up the
+ * device).  Activations are fp16 or bf16 (`dtype`); sums, softmax statistics, states and angles are held in 32 bits or
+ * more.  Row pointers are 16-byte aligned and strides (in elements, between tokens) multiples of 8; the heads of one
+ * token lie back to back.  An output may not overlap an input unless an argument says so. */
+#define SKV_DTYPE_F16 0
+#define SKV_DTYPE_BF16 1
+
+/* cache formats: fp16 values, or int8 codes with one fp16 scale per 64 values of a cell */
+#define SKV_KV_F16 0
+#define SKV_KV_INT8 1
+
+/* device status word bit: a state_index entry was outside [0, state_rows): the sequence was left alone */
+#define SKV_STATUS_BAD_STATE_ROW 0x8u
+
+/* One layer's paged K and V over a batch of sequences.  Logical page p of sequence s is pool page
+ * page_tables[s * table_stride + p] of both pools (with a block pool: v_pool = k_pool + pages_per_block pages, and
+ * page_limit = n_blocks * slot_pages - pages_per_block).  A page is [kv_head][page_size][head_dim] values; the scales
+ * of an int8 page are [kv_head][page_size][head_dim / 64] fp16.  head_dim is 64, 128 or 256, page_size a power of two
+ * up to 256.  A table entry outside [0, page_limit) is not dereferenced: its cells are skipped and
+ * SKV_STATUS_BAD_SRC_PAGE (reading) or SKV_STATUS_BAD_DST_PAGE (writing) is set. */
+typedef struct skv_kv_layer {
+    void* k_pool;
+    void* v_pool;
+    void* k_scale;                /* SKV_KV_INT8 only */
+    void* v_scale;
+    const int32_t* page_tables;   /* device, n_tables rows of table_stride entries */
+    int64_t table_stride;
+    int64_t page_limit;
+    int32_t n_tables;
+    int32_t n_head_kv;
+    int32_t head_dim;
+    int32_t page_size;
+    int32_t format;
+    int32_t reserved;
+} skv_kv_layer;
+
+/* skv_kv_append - write the K and V of new tokens into their cells, with the rotary positions applied to K on the way.
+ *
+ * Rows [seq_starts[s], seq_starts[s+1]) of k and v belong to sequence s and go to its cells lengths[s], lengths[s]+1, ...
+ * (seq_starts null: one row per sequence).  Rows before the first or behind the last sequence are neither read nor
+ * written.  A cell is rotated by its own number: pair j turns by cell * inv_freq[j], the product taken in 64 bits, and
+ * is scaled by rope_scale.  SKV_ROPE_HALF pairs value j with j + n_rot/2, SKV_ROPE_PAIRS value 2j with 2j+1; values
+ * from n_rot on pass through; n_rot 0 (inv_freq null) rotates nothing.  q, when given, is rotated the same way into
+ * q_out, which may be q itself.  int8: scale = fp16(max |x| / 127) per 64 values, code = x / scale rounded to nearest
+ * even, within +-127 (a zero scale gives codes 0; a scale past fp16 saturates; a NaN takes code 0).
+ * lengths_out, when given, gets lengths[s] + the number of its rows.
+ * A cell past the table (table_stride * page_size) or a negative length sets SKV_STATUS_BAD_DST_PAGE; nothing is
+ * written for it in the cache (q_out is).  Two rows must not name the same cell. */
+#define SKV_ROPE_HALF 0
+#define SKV_ROPE_PAIRS 1
+typedef struct skv_append_args {
+    const void* k;               /* [n_tokens][n_head_kv][head_dim] */
+    const void* v;
+    int64_t k_stride;
+    int64_t v_stride;
+    const void* q;               /* optional with q_out: [n_tokens][n_head][head_dim] */
+    void* q_out;
+    int64_t q_stride;
+    int64_t q_out_stride;
+    const int32_t* seq_starts;   /* device [n_seqs + 1] ascending, or null */
+    const int32_t* lengths;      /* device [n_seqs]: cells already held */
+    int32_t* lengths_out;        /* device [n_seqs], optional, not `lengths` itself */
+    const float* inv_freq;       /* device [n_rot / 2] */
+    int32_t n_tokens;
+    int32_t n_seqs;
+    int32_t n_head;
+    int32_t n_rot;               /* a multiple of 16, at most head_dim */
+    int32_t rope_style;
+    int32_t dtype;
+    float rope_scale;
+    int32_t reserved;
+} skv_append_args;
+SKV_API int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* args, void* stream);
+
+/* skv_decode_attention - softmax(scale * q K^T) V of one new token per sequence over the first lengths[s] cells of its
+ * cache.  Query head h reads K/V head h / (n_head / n_head_kv).  lse, when given, gets the natural logarithm of the
+ * sum of the exponentials per (sequence, head), so parts of one cache held apart can be joined.  A sequence of length
+ * 0 (or one whose every cell was skipped, or scored minus infinity) gives zeros and lse -inf.  A length past the table
+ * attends what the table holds and sets SKV_STATUS_BAD_SRC_PAGE; so does a negative one, which attends nothing.
+ * Results do not depend on timing: the same inputs give the same bits.
+ * workspace: skv_decode_attention_workspace bytes of device memory, 256-byte aligned.  Its content is nobody's between
+ * calls; two calls that may overlap on the GPU (two streams, two graphs) need one each. */
+typedef struct skv_attention_args {
+    const void* q;               /* [n_seqs][n_head][head_dim] */
+    void* out;                   /* [n_seqs][n_head][head_dim] */
+    int64_t q_stride;
+    int64_t out_stride;
+    float* lse;                  /* [n_seqs][n_head], optional */
+    const int32_t* lengths;      /* device [n_seqs] */
+    void* workspace;
+    uint64_t workspace_bytes;
+    int32_t n_seqs;
+    int32_t n_head;
+    int32_t dtype;
+    float scale;
+} skv_attention_args;
+SKV_API int skv_decode_attention(const skv_kv_layer* layer, const skv_attention_args* args, void* stream);
+SKV_API int skv_decode_attention_workspace(const skv_kv_layer* layer, int n_seqs, int n_head, uint64_t* out_bytes);
+
+/* skv_gated_delta - the gated delta rule of a linear-attention layer over packed sequences, token by token
+ *     S <- exp(g) S;   S <- S + beta k (v - k^T S)^T;   out = scale * S^T q
+ * with the fp32 state row of each sequence read before its first token and written after its last.  Row r of the
+ * state is [n_v_heads][head_dim key][head_dim value] floats at state + r * state_stride; sequence s uses row
+ * state_index[s] (null: s).  Each row at most once per call.  Value head h uses key head h / (n_v_heads / n_k_heads).
+ * g is the logarithm of the decay (<= 0; -inf forgets everything), beta the write strength, k of about unit length.
+ * seq_starts as in skv_kv_append; max_tokens bounds the tokens of one sequence (a longer one is cut there).  Few tokens
+ * a sequence run token by token, long ones in chunks through the tensor cores; both hold S in 32 bits.
+ * workspace: skv_gated_delta_workspace bytes of device memory, 256-byte aligned; as for skv_decode_attention. */
+typedef struct skv_gdn_args {
+    const void* q;               /* [n_tokens][n_k_heads][head_dim] */
+    const void* k;
+    const void* v;               /* [n_tokens][n_v_heads][head_dim] */
+    void* out;                   /* [n_tokens][n_v_heads][head_dim] */
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t out_stride;
+    const float* g;              /* [n_tokens][n_v_heads] */
+    const float* beta;
+    int64_t g_stride;            /* elements between tokens, any */
+    int64_t beta_stride;
+    float* state;
+    int64_t state_stride;        /* floats between rows, a multiple of 4 */
+    int64_t state_rows;
+    const int32_t* state_index;  /* device [n_seqs] or null */
+    const int32_t* seq_starts;   /* device [n_seqs + 1] or null: one token per sequence */
+    void* workspace;
+    uint64_t workspace_bytes;
+    int32_t n_tokens;
+    int32_t n_seqs;
+    int32_t n_k_heads;
+    int32_t n_v_heads;
+    int32_t head_dim;            /* 64 or 128 */
+    int32_t max_tokens;
+    int32_t dtype;
+    float scale;
+} skv_gdn_args;
+SKV_API int skv_gated_delta(const skv_gdn_args* args, void* stream);
+SKV_API int skv_gated_delta_workspace(int n_tokens, int n_seqs, int n_v_heads, int head_dim, int max_tokens,
+                                      uint64_t* out_bytes);
+
 #ifdef __cplusplus
 }
 #endif

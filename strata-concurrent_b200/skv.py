@@ -1,7 +1,7 @@
 """skv.py - Python bindings of libstrata_kv.so (the B200 KV handoff / park-resume C ABI, include/strata_kv.h).
 
-This is the host mirror the tests and bench.py drive.  It is plumbing over the C ABI: every byte is moved by
-the sm_100a kernels in csrc/skv_copy.cu.  There is no Python or CPU fallback: if the library is missing the
+This is the host mirror the tests and bench.py drive.  It is plumbing over the C ABI: every byte is moved and computed by
+the sm_100a kernels in csrc/.  There is no Python or CPU fallback: if the library is missing the
 import of any entry point raises.
 
 Layout of a sequence's cache in a block pool (one pool per GPU):
@@ -24,11 +24,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libstrata_kv.so")
 
 OK, EINVAL, ECUDA, ENOMEM, ETIMEOUT, EDEVICE, ERANGE = range(7)
-STATUS_BAD_SRC_PAGE, STATUS_BAD_DST_PAGE, STATUS_WAIT_TIMEOUT = 0x1, 0x2, 0x4
+STATUS_BAD_SRC_PAGE, STATUS_BAD_DST_PAGE, STATUS_WAIT_TIMEOUT, STATUS_BAD_STATE_ROW = 0x1, 0x2, 0x4, 0x8
 COPY_AUTO, COPY_TMA, COPY_VEC = 0, 1, 2
 PARK_DIRECT, PARK_STAGED = 1, 2
 MAX_SEGMENTS = 64
 NOALLOC_MAX_SEGMENTS = 512
+
+DTYPE_F16, DTYPE_BF16 = 0, 1
+KV_F16, KV_INT8 = 0, 1
+ROPE_STYLES = {"half": 0, "pairs": 1}
 
 PAGE_CELLS = 4
 BLOCK_TOKENS = 256
@@ -50,6 +54,42 @@ class SchedRun(C.Structure):
     """skv_sched_run: one transfer of a many-to-many hand-off batch (skv_schedule_phases)."""
     _fields_ = [("phase", C.c_int32), ("src", C.c_int32), ("lo", C.c_uint64), ("hi", C.c_uint64),
                 ("wait", C.c_int32), ("signal_dst", C.c_int32), ("signal_idx", C.c_int32), ("reserved", C.c_int32)]
+
+
+class KvLayerArgs(C.Structure):
+    """skv_kv_layer."""
+    _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("page_tables", C.c_void_p), ("table_stride", C.c_int64), ("page_limit", C.c_int64),
+                ("n_tables", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+                ("format", C.c_int32), ("reserved", C.c_int32)]
+
+
+class AppendArgs(C.Structure):
+    """skv_append_args."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("seq_starts", C.c_void_p), ("lengths", C.c_void_p), ("lengths_out", C.c_void_p), ("inv_freq", C.c_void_p),
+                ("n_tokens", C.c_int32), ("n_seqs", C.c_int32), ("n_head", C.c_int32), ("n_rot", C.c_int32),
+                ("rope_style", C.c_int32), ("dtype", C.c_int32), ("rope_scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class AttentionArgs(C.Structure):
+    """skv_attention_args."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("lse", C.c_void_p), ("lengths", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("n_seqs", C.c_int32), ("n_head", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float)]
+
+
+class GatedDeltaArgs(C.Structure):
+    """skv_gdn_args."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("g", C.c_void_p), ("beta", C.c_void_p), ("g_stride", C.c_int64), ("beta_stride", C.c_int64),
+                ("state", C.c_void_p), ("state_stride", C.c_int64), ("state_rows", C.c_int64),
+                ("state_index", C.c_void_p), ("seq_starts", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64), ("n_tokens", C.c_int32), ("n_seqs", C.c_int32),
+                ("n_k_heads", C.c_int32), ("n_v_heads", C.c_int32), ("head_dim", C.c_int32), ("max_tokens", C.c_int32),
+                ("dtype", C.c_int32), ("scale", C.c_float)]
 
 
 _lib = None
@@ -95,6 +135,11 @@ _SIGNATURES = {
                              C.POINTER(C.c_int)], C.c_int),
     "skv_slice_segments": ([C.c_void_p, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p, C.c_int, C.POINTER(C.c_int)],
                            C.c_int),
+    "skv_kv_append": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "skv_decode_attention": ([C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+    "skv_decode_attention_workspace": ([C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_uint64)], C.c_int),
+    "skv_gated_delta": ([C.c_void_p, C.c_void_p], C.c_int),
+    "skv_gated_delta_workspace": ([C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_uint64)], C.c_int),
 }
 
 
@@ -547,3 +592,173 @@ def unpack_segments(image, dst: PooledSequence) -> list:
     segs.append(segment(base + off["gdn"], dst.gdn, g.gdn_bytes))
     segs.append(segment(base + off["ids"], dst.ids, 16 * ((4 * t + 15) // 16)))
     return segs
+
+
+# ------------------------------------------------------------------------------------------------ operators
+# On device tensors (torch's, or anything with its data_ptr, shape, stride, dtype and device).  They run on the current
+# device and, like the copies, on `stream` (None: the legacy default stream).
+
+_CODES = {"torch.float16": DTYPE_F16, "torch.bfloat16": DTYPE_BF16}
+_KNOWN = {}     # dtype object -> (its name, its code or None), so that a call formats no text
+
+
+def _dtype(x) -> tuple:
+    got = _KNOWN.get(x.dtype)
+    if got is None:
+        name = str(x.dtype)
+        got = _KNOWN[x.dtype] = (name, _CODES.get(name))
+    return got
+
+
+def _rows(x, what: str, like=None) -> tuple:
+    """(address, rows, heads, values, elements between rows) of a [row][head][value] tensor whose heads lie back to back."""
+    n, heads, dim = x.shape
+    step, between, one = x.stride()
+    if (between != dim and heads > 1) or (one != 1 and dim > 1):
+        raise ValueError(f"{what}: the heads of a row must lie back to back")
+    if _dtype(x)[1] is None or (like is not None and x.dtype != like.dtype):
+        raise TypeError(f"{what}: {x.dtype} (all of a call's activations are float16, or all bfloat16)")
+    if not x.is_cuda:
+        raise ValueError(f"{what}: not on a GPU")
+    return x.data_ptr(), n, heads, dim, step if n > 1 else heads * dim
+
+
+def _vector(x, what: str, name: str, at_least: int):
+    """The address of a contiguous 1-d device tensor of `name` values; None for None."""
+    if x is None:
+        return None
+    if _dtype(x)[0] != name or x.dim() != 1 or not x.is_cuda or (x.shape[0] > 1 and x.stride(0) != 1):
+        raise TypeError(f"{what}: a contiguous 1-d {name} tensor on the GPU")
+    if x.shape[0] < at_least:
+        raise ValueError(f"{what}: {x.shape[0]} entries, {at_least} needed")
+    return x.data_ptr()
+
+
+class KvLayer:
+    """One layer's paged K and V over a batch of sequences (skv_kv_layer): pools of [page][kv_head][cell][head_dim]
+    values (float16, or int8 with float16 scales [page][kv_head][cell][head_dim / 64]) and int32 page tables
+    [sequence][page], all on the GPU.  Keeps references to the tensors it was made of."""
+
+    def __init__(self, k_pool, v_pool, page_tables, *, k_scale=None, v_scale=None):
+        pages, n_head_kv, page_size, head_dim = k_pool.shape
+        fmt = {"torch.float16": KV_F16, "torch.int8": KV_INT8}.get(_dtype(k_pool)[0])
+        if fmt is None or k_pool.dtype != v_pool.dtype or k_pool.shape != v_pool.shape:
+            raise TypeError("KvLayer: two float16 or two int8 pools of one shape")
+        scales = [x for x in (k_scale, v_scale) if x is not None]
+        if len(scales) != (2 if fmt == KV_INT8 else 0):
+            raise ValueError("KvLayer: an int8 pool comes with its scales, a float16 pool with none")
+        for x in scales:
+            if _dtype(x)[0] != "torch.float16" or tuple(x.shape) != (pages, n_head_kv, page_size, head_dim // 64):
+                raise TypeError("KvLayer: scales are float16, [page][kv_head][cell][head_dim / 64]")
+        for x in (k_pool, v_pool, *scales):
+            if not x.is_contiguous() or not x.is_cuda:
+                raise ValueError("KvLayer: pools and scales must be contiguous and on the GPU")
+        self._init(k_pool, v_pool, k_scale, v_scale, page_tables, pages, n_head_kv, head_dim, page_size, fmt)
+
+    def _init(self, k, v, k_scale, v_scale, tables, limit, n_head_kv, head_dim, page_size, fmt):
+        if _dtype(tables)[0] != "torch.int32" or tables.dim() != 2 or not tables.is_cuda or (tables.shape[1] > 1 and tables.stride(1) != 1):
+            raise TypeError("KvLayer: page tables are int32, [sequence][page], on the GPU, the pages of a row contiguous")
+        n_tables, width = tables.shape
+        step = tables.stride(0) if n_tables > 1 else width
+        if step < width:
+            raise ValueError("KvLayer: the rows of the page tables overlap")
+        self.tensors = (k, v, k_scale, v_scale, tables)
+        self.n_head_kv, self.head_dim, self.n_tables = n_head_kv, head_dim, n_tables
+        self.args = KvLayerArgs(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), tables.data_ptr(), step, limit, n_tables,
+                                n_head_kv, head_dim, page_size, fmt, 0)
+        self.at = C.addressof(self.args)
+
+    @classmethod
+    def of_pool(cls, g: KvGeometry, pool: Pool, page_tables) -> "KvLayer":
+        """A layer held in a block pool: `page_tables` are the K tables (layer_page_tables) of its sequences; the V page
+        of a slot lies pages_per_block pages behind its K page."""
+        self = cls.__new__(cls)
+        shift = g.pages_per_block
+        self._init(pool.base, pool.base + shift * g.page_bytes, None, None, page_tables,
+                   pool.n_blocks * g.slot_pages - shift, g.n_head_kv, g.head_dim, PAGE_CELLS, KV_F16)
+        self.pool = pool
+        return self
+
+
+def kv_append(layer: KvLayer, k, v, lengths, *, seq_starts=None, q=None, q_out=None, inv_freq=None,
+              rope_style: str = "half", rope_scale: float = 1.0, lengths_out=None, stream=None) -> None:
+    """Write the K and V rows of new tokens ([token][kv_head][head_dim]) into cells lengths[s], lengths[s]+1, ... of
+    their sequences, K rotated by its cell's number, and q rotated into q_out (skv_kv_append)."""
+    kp, n, kv, dim, ks = _rows(k, "k")
+    vp, vn, vkv, vdim, vs = _rows(v, "v", k)
+    if (vn, vkv, vdim) != (n, kv, dim) or kv != layer.n_head_kv or dim != layer.head_dim:
+        raise ValueError("kv_append: k and v are [token][kv_head][head_dim] of the layer")
+    n_seqs = n if seq_starts is None else seq_starts.shape[0] - 1
+    qp = qo = None
+    qs = qos = heads = 0
+    if (q is None) != (q_out is None):
+        raise ValueError("kv_append: q and q_out come together")
+    if q is not None:
+        qp, qn, heads, qd, qs = _rows(q, "q", k)
+        qo, on, oh, od, qos = _rows(q_out, "q_out", k)
+        if (qn, qd) != (n, dim) or (on, oh, od) != (qn, heads, qd):
+            raise ValueError("kv_append: q and q_out are [token][head][head_dim]")
+    args = AppendArgs(kp, vp, ks, vs, qp, qo, qs, qos, _vector(seq_starts, "seq_starts", "torch.int32", 1),
+                      _vector(lengths, "lengths", "torch.int32", n_seqs),
+                      _vector(lengths_out, "lengths_out", "torch.int32", n_seqs), _vector(inv_freq, "inv_freq", "torch.float32", 0),
+                      n, n_seqs, heads, 0 if inv_freq is None else 2 * inv_freq.shape[0], ROPE_STYLES[rope_style], _dtype(k)[1],
+                      rope_scale, 0)
+    check(lib().skv_kv_append(layer.at, C.addressof(args), _stream(stream)))
+
+
+def decode_attention_workspace(layer: KvLayer, n_seqs: int, n_head: int) -> int:
+    """Bytes of device memory that decode_attention needs beside its tensors."""
+    out = C.c_uint64()
+    check(lib().skv_decode_attention_workspace(layer.at, n_seqs, n_head, C.byref(out)))
+    return out.value
+
+
+def decode_attention(layer: KvLayer, q, lengths, out, *, workspace, scale: float | None = None, lse=None, stream=None) -> None:
+    """out = softmax(scale * q K^T) V of one new token per sequence ([sequence][head][head_dim]) over the first
+    lengths[s] cells of its cache (skv_decode_attention).  scale: head_dim ** -0.5 when None."""
+    qp, n, heads, dim, qs = _rows(q, "q")
+    op, on, oh, od, os_ = _rows(out, "out", q)
+    if (on, oh, od) != (n, heads, dim) or dim != layer.head_dim:
+        raise ValueError("decode_attention: q and out are [sequence][head][head_dim] of the layer")
+    if lse is not None and (_dtype(lse)[0] != "torch.float32" or tuple(lse.shape) != (n, heads) or not lse.is_contiguous() or not lse.is_cuda):
+        raise TypeError("decode_attention: lse is a contiguous float32 [sequence][head] tensor on the GPU")
+    args = AttentionArgs(qp, op, qs, os_, _ptr(lse), _vector(lengths, "lengths", "torch.int32", n), _ptr(workspace),
+                         workspace.numel() * workspace.element_size(), n, heads, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
+    check(lib().skv_decode_attention(layer.at, C.addressof(args), _stream(stream)))
+
+
+def gated_delta_workspace(n_tokens: int, n_seqs: int, n_v_heads: int, head_dim: int, max_tokens: int) -> int:
+    """Bytes of device memory that gated_delta needs beside its tensors (0 where every sequence is short)."""
+    out = C.c_uint64()
+    check(lib().skv_gated_delta_workspace(n_tokens, n_seqs, n_v_heads, head_dim, max_tokens, C.byref(out)))
+    return out.value
+
+
+def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=None, max_tokens: int | None = None,
+                scale: float | None = None, workspace=None, stream=None) -> None:
+    """The gated delta rule over packed sequences (skv_gated_delta): q, k [token][k_head][dim], v, out
+    [token][v_head][dim], g, beta float32 [token][v_head], state float32 [row][v_head][dim key][dim value], updated in
+    place.  max_tokens bounds the tokens of one sequence (all of them when None).  scale: dim ** -0.5 when None."""
+    qp, n, kh, dim, qs = _rows(q, "q")
+    kp, kn, kkh, kd, ks = _rows(k, "k", q)
+    vp, vn, vh, vd, vs = _rows(v, "v", q)
+    op, on, oh, od, os_ = _rows(out, "out", q)
+    if (kn, kkh, kd) != (n, kh, dim) or (vn, vd) != (n, dim) or (on, oh, od) != (n, vh, dim):
+        raise ValueError("gated_delta: q and k are [token][k_head][dim], v and out [token][v_head][dim]")
+    for x, what in ((g, "g"), (beta, "beta")):
+        if _dtype(x)[0] != "torch.float32" or tuple(x.shape) != (n, vh) or (vh > 1 and n and x.stride(1) != 1) or not x.is_cuda:
+            raise TypeError(f"gated_delta: {what} is a float32 [token][v_head] tensor on the GPU")
+    rows = state.shape[0]
+    if (_dtype(state)[0] != "torch.float32" or tuple(state.shape[1:]) != (vh, dim, dim) or not state.is_cuda
+            or (rows and not state[0].is_contiguous())):
+        raise TypeError("gated_delta: state is float32 [row][v_head][dim][dim] on the GPU, each row contiguous")
+    n_seqs = n if seq_starts is None else seq_starts.shape[0] - 1
+    if max_tokens is None:
+        max_tokens = 1 if seq_starts is None else n
+    args = GatedDeltaArgs(qp, kp, vp, op, qs, ks, vs, os_, g.data_ptr(), beta.data_ptr(), g.stride(0) if n > 1 else vh,
+                          beta.stride(0) if n > 1 else vh, state.data_ptr(), state.stride(0) if rows > 1 else vh * dim * dim, rows,
+                          _vector(state_index, "state_index", "torch.int32", n_seqs),
+                          _vector(seq_starts, "seq_starts", "torch.int32", 1), _ptr(workspace),
+                          0 if workspace is None else workspace.numel() * workspace.element_size(), n, n_seqs, kh, vh, dim,
+                          max_tokens, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
+    check(lib().skv_gated_delta(C.addressof(args), _stream(stream)))

@@ -1,0 +1,136 @@
+"""The operators' refusals and their binding, without a GPU: every bad call ends before anything reaches a device."""
+import ctypes as C
+
+import pytest
+
+import skv
+
+P = 0x10000     # a 256-byte aligned address that is never followed
+
+
+def layer(**kw):
+    base = dict(k_pool=P, v_pool=P, page_tables=P, table_stride=8, page_limit=64, n_tables=4, n_head_kv=2, head_dim=256,
+                page_size=4, format=skv.KV_F16)
+    return skv.KvLayerArgs(**{**base, **kw})
+
+
+def append(**kw):
+    base = dict(k=P, v=P, k_stride=512, v_stride=512, q=P, q_out=P, q_stride=6144, q_out_stride=6144, lengths=P, inv_freq=P,
+                n_tokens=4, n_seqs=4, n_head=24, n_rot=64, rope_style=0, dtype=0, rope_scale=1.0)
+    return skv.AppendArgs(**{**base, **kw})
+
+
+def attention(**kw):
+    base = dict(q=P, out=P, q_stride=6144, out_stride=6144, lengths=P, workspace=P, workspace_bytes=1 << 40, n_seqs=4,
+                n_head=24, dtype=0, scale=0.0625)
+    return skv.AttentionArgs(**{**base, **kw})
+
+
+def delta(**kw):
+    base = dict(q=P, k=P, v=P, out=P, q_stride=2048, k_stride=2048, v_stride=4096, out_stride=4096, g=P, beta=P, g_stride=32,
+                beta_stride=32, state=P, state_stride=32 * 128 * 128, state_rows=4, workspace=P, workspace_bytes=1 << 40,
+                n_tokens=4, n_seqs=4, n_k_heads=16, n_v_heads=32, head_dim=128, max_tokens=1, dtype=1, scale=0.1)
+    return skv.GatedDeltaArgs(**{**base, **kw})
+
+
+def refused(rc, text):
+    assert rc == skv.EINVAL, (rc, skv.lib().skv_last_error())
+    assert text in skv.lib().skv_last_error().decode()
+
+
+BAD_LAYERS = [
+    (dict(head_dim=96), "head_dim"), (dict(page_size=3), "page_size"), (dict(page_size=512), "page_size"), (dict(page_size=0), "page_size"),
+    (dict(n_head_kv=0), "n_head_kv"), (dict(k_pool=None), "missing pool"), (dict(v_pool=None), "missing pool"),
+    (dict(page_tables=None), "missing pool"), (dict(v_pool=P + 8), "16-byte"), (dict(format=2), "format"),
+    (dict(format=skv.KV_INT8), "scales"), (dict(format=skv.KV_INT8, k_scale=P, v_scale=P + 4), "8-byte"),
+    (dict(page_limit=0), "page_limit"), (dict(page_limit=1 << 31), "page_limit"), (dict(table_stride=0), "table_stride"),
+    (dict(n_tables=3), "page tables"), (dict(page_tables=P + 2), "4-byte"),
+]
+
+
+@pytest.mark.parametrize("bad,text", BAD_LAYERS)
+def test_a_layer_that_cannot_be_addressed_is_refused(bad, text):
+    L = skv.lib()
+    refused(L.skv_kv_append(C.byref(layer(**bad)), C.byref(append()), None), text)
+    refused(L.skv_decode_attention(C.byref(layer(**bad)), C.byref(attention()), None), text)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(n_tokens=-1), "negative"), (dict(n_seqs=-1), "negative"), (dict(k=None), "missing"), (dict(v=None), "missing"),
+    (dict(k=P + 2), "16-byte"), (dict(v_stride=516), "multiples of 8"), (dict(k_stride=256), "shorter"), (dict(lengths=None), "lengths"),
+    (dict(n_tokens=5), "one row"), (dict(lengths_out=P), "lengths_out"), (dict(dtype=2), "dtype"), (dict(rope_style=2), "style"),
+    (dict(n_rot=24), "n_rot"), (dict(n_rot=272), "n_rot"), (dict(n_rot=-16), "n_rot"), (dict(inv_freq=None), "inv_freq"),
+    (dict(q=None), "together"), (dict(q_out=None), "together"), (dict(n_head=0), "n_head"), (dict(q_stride=4096), "shorter"),
+    (dict(q_out=P + 4), "16-byte"), (dict(q_stride=8192), "in place"),
+])
+def test_append_refuses(bad, text):
+    refused(skv.lib().skv_kv_append(C.byref(layer()), C.byref(append(**bad)), None), text)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(n_seqs=-1), "n_seqs"), (dict(n_head=0), "n_head"), (dict(n_head=25), "multiple"), (dict(dtype=7), "dtype"),
+    (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(q=None), "missing"), (dict(out=None), "missing"),
+    (dict(lengths=None), "missing"), (dict(q=P + 8), "16-byte"), (dict(out_stride=6148), "multiples of 8"),
+    (dict(out_stride=2048), "shorter"), (dict(workspace=None), "workspace"), (dict(workspace=P + 16), "workspace"),
+    (dict(workspace_bytes=0), "workspace"),
+])
+def test_attention_refuses(bad, text):
+    refused(skv.lib().skv_decode_attention(C.byref(layer()), C.byref(attention(**bad)), None), text)
+
+
+@pytest.mark.parametrize("bad,text", [
+    (dict(n_tokens=-1), "negative"), (dict(head_dim=96), "head_dim"), (dict(n_k_heads=0), "multiple"), (dict(n_v_heads=24), "multiple"),
+    (dict(dtype=2), "dtype"), (dict(scale=float("nan")), "finite"), (dict(n_tokens=3), "one token"), (dict(max_tokens=-1), "negative"),
+    (dict(q=None), "missing"), (dict(state=None), "missing"), (dict(g=None), "missing"), (dict(v=P + 8), "16-byte"),
+    (dict(state=P + 4), "16-byte"), (dict(out_stride=4100), "multiples"), (dict(state_stride=32 * 128 * 128 + 2), "multiples"),
+    (dict(k_stride=1024), "shorter"), (dict(state_stride=128), "overlap"), (dict(state_rows=0), "none"), (dict(state_rows=3), "fewer"),
+])
+def test_delta_refuses(bad, text):
+    refused(skv.lib().skv_gated_delta(C.byref(delta(**bad)), None), text)
+
+
+def test_no_arguments_and_nothing_to_do():
+    L = skv.lib()
+    refused(L.skv_kv_append(None, C.byref(append()), None), "no layer")
+    refused(L.skv_kv_append(C.byref(layer()), None, None), "no arguments")
+    refused(L.skv_decode_attention(None, C.byref(attention()), None), "no layer")
+    refused(L.skv_decode_attention(C.byref(layer()), None, None), "no arguments")
+    refused(L.skv_gated_delta(None, None), "no arguments")
+    assert L.skv_kv_append(C.byref(layer()), C.byref(append(n_seqs=0, n_tokens=0)), None) == skv.OK
+    assert L.skv_decode_attention(C.byref(layer()), C.byref(attention(n_seqs=0)), None) == skv.OK
+    assert L.skv_gated_delta(C.byref(delta(n_seqs=0, n_tokens=0)), None) == skv.OK
+    assert L.skv_gated_delta(C.byref(delta(max_tokens=0)), None) == skv.OK
+
+
+def test_workspace_sizes():
+    L, out = skv.lib(), C.c_uint64(7)
+    assert L.skv_decode_attention_workspace(C.byref(layer()), 4, 24, C.byref(out)) == skv.OK and out.value % 256 == 0
+    refused(L.skv_decode_attention_workspace(C.byref(layer()), 4, 24, None), "null output")
+    refused(L.skv_decode_attention_workspace(C.byref(layer()), 4, 0, C.byref(out)), "bad counts")
+    assert L.skv_gated_delta_workspace(100, 3, 32, 128, 50, C.byref(out)) == skv.OK and out.value % 256 == 0
+    refused(L.skv_gated_delta_workspace(100, 3, 32, 100, 50, C.byref(out)), "bad sizes")
+    refused(L.skv_gated_delta_workspace(-1, 3, 32, 128, 50, C.byref(out)), "bad sizes")
+
+
+def test_the_binding_refuses_tensors_that_do_not_fit():
+    """CPU tensors, wrong types, shapes and layouts never reach the library."""
+    torch = pytest.importorskip("torch")
+    pool = torch.zeros(8, 2, 4, 256, dtype=torch.float16)
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="on the GPU"):
+        skv.KvLayer(pool, pool.clone(), table)
+    with pytest.raises(TypeError, match="float16 or two int8"):
+        skv.KvLayer(pool.float(), pool.float(), table)
+    with pytest.raises(ValueError, match="scales"):
+        skv.KvLayer(pool.to(torch.int8), pool.to(torch.int8), table)
+    x = torch.zeros(1, 2, 256, dtype=torch.float16)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        skv._rows(x, "q")
+    with pytest.raises(TypeError, match="float16"):
+        skv._rows(x.float(), "q")
+    with pytest.raises(TypeError, match="all"):
+        skv._rows(x, "q", x.bfloat16())
+    with pytest.raises(ValueError, match="back to back"):
+        skv._rows(x.transpose(1, 2), "q")
+    with pytest.raises(TypeError, match="int32"):
+        skv._vector(torch.zeros(3), "lengths", "torch.int32", 3)
