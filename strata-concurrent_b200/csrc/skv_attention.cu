@@ -2,109 +2,696 @@
 //
 //   s_t = scale * q . k_t;   m = max s_t;   out = sum e^(s_t - m) v_t / sum e^(s_t - m);   lse = m + ln sum
 //
-// One CTA per (query head, sequence): each warp walks every eighth cell with a running maximum and sum, holding
-// head_dim / 32 values of q and of the output per lane, and the warps' parts are joined through shared memory.
+// The cache is read once, so its bytes bound the operator, and everything else has to fit beside the stream: the products
+// go through the tensor cores (the up to 16 query heads that share a K/V head are the 16 rows of an m16n8k16 product, as
+// 12 of them on CUDA cores would take 12 flops per byte, more than the cores have at this bandwidth).
+//
+// Split.  The work is the tiles of all (sequence, K/V head) items laid end to end; one CTA per SM takes an equal,
+// contiguous share of them, worked out from the lengths on the device.  So one long sequence and many ragged ones load
+// the GPU alike.  An item that lies inside one share is finished there; an item cut by a share's border leaves parts
+// (its unnormalised output, maximum and sum) that join_kernel adds up in a fixed order.
+//
+// A tile is 32 KiB of K and as much of V (64 cells of 256 fp16 values): three stages fill the shared memory and keep at
+// least 64 KiB per SM in flight, twice what bandwidth x latency asks for.  Each warp copies (16-byte cp.async, chunks
+// swizzled by the row so that ldmatrix meets no bank twice), then scores, its own eighth of the cells; the warps
+// exchange row maxima and weights through shared memory and each multiplies all weights with its own eighth of V's
+// columns.  So no warp holds an output that another has to add, and a tile costs two barriers.
+//
+// Precision.  fp16 queries and cache values meet in exact products, summed in 32 bits.  A bfloat16 query row is scaled by a
+// power of two to below 2 and becomes fp16 without loss, up to values 2^-24 of its largest.  Weights are rounded to fp16
+// for the product with V (2^-11 each; they are scaled by 2^15, so a weight is a normal number down to 2^-29 of the
+// largest), their sum is taken before that rounding.  int8 codes are exact in fp16; K's scales are applied to the 32-bit
+// sums of their 64 values, V's to the weights before they are rounded, under a running power of two per group.
 #include "skv_ops.h"
 
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 namespace skv {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;        // query heads per item: the rows of one matrix product
+constexpr int kStages = 3;
+constexpr int kMaxCtas = 192;    // shares at most; the grid is one CTA per SM
 
 struct AttnDev {
     LayerDev layer;
     skv_attention_args a;
     uint32_t* status;
-    int group;
+    int group;      // query heads per K/V head
+    int blocks;     // items per (sequence, K/V head): group / 16, rounded up
+    float* part_o;  // [share][2][16][dim]
+    float2* part_ml;// [share][2][16]: maximum (of base-2 exponents) and sum
+    int2* cut;      // [share]: the item whose first part is this share's second (-1: none), and its parts
 };
 
-template <typename T, int kDim, bool kInt8>
-__global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_constant__ AttnDev p) {
-    constexpr int kPer = kDim / 32;
-    const skv_attention_args& a = p.a;
-    const int head = blockIdx.x, seq = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t table_cells = p.layer.table_stride << p.layer.page_shift;
-    const int asked = __ldg(a.lengths + seq);
-    const int64_t n = asked < 0 ? 0 : asked > table_cells ? table_cells : asked;
-    if ((asked < 0 || asked > table_cells) && threadIdx.x == 0) atomicOr(p.status, SKV_STATUS_BAD_SRC_PAGE);
-    float q[kPer], o[kPer], m = -INFINITY, sum = 0.0f;
-    const T* qr = static_cast<const T*>(a.q) + seq * a.q_stride + head * kDim + lane * kPer;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        q[i] = (float) qr[i] * a.scale;
-        o[i] = 0.0f;
-    }
-    for (int64_t t = warp; t < n; t += kWarps) {
-        const int64_t row = cell_row(p.layer, seq, t, head / p.group);
-        if (row < 0) {
-            if (lane == 0) atomicOr(p.status, SKV_STATUS_BAD_SRC_PAGE);
-            continue;
-        }
-        float k[kPer], v[kPer];
-        if (kInt8) {
-            const int g = lane * kPer / kInt8Group;
-            const float ks = __half2float(p.layer.k_scale[row * (kDim / kInt8Group) + g]);
-            const float vs = __half2float(p.layer.v_scale[row * (kDim / kInt8Group) + g]);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                k[i] = ks * (float) reinterpret_cast<const int8_t*>(p.layer.k)[row * kDim + lane * kPer + i];
-                v[i] = vs * (float) reinterpret_cast<const int8_t*>(p.layer.v)[row * kDim + lane * kPer + i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                k[i] = __half2float(reinterpret_cast<const __half*>(p.layer.k)[row * kDim + lane * kPer + i]);
-                v[i] = __half2float(reinterpret_cast<const __half*>(p.layer.v)[row * kDim + lane * kPer + i]);
-            }
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) s = fmaf(q[i], k[i], s);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (s == -INFINITY) continue;   // a weight of zero, and no maximum to take a difference from
-        const float top = fmaxf(m, s), keep = expf(m - top), w = expf(s - top);
-        sum = sum * keep + w;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) o[i] = o[i] * keep + w * v[i];
-        m = top;
-    }
-    __shared__ float s_m[kWarps], s_sum[kWarps], s_o[kWarps][kDim];
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_sum[warp] = sum;
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) s_o[warp][lane * kPer + i] = o[i];
-    __syncthreads();
-    float top = -INFINITY, total = 0.0f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w]);
-    for (int w = 0; w < kWarps; ++w) total += s_sum[w] != 0.0f ? s_sum[w] * expf(s_m[w] - top) : 0.0f;
-    if (threadIdx.x < kDim) {
-        float x = 0.0f;
-        for (int w = 0; w < kWarps; ++w)
-            if (s_sum[w] != 0.0f) x += s_o[w][threadIdx.x] * expf(s_m[w] - top);
-        static_cast<T*>(a.out)[seq * a.out_stride + head * kDim + threadIdx.x] = Pair<T>::one(total != 0.0f ? x / total : 0.0f);
-    }
-    if (a.lse && threadIdx.x == 0) a.lse[(int64_t) seq * a.n_head + head] = total != 0.0f ? top + logf(total) : -INFINITY;
+template <int kDim, bool kInt8>
+struct Geo {
+    static constexpr int kRowBytes = kDim * (kInt8 ? 1 : 2);
+    static constexpr int kTile = 32768 / kRowBytes < 256 ? 32768 / kRowBytes : 256;   // cells per tile
+    static constexpr int kCells = kTile / kWarps;                                     // per warp
+    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kGroups = kInt8 ? kDim / kInt8Group : 1;
+    static constexpr int kScaleBytes = kInt8 ? (kGroups * 2 < 4 ? 4 : kGroups * 2) : 0;
+    static constexpr int kPlane = kTile * kRowBytes;
+    static constexpr int kStageBytes = 2 * kPlane + 2 * kTile * kScaleBytes;
+    static constexpr int kWeightStride = kTile + 8;   // halves: rows 16 bytes apart modulo 128, ldmatrix meets no bank twice
+    static constexpr int kWeightBytes = kGroups * kRows * kWeightStride * 2;
+    static constexpr int kSmem = kStages * kStageBytes + kWeightBytes;
+    static constexpr int kCols = kDim / kWarps;       // of the output, per warp
+    static constexpr int kOutTiles = kCols / 8;
+};
+
+// ---------------------------------------------------------------- small pieces
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool on) {   // off: zeros, nothing is read
+    if constexpr (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(on ? kBytes : 0) : "memory");
+}
+__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void wait_async() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+/// c += a b, 16 x 8 x 16 in fp16 with 32-bit sums.
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+/// Two of four signed codes as fp16, exactly: the byte u = code + 128 under the exponent of 1024 is 1024 + u.
+template <uint32_t kPick>
+__device__ __forceinline__ uint32_t codes_to_half(uint32_t biased) {
+    const uint32_t w = __byte_perm(biased, 0x64646464u, kPick);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x6480)));   // 1152
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float power_of_two(int e) {   // e clamped to the normal numbers
+    return __int_as_float((min(max(e, -126), 127) + 127) << 23);
+}
+/// The 16-byte chunk `chunk` of row `row` of a tile, swizzled so that eight rows' equal chunks lie in eight bank groups.
+template <int kChunks>
+__device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
+    return (uint32_t) (row * kChunks + (kChunks >= 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3))) * 16u;
 }
 
+/// The cells of a sequence that are attended.
+__device__ __forceinline__ int64_t cells_of(const AttnDev& p, int seq) {
+    const int64_t table = p.layer.table_stride << p.layer.page_shift;
+    const int n = __ldg(p.a.lengths + seq);
+    return n < 0 ? 0 : n > table ? table : n;
+}
+
+/// Sum over the CTA; every thread calls it.
+__device__ __forceinline__ int64_t cta_sum(int64_t v, int64_t* scratch) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    int64_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += scratch[w];
+    __syncthreads();
+    return sum;
+}
+
+/// A place in the sequence of all tiles.
+struct Cursor {
+    int seq, item;        // item: the K/V head and block of heads within the sequence
+    int tile, tiles;      // of the sequence
+    int64_t cells;
+};
+template <int kTile>
+__device__ __forceinline__ void step(Cursor& c, const AttnDev& p, int items) {
+    if (++c.tile < c.tiles) return;
+    c.tile = 0;
+    if (++c.item < items) return;
+    c.item = 0;
+    do {
+        if (++c.seq >= p.a.n_seqs) return;   // the last share's end
+        c.cells = cells_of(p, c.seq);
+    } while (c.cells == 0);
+    c.tiles = (int) ((c.cells + kTile - 1) / kTile);
+}
+
+// ---------------------------------------------------------------- the kernel
+
+template <typename T, int kDim, bool kInt8>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttnDev p) {
+    using G = Geo<kDim, kInt8>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float s_top[kWarps][kRows], s_sum[kWarps][kRows];
+    __shared__ int s_power[kWarps][4];
+    __shared__ uint32_t s_mask[kStages][kWarps];
+    __shared__ int64_t s_scan[kWarps];
+    __shared__ int64_t s_first[2];   // the first sequence of the share, and the tiles before it
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+    const int items = p.layer.n_head_kv * p.blocks, n_seqs = p.a.n_seqs;
+    const skv_attention_args& a = p.a;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- the share: tiles [from, to) of all
+    int64_t mine = 0;
+    for (int s = tid; s < n_seqs; s += kThreads) mine += (cells_of(p, s) + G::kTile - 1) / G::kTile;
+    const int64_t total = cta_sum(mine, s_scan) * items;
+    const int64_t shares = total < (int64_t) gridDim.x ? total : (int64_t) gridDim.x;
+    // sequences without cells
+    for (int s = blockIdx.x; s < n_seqs; s += gridDim.x) {
+        const int asked = __ldg(a.lengths + s);
+        if (tid == 0 && (asked < 0 || asked > (p.layer.table_stride << p.layer.page_shift))) atomicOr(p.status, SKV_STATUS_BAD_SRC_PAGE);
+        if (asked > 0) continue;
+        for (int i = tid; i < a.n_head * kDim / 8; i += kThreads)
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + s * a.out_stride + i * 8) = make_uint4(0, 0, 0, 0);
+        if (a.lse)
+            for (int i = tid; i < a.n_head; i += kThreads) a.lse[(int64_t) s * a.n_head + i] = -INFINITY;
+    }
+    if ((int64_t) blockIdx.x >= shares) {
+        if (tid == 0) p.cut[blockIdx.x] = make_int2(-1, 0);
+        return;
+    }
+    const int64_t from = total * blockIdx.x / shares, to = total * (blockIdx.x + 1) / shares;
+    {
+        // the sequence that holds tile `from`: a running sum over the sequences, 256 at a time
+        int64_t before = 0;
+        for (int base = 0; base < n_seqs; base += kThreads) {
+            const int s = base + tid;
+            const int64_t n = s < n_seqs ? (cells_of(p, s) + G::kTile - 1) / G::kTile * items : 0;
+            int64_t up = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, up, d);
+                if (lane >= d) up += o;
+            }
+            if (lane == 31) s_scan[warp] = up;
+            __syncthreads();
+            int64_t at = before;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) at += s_scan[w];
+                before += s_scan[w];
+            }
+            const int64_t end = at + up;
+            if (n && from >= end - n && from < end) {
+                s_first[0] = s;
+                s_first[1] = end - n;
+            }
+            __syncthreads();
+            if (from < before) break;
+        }
+    }
+    Cursor load;
+    load.seq = (int) s_first[0];
+    load.cells = cells_of(p, load.seq);
+    load.tiles = (int) ((load.cells + G::kTile - 1) / G::kTile);
+    load.item = (int) ((from - s_first[1]) / load.tiles);
+    load.tile = (int) ((from - s_first[1]) % load.tiles);
+    Cursor here = load;
+    const int64_t count = to - from;
+
+    // ---- loading: lane i of a warp finds the row of the warp's cell i, one tile ahead of the copies
+    static_assert(G::kCells <= 32, "a lane per cell");
+    int64_t row = -1;
+    bool inside = false;
+    auto find_rows = [&]() {
+        const int64_t cell = (int64_t) load.tile * G::kTile + warp * G::kCells + lane;
+        inside = lane < G::kCells && cell < load.cells;
+        row = inside ? cell_row(p.layer, load.seq, cell, load.item / p.blocks) : -1;
+    };
+    int64_t asked = 0;    // tiles whose copies were issued
+    int fill = 0;         // the stage that the next one fills
+    auto issue = [&]() {
+        if (asked < count) {
+            const int stage = fill;
+            fill = fill + 1 == kStages ? 0 : fill + 1;
+            uint8_t* base = smem + stage * G::kStageBytes;
+            if (inside && row < 0) atomicOr(p.status, SKV_STATUS_BAD_SRC_PAGE);
+            const uint32_t held = __ballot_sync(0xffffffffu, row >= 0);
+            if (lane == 0) s_mask[stage][warp] = held;
+            constexpr int kPer = 32 / G::kChunks;   // rows per trip of the warp
+            const uint32_t k_at = smem_at(base) + warp * G::kCells * G::kRowBytes, v_at = k_at + G::kPlane;
+#pragma unroll
+            for (int i = 0; i < G::kCells / kPer; ++i) {
+                const int r = i * kPer + lane / G::kChunks, chunk = lane % G::kChunks;
+                const int64_t from_row = __shfl_sync(0xffffffffu, row, r);
+                const bool on = from_row >= 0;
+                const int64_t byte = on ? from_row * G::kRowBytes + chunk * 16 : 0;
+                const uint32_t to_byte = chunk_at<G::kChunks>(r, chunk);   // a warp's first row is a multiple of 8
+                copy_async<16>(k_at + to_byte, p.layer.k + byte, on);
+                copy_async<16>(v_at + to_byte, p.layer.v + byte, on);
+            }
+            if constexpr (kInt8) {
+                // head_dim 64 has one two-byte scale per cell: the aligned word that holds it
+                if (lane < G::kCells) {
+                    const uint32_t s_at = smem_at(base) + 2 * G::kPlane + (warp * G::kCells + lane) * G::kScaleBytes;
+                    const int64_t byte = row >= 0 ? (row * G::kGroups * 2) & ~(int64_t) 3 : 0;
+                    copy_async<G::kScaleBytes>(s_at, reinterpret_cast<const uint8_t*>(p.layer.k_scale) + byte, row >= 0);
+                    copy_async<G::kScaleBytes>(s_at + G::kTile * G::kScaleBytes, reinterpret_cast<const uint8_t*>(p.layer.v_scale) + byte, row >= 0);
+                    // which half of the word (only head_dim 64 has two)
+                    if constexpr (kDim == 64) {
+                        const uint32_t odd = __ballot_sync(0xffffffffu, row & 1);
+                        if (lane == 0) s_power[warp][1 + stage] = (int) odd;
+                    }
+                }
+            }
+            step<G::kTile>(load, p, items);
+            ++asked;
+            if (asked < count) find_rows();
+        }
+        commit_async();   // a group per call, empty ones too: the count of groups stands for the count of tiles
+    };
+    find_rows();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue();
+
+    // ---- the item's query, 16 heads x kDim, as the left operands of all its products
+    uint32_t q[kDim / 16][4];
+    float factor[2];   // of rows g and g + 8: scale, log2 e, and the power of two the row was divided by
+    auto load_query = [&]() {
+        const int kv = here.item / p.blocks, first = (here.item % p.blocks) * kRows;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = first + g + h * 8;
+            const bool on = r < p.group;
+            const T* src = static_cast<const T*>(a.q) + (int64_t) here.seq * a.q_stride + (int64_t) (kv * p.group + (on ? r : 0)) * kDim;
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kDim / 16; ++i) {
+                // fp16 cache: values 2c, 2c+1 and 2c+8, 2c+9 of each 16, as ldmatrix hands out K's rows;
+                // int8: values 4c .. 4c+3, as a register of four codes holds them
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(src + i * 16);
+                q[i][h] = on ? w[kInt8 ? 2 * c : c] : 0u;
+                q[i][h + 2] = on ? w[kInt8 ? 2 * c + 1 : c + 4] : 0u;
+                if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+                    const float2 x = Pair<T>::up(q[i][h]), y = Pair<T>::up(q[i][h + 2]);
+                    top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+                }
+            }
+            int e = 0;
+            if constexpr (!std::is_same<T, __half>::value) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^-e in range for every finite row; a row with an infinity keeps it
+                e = top > 0.0f && top < INFINITY ? min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -126), 126) : 0;
+                const float down = power_of_two(-e);
+#pragma unroll
+                for (int i = 0; i < kDim / 16; ++i) {
+                    const float2 x = Pair<T>::up(q[i][h]), y = Pair<T>::up(q[i][h + 2]);
+                    q[i][h] = Pair<__half>::down(x.x * down, x.y * down);
+                    q[i][h + 2] = Pair<__half>::down(y.x * down, y.y * down);
+                }
+            }
+            factor[h] = a.scale * 1.4426950408889634f * power_of_two(e);
+        }
+    };
+    load_query();
+
+    float out[G::kOutTiles][4], top[2], sum[2];
+    int powers[G::kGroups];   // int8: the running power of two above V's scales, per group
+    auto clear = [&]() {
+#pragma unroll
+        for (int i = 0; i < G::kOutTiles; ++i) out[i][0] = out[i][1] = out[i][2] = out[i][3] = 0.0f;
+        top[0] = top[1] = -INFINITY;
+        sum[0] = sum[1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < G::kGroups; ++i) powers[i] = -24;
+    };
+    clear();
+    uint8_t* const weights = smem + kStages * G::kStageBytes;
+    int first_tile = here.tile;   // of the item, in this share
+
+    int stage = kStages - 1;
+    for (int64_t n = 0; n < count; ++n) {
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        const uint8_t* base = smem + stage * G::kStageBytes;
+        wait_async<kStages - 2>();
+        __syncwarp();
+
+        // ---- scores of the warp's cells: rows g, g + 8; cells 8 t + 2c, 2c + 1
+        constexpr int kTiles = G::kCells / 8;
+        float score[kTiles][4];
+        const uint32_t k_at = smem_at(base) + warp * G::kCells * G::kRowBytes;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            if constexpr (!kInt8) {
+                float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};   // two chains of sums
+#pragma unroll
+                for (int i = 0; i < kDim / 32; ++i) {
+                    uint32_t b[4];
+                    load_matrices(b, k_at + chunk_at<G::kChunks>(t * 8 + (lane & 7), i * 4 + (lane >> 3)));
+                    multiply(x, q[2 * i], b[0], b[1]);
+                    multiply(y, q[2 * i + 1], b[2], b[3]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) score[t][j] = x[j] + y[j];
+            } else {
+                score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.0f;
+                const int cell = t * 8 + 2 * c;
+                const uint8_t* s_at = base + 2 * G::kPlane + (warp * G::kCells + cell) * G::kScaleBytes;
+                const uint32_t odd = kDim == 64 ? (uint32_t) s_power[warp][1 + stage] : 0u;
+#pragma unroll
+                for (int i = 0; i < G::kGroups; ++i) {
+                    uint32_t b[4];
+                    load_matrices(b, k_at + chunk_at<G::kChunks>(t * 8 + (lane & 7), i * 4 + (lane >> 3)));
+                    float x[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t u = b[j] ^ 0x80808080u;
+                        multiply(x, q[4 * i + j], codes_to_half<0x4140>(u), codes_to_half<0x4342>(u));
+                    }
+                    const int h0 = kDim == 64 ? (odd >> cell) & 1 : i, h1 = kDim == 64 ? (odd >> (cell + 1)) & 1 : i;
+                    const float s0 = __half2float(reinterpret_cast<const __half*>(s_at)[h0]);
+                    const float s1 = __half2float(reinterpret_cast<const __half*>(s_at + G::kScaleBytes)[h1]);
+                    score[t][0] = fmaf(x[0], s0, score[t][0]);
+                    score[t][1] = fmaf(x[1], s1, score[t][1]);
+                    score[t][2] = fmaf(x[2], s0, score[t][2]);
+                    score[t][3] = fmaf(x[3], s1, score[t][3]);
+                }
+            }
+        }
+        const uint32_t held = s_mask[stage][warp];
+        float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool on = (held >> (t * 8 + 2 * c + (j & 1))) & 1u;
+                score[t][j] = on ? score[t][j] * factor[j >> 1] : -INFINITY;
+                most[j >> 1] = fmaxf(most[j >> 1], score[t][j]);   // fmaxf passes a NaN over; its weight is NaN all the same
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+            if (c == 0) s_top[warp][g + h * 8] = most[h];
+        }
+        if constexpr (kInt8) {
+            // the largest V scale of the warp's cells per group, as the power of two above it
+            const uint8_t* s_at = base + 2 * G::kPlane + (G::kTile + warp * G::kCells + (lane < G::kCells ? lane : 0)) * G::kScaleBytes;
+            const uint32_t odd = kDim == 64 ? (uint32_t) s_power[warp][1 + stage] : 0u;
+#pragma unroll
+            for (int i = 0; i < G::kGroups; ++i) {
+                const float s = fabsf(__half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd >> lane) & 1 : i]));
+                int e = s > 0.0f && lane < G::kCells ? ((__float_as_int(s) >> 23) & 0xff) - 126 : -24;
+                e = __reduce_max_sync(0xffffffffu, e);
+                if (lane == 0) s_power[warp][kDim == 64 ? 0 : i] = min(e, 17);
+            }
+        }
+        __syncthreads();   // row maxima; and every warp is done with the tile before, whose stage is filled again
+        issue();
+
+        float keep[2], now[2], shrink = 1.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float x = top[h];
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) x = fmaxf(x, s_top[w][g + h * 8]);
+            now[h] = x == -INFINITY ? 0.0f : x;   // nothing but minus infinity so far: any reference will do
+            keep[h] = exp2f(top[h] - now[h]);
+            top[h] = x;
+            sum[h] *= keep[h];
+        }
+        if constexpr (kInt8) {
+            // within an item a power only grows: what was summed under a smaller one is scaled down
+            const int mine = warp * G::kCols / kInt8Group;
+#pragma unroll
+            for (int i = 0; i < G::kGroups; ++i) {
+                int x = powers[i];
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) x = max(x, s_power[w][i]);
+                if (i == mine) shrink = power_of_two(powers[i] - x);
+                powers[i] = x;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int cell = warp * G::kCells + t * 8 + 2 * c;
+            float w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = exp2f(score[t][j] - now[j >> 1]);
+                sum[j >> 1] += w[j];
+                w[j] *= 32768.0f;
+            }
+            if constexpr (!kInt8) {
+                uint32_t* at = reinterpret_cast<uint32_t*>(weights + (g * G::kWeightStride + cell) * 2);
+                at[0] = Pair<__half>::down(w[0], w[1]);
+                at[8 * G::kWeightStride / 2] = Pair<__half>::down(w[2], w[3]);
+            } else {
+                const uint8_t* s_at = base + 2 * G::kPlane + (G::kTile + cell) * G::kScaleBytes;
+                const uint32_t odd = kDim == 64 ? (uint32_t) s_power[warp][1 + stage] : 0u;
+                const int in = t * 8 + 2 * c;
+#pragma unroll
+                for (int i = 0; i < G::kGroups; ++i) {
+                    const float down = power_of_two(-powers[i]);
+                    const float s0 = down * __half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd >> in) & 1 : i]);
+                    const float s1 = down * __half2float(reinterpret_cast<const __half*>(s_at + G::kScaleBytes)[kDim == 64 ? (odd >> (in + 1)) & 1 : i]);
+                    uint32_t* at = reinterpret_cast<uint32_t*>(weights + ((i * kRows + g) * G::kWeightStride + cell) * 2);
+                    at[0] = Pair<__half>::down(w[0] * s0, w[1] * s1);
+                    at[8 * G::kWeightStride / 2] = Pair<__half>::down(w[2] * s0, w[3] * s1);
+                }
+            }
+        }
+        __syncthreads();   // weights; and all of V has landed
+
+        // ---- output: all cells x the warp's columns
+#pragma unroll
+        for (int i = 0; i < G::kOutTiles; ++i) {
+            out[i][0] *= keep[0] * shrink;
+            out[i][1] *= keep[0] * shrink;
+            out[i][2] *= keep[1] * shrink;
+            out[i][3] *= keep[1] * shrink;
+        }
+        const int group = kInt8 ? warp * G::kCols / kInt8Group : 0;
+        const uint32_t w_at = smem_at(weights) + ((group * kRows + (lane & 15)) * G::kWeightStride + (lane >> 4) * 8) * 2;
+        const uint32_t v_at = smem_at(base) + G::kPlane;
+#pragma unroll
+        for (int k = 0; k < G::kTile / 32; ++k) {   // 32 cells: two products deep
+            uint32_t w0[4], w1[4];
+            load_matrices(w0, w_at + k * 64);
+            load_matrices(w1, w_at + k * 64 + 32);
+            if constexpr (kInt8) {
+                constexpr int kPieces = G::kCols >= 16 ? G::kCols / 16 : 1;
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    uint32_t b[4];
+                    load_matrices_t(b, v_at + chunk_at<G::kChunks>(k * 32 + lane, warp * G::kCols / 16 + j));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) b[i] ^= 0x80808080u;
+                    if constexpr (G::kCols >= 16) {   // even columns, odd columns
+                        multiply(out[2 * j], w0, codes_to_half<0x4240>(b[0]), codes_to_half<0x4240>(b[1]));
+                        multiply(out[2 * j + 1], w0, codes_to_half<0x4341>(b[0]), codes_to_half<0x4341>(b[1]));
+                        multiply(out[2 * j], w1, codes_to_half<0x4240>(b[2]), codes_to_half<0x4240>(b[3]));
+                        multiply(out[2 * j + 1], w1, codes_to_half<0x4341>(b[2]), codes_to_half<0x4341>(b[3]));
+                    } else if (warp & 1) {            // two warps share a chunk of 16 columns
+                        multiply(out[0], w0, codes_to_half<0x4341>(b[0]), codes_to_half<0x4341>(b[1]));
+                        multiply(out[0], w1, codes_to_half<0x4341>(b[2]), codes_to_half<0x4341>(b[3]));
+                    } else {
+                        multiply(out[0], w0, codes_to_half<0x4240>(b[0]), codes_to_half<0x4240>(b[1]));
+                        multiply(out[0], w1, codes_to_half<0x4240>(b[2]), codes_to_half<0x4240>(b[3]));
+                    }
+                }
+            } else if constexpr (G::kOutTiles >= 2) {
+#pragma unroll
+                for (int j = 0; j < G::kOutTiles / 2; ++j) {
+                    uint32_t b[4];
+                    const int chunk = warp * G::kOutTiles + j * 2 + (lane >> 4);
+                    load_matrices_t(b, v_at + chunk_at<G::kChunks>(k * 32 + (lane & 15), chunk));
+                    multiply(out[2 * j], w0, b[0], b[1]);
+                    multiply(out[2 * j + 1], w0, b[2], b[3]);
+                    load_matrices_t(b, v_at + chunk_at<G::kChunks>(k * 32 + 16 + (lane & 15), chunk));
+                    multiply(out[2 * j], w1, b[0], b[1]);
+                    multiply(out[2 * j + 1], w1, b[2], b[3]);
+                }
+            } else {
+                uint32_t b[4];
+                load_matrices_t(b, v_at + chunk_at<G::kChunks>(k * 32 + lane, warp));
+                multiply(out[0], w0, b[0], b[1]);
+                multiply(out[0], w1, b[2], b[3]);
+            }
+        }
+
+        // ---- the item's end, or the share's
+        if (here.tile + 1 == here.tiles || n + 1 == count) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+                if (c == 0) s_sum[warp][g + h * 8] = sum[h];
+            }
+            __syncthreads();
+            const bool whole = first_tile == 0 && here.tile + 1 == here.tiles;
+            const int slot = first_tile == 0 ? 1 : 0;
+            const int kv = here.item / p.blocks, first = (here.item % p.blocks) * kRows;
+            float fit = 1.0f / 32768.0f;
+            if constexpr (kInt8) {
+#pragma unroll
+                for (int i = 0; i < G::kGroups; ++i)
+                    if (i == group) fit *= power_of_two(powers[i]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = first + g + h * 8;
+                float l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) l += s_sum[w][g + h * 8];
+                if (r < p.group) {
+                    const int64_t head = (int64_t) kv * p.group + r;
+                    const float by = whole ? (l != 0.0f ? fit / l : 0.0f) : fit;
+                    T* to = static_cast<T*>(a.out) + (int64_t) here.seq * a.out_stride + head * kDim;
+                    float* part = p.part_o + (((int64_t) blockIdx.x * 2 + slot) * kRows + g + h * 8) * kDim;
+#pragma unroll
+                    for (int i = 0; i < G::kOutTiles; ++i) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            int d;
+                            if constexpr (!kInt8) d = warp * G::kCols + i * 8 + 2 * c + j;
+                            else if constexpr (G::kCols >= 16) d = warp * G::kCols + (i >> 1) * 16 + 4 * c + 2 * j + (i & 1);
+                            else d = (warp >> 1) * 16 + 4 * c + 2 * j + (warp & 1);
+                            // an empty row (nothing held, or minus infinity throughout) is zeros
+                            const float x = whole && l == 0.0f ? 0.0f : out[i][h * 2 + j] * by;
+                            if (whole) to[d] = Pair<T>::one(x);
+                            else part[d] = x;
+                        }
+                    }
+                    if (warp == 0 && c == 0) {
+                        if (!whole) p.part_ml[((int64_t) blockIdx.x * 2 + slot) * kRows + g + h * 8] = make_float2(top[h], l);
+                        else if (a.lse)
+                            a.lse[(int64_t) here.seq * a.n_head + head] = l != 0.0f ? (top[h] + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                    }
+                }
+            }
+            if (tid == 0 && n + 1 == count) {
+                const int64_t last = from + n + (here.tiles - 1 - here.tile);   // the item's last tile, and the share that has it
+                const int64_t holder = ((last + 1) * shares - 1) / total;
+                p.cut[blockIdx.x] = !whole && slot == 1 ? make_int2(here.seq * items + here.item, (int) (holder - blockIdx.x) + 1) : make_int2(-1, 0);
+            }
+            if (n + 1 < count) {
+                step<G::kTile>(here, p, items);
+                first_tile = 0;
+                clear();
+                load_query();
+            }
+        } else {
+            ++here.tile;
+        }
+    }
+    wait_async<0>();
+}
+
+/// Joins the parts of the item that share blockIdx.x began and others went on with, head by head (blockIdx.y): each part
+/// counts by 2^(its maximum - the largest), in the order of the shares.
 template <typename T, int kDim>
-void launch(const AttnDev& p, bool int8, cudaStream_t stream) {
-    const dim3 grid((unsigned) p.a.n_head, (unsigned) p.a.n_seqs);
-    if (int8) attention_kernel<T, kDim, true><<<grid, kThreads, 0, stream>>>(p);
-    else attention_kernel<T, kDim, false><<<grid, kThreads, 0, stream>>>(p);
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ AttnDev p) {
+    constexpr int kLanes = kDim / 4, kSets = kThreads / kLanes;
+    __shared__ float s_weight[kMaxCtas];
+    __shared__ float s_top[kWarps], s_sum[kWarps];
+    __shared__ float4 s_out[kSets][kLanes];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int2 cut = p.cut[blockIdx.x];
+    if (cut.x < 0) return;
+    const int items = p.layer.n_head_kv * p.blocks, seq = cut.x / items, item = cut.x % items;
+    const int kv = item / p.blocks, r = (item % p.blocks) * kRows + blockIdx.y;
+    if (r >= p.group) return;
+    const int tid = threadIdx.x, n = cut.y;
+    const auto place = [&](int i) { return (((int64_t) blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + blockIdx.y; };
+    const float2 ml = tid < n ? p.part_ml[place(tid)] : make_float2(-INFINITY, 0.0f);
+    float top = ml.x;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if ((tid & 31) == 0) s_top[tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
+    const float weight = exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+    if (tid < n) s_weight[tid] = weight;
+    float sum = weight * ml.y;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += s_sum[w];
+    const int lane = tid % kLanes, set = tid / kLanes;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+    for (int i = set; i < n; i += kSets) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + place(i) * kDim) + lane);
+        const float w = s_weight[i];
+        o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+    }
+    s_out[set][lane] = o;
+    __syncthreads();
+    const int64_t head = (int64_t) kv * p.group + r;
+    if (set == 0) {
+#pragma unroll
+        for (int i = 1; i < kSets; ++i) {
+            const float4 x = s_out[i][lane];
+            o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        }
+        const float by = 1.0f / sum;
+        if (sum == 0.0f) o = make_float4(0, 0, 0, 0);
+        else o = make_float4(o.x * by, o.y * by, o.z * by, o.w * by);
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + (int64_t) seq * p.a.out_stride + head * kDim + lane * 4) =
+            make_uint2(Pair<T>::down(o.x, o.y), Pair<T>::down(o.z, o.w));
+    }
+    if (tid == 0 && p.a.lse)
+        p.a.lse[(int64_t) seq * p.a.n_head + head] = sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <typename T, int kDim, bool kInt8>
+cudaError_t launch(const AttnDev& p, int ctas, cudaStream_t stream) {
+    constexpr int kSmem = Geo<kDim, kInt8>::kSmem;
+    static_assert(kSmem + 4096 <= 227 * 1024, "the stages fit an SM");
+    cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kDim, kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    attention_kernel<T, kDim, kInt8><<<ctas, kThreads, kSmem, stream>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // the join is resident, or next in line, when the last share ends; it waits for all of them before its first read
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned) ctas, (unsigned) (p.group < kRows ? p.group : kRows));
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, join_kernel<T, kDim>, p);
 }
 template <typename T>
-void launch(const AttnDev& p, int dim, bool int8, cudaStream_t stream) {
-    if (dim == 64) launch<T, 64>(p, int8, stream);
-    else if (dim == 128) launch<T, 128>(p, int8, stream);
-    else launch<T, 256>(p, int8, stream);
+cudaError_t launch(const AttnDev& p, int dim, bool int8, int ctas, cudaStream_t stream) {
+    if (dim == 64) return int8 ? launch<T, 64, true>(p, ctas, stream) : launch<T, 64, false>(p, ctas, stream);
+    if (dim == 128) return int8 ? launch<T, 128, true>(p, ctas, stream) : launch<T, 128, false>(p, ctas, stream);
+    return int8 ? launch<T, 256, true>(p, ctas, stream) : launch<T, 256, false>(p, ctas, stream);
 }
+
+/// The workspace: parts, their maxima and sums, the shares' cuts.
+struct Room {
+    size_t ml, cut, bytes;
+    explicit Room(int dim) {
+        ml = (size_t) kMaxCtas * 2 * kRows * dim * sizeof(float);
+        cut = ml + (size_t) kMaxCtas * 2 * kRows * sizeof(float2);
+        bytes = (cut + kMaxCtas * sizeof(int2) + 255) / 256 * 256;
+    }
+};
 
 }  // namespace
 }  // namespace skv
@@ -112,13 +699,12 @@ void launch(const AttnDev& p, int dim, bool int8, cudaStream_t stream) {
 using namespace skv;
 
 extern "C" {
-
 int skv_decode_attention_workspace(const skv_kv_layer* layer, int n_seqs, int n_head, uint64_t* out_bytes) {
     if (!out_bytes) return fail(SKV_EINVAL, "skv_decode_attention_workspace: null output");
     *out_bytes = 0;
     if (n_seqs < 0 || n_head < 1) return fail(SKV_EINVAL, "skv_decode_attention_workspace: bad counts");
     if (const int rc = check_layer(layer, n_seqs, "skv_decode_attention_workspace")) return rc;
-    *out_bytes = 256;
+    *out_bytes = Room(layer->head_dim).bytes;
     return SKV_OK;
 }
 
@@ -144,15 +730,21 @@ int skv_decode_attention(const skv_kv_layer* layer, const skv_attention_args* ar
     DeviceCtx* ctx = current_ctx();
     if (!ctx) return SKV_ECUDA;
     if (!ops_own_memory(layer->k_pool, ctx->device)) return no("the pool is not memory of the current device");
+    const Room room(layer->head_dim);
     AttnDev p{};
     p.layer = to_device(*layer);
     p.a = a;
     p.status = ctx->status;
     p.group = a.n_head / layer->n_head_kv;
+    p.blocks = (p.group + kRows - 1) / kRows;
+    p.part_o = static_cast<float*>(a.workspace);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.workspace) + room.ml);
+    p.cut = reinterpret_cast<int2*>(static_cast<uint8_t*>(a.workspace) + room.cut);
+    const int ctas = ctx->sms < kMaxCtas ? ctx->sms : kMaxCtas;
     const auto s = static_cast<cudaStream_t>(stream);
-    if (a.dtype == SKV_DTYPE_F16) launch<__half>(p, layer->head_dim, layer->format == SKV_KV_INT8, s);
-    else launch<__nv_bfloat16>(p, layer->head_dim, layer->format == SKV_KV_INT8, s);
-    const cudaError_t e = cudaGetLastError();
+    const bool int8 = layer->format == SKV_KV_INT8;
+    const cudaError_t e = a.dtype == SKV_DTYPE_F16 ? launch<__half>(p, layer->head_dim, int8, ctas, s)
+                                                   : launch<__nv_bfloat16>(p, layer->head_dim, int8, ctas, s);
     return e == cudaSuccess ? SKV_OK : cuda_fail(e, "skv_decode_attention");
 }
 
