@@ -31,11 +31,11 @@
 namespace skv {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;        // query heads per item: the rows of one matrix product
-constexpr int kStages = 3;
-constexpr int kMaxCtas = 192;    // shares at most; the grid is one CTA per SM
+constexpr int kMaxSms = 160;
+constexpr int kJoinThreads = 256;
 
 struct AttnDev {
     LayerDev layer;
@@ -51,16 +51,19 @@ struct AttnDev {
 template <int kDim, bool kInt8>
 struct Geo {
     static constexpr int kRowBytes = kDim * (kInt8 ? 1 : 2);
-    static constexpr int kTile = 32768 / kRowBytes < 256 ? 32768 / kRowBytes : 256;   // cells per tile
+    // cells per tile: a plane (K or V of a tile) of 32 KiB, at most a lane per cell of a warp; 96 where four sets of weights
+    // lie beside it
+    static constexpr int kTile = kInt8 && kDim == 256 ? 96 : 32768 / kRowBytes < 128 ? 32768 / kRowBytes : 128;
     static constexpr int kCells = kTile / kWarps;                                     // per warp
     static constexpr int kChunks = kRowBytes / 16;
     static constexpr int kGroups = kInt8 ? kDim / kInt8Group : 1;
     static constexpr int kScaleBytes = kInt8 ? (kGroups * 2 < 4 ? 4 : kGroups * 2) : 0;
     static constexpr int kPlane = kTile * kRowBytes;
-    static constexpr int kStageBytes = 2 * kPlane + 2 * kTile * kScaleBytes;
+    static constexpr int kSlotBytes = kPlane + kTile * kScaleBytes;
     static constexpr int kWeightStride = kTile + 8;   // halves: rows 16 bytes apart modulo 128, ldmatrix meets no bank twice
     static constexpr int kWeightBytes = kGroups * kRows * kWeightStride * 2;
-    static constexpr int kSmem = kStages * kStageBytes + kWeightBytes;
+    static constexpr int kSmem = 3 * kSlotBytes + kWeightBytes;   // K, and V twice
+    static constexpr int kPerSm = kPlane > 24000 ? 2 : kPlane > 12000 ? 3 : 4;   // CTAs: enough copies in flight
     static constexpr int kCols = kDim / kWarps;       // of the output, per warp
     static constexpr int kOutTiles = kCols / 8;
 };
@@ -152,12 +155,11 @@ __device__ __forceinline__ void step(Cursor& c, const AttnDev& p, int items) {
 // ---------------------------------------------------------------- the kernel
 
 template <typename T, int kDim, bool kInt8>
-__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttnDev p) {
+__global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_kernel(const __grid_constant__ AttnDev p) {
     using G = Geo<kDim, kInt8>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_top[kWarps][kRows], s_sum[kWarps][kRows];
-    __shared__ int s_power[kWarps][4];
-    __shared__ uint32_t s_mask[kStages][kWarps];
+    __shared__ int s_power[kWarps][4];   // int8: per V scale group
     __shared__ int64_t s_scan[kWarps];
     __shared__ int64_t s_first[2];   // the first sequence of the share, and the tiles before it
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     }
     const int64_t from = total * blockIdx.x / shares, to = total * (blockIdx.x + 1) / shares;
     {
-        // the sequence that holds tile `from`: a running sum over the sequences, 256 at a time
+        // the sequence that holds tile `from`: a running sum over the sequences, one per thread at a time
         int64_t before = 0;
         for (int base = 0; base < n_seqs; base += kThreads) {
             const int s = base + tid;
@@ -223,60 +225,63 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     Cursor here = load;
     const int64_t count = to - from;
 
-    // ---- loading: lane i of a warp finds the row of the warp's cell i, one tile ahead of the copies
-    static_assert(G::kCells <= 32, "a lane per cell");
-    int64_t row = -1;
-    bool inside = false;
-    auto find_rows = [&]() {
+    // ---- loading.  Lane i of a warp knows the warp's cell i; its table entry is read a tile before its copies are issued.
+    // A warp alone reads the K it copied, so the next tile's K follows as soon as it has its scores; V has two slots, and
+    // the next tile's follows once all warps have met after using the one before.
+    static_assert(G::kCells <= 32 && G::kCells % 8 == 0, "a lane per cell, whole 8-row matrices");
+    int entry = 0, within = -1;      // the next tile's table entry, and its cell's row within the page (-1: no cell)
+    auto find = [&]() {
         const int64_t cell = (int64_t) load.tile * G::kTile + warp * G::kCells + lane;
-        inside = lane < G::kCells && cell < load.cells;
-        row = inside ? cell_row(p.layer, load.seq, cell, load.item / p.blocks) : -1;
-    };
-    int64_t asked = 0;    // tiles whose copies were issued
-    int fill = 0;         // the stage that the next one fills
-    auto issue = [&]() {
-        if (asked < count) {
-            const int stage = fill;
-            fill = fill + 1 == kStages ? 0 : fill + 1;
-            uint8_t* base = smem + stage * G::kStageBytes;
-            if (inside && row < 0) atomicOr(p.status, SKV_STATUS_BAD_SRC_PAGE);
-            const uint32_t held = __ballot_sync(0xffffffffu, row >= 0);
-            if (lane == 0) s_mask[stage][warp] = held;
-            constexpr int kPer = 32 / G::kChunks;   // rows per trip of the warp
-            const uint32_t k_at = smem_at(base) + warp * G::kCells * G::kRowBytes, v_at = k_at + G::kPlane;
-#pragma unroll
-            for (int i = 0; i < G::kCells / kPer; ++i) {
-                const int r = i * kPer + lane / G::kChunks, chunk = lane % G::kChunks;
-                const int64_t from_row = __shfl_sync(0xffffffffu, row, r);
-                const bool on = from_row >= 0;
-                const int64_t byte = on ? from_row * G::kRowBytes + chunk * 16 : 0;
-                const uint32_t to_byte = chunk_at<G::kChunks>(r, chunk);   // a warp's first row is a multiple of 8
-                copy_async<16>(k_at + to_byte, p.layer.k + byte, on);
-                copy_async<16>(v_at + to_byte, p.layer.v + byte, on);
-            }
-            if constexpr (kInt8) {
-                // head_dim 64 has one two-byte scale per cell: the aligned word that holds it
-                if (lane < G::kCells) {
-                    const uint32_t s_at = smem_at(base) + 2 * G::kPlane + (warp * G::kCells + lane) * G::kScaleBytes;
-                    const int64_t byte = row >= 0 ? (row * G::kGroups * 2) & ~(int64_t) 3 : 0;
-                    copy_async<G::kScaleBytes>(s_at, reinterpret_cast<const uint8_t*>(p.layer.k_scale) + byte, row >= 0);
-                    copy_async<G::kScaleBytes>(s_at + G::kTile * G::kScaleBytes, reinterpret_cast<const uint8_t*>(p.layer.v_scale) + byte, row >= 0);
-                    // which half of the word (only head_dim 64 has two)
-                    if constexpr (kDim == 64) {
-                        const uint32_t odd = __ballot_sync(0xffffffffu, row & 1);
-                        if (lane == 0) s_power[warp][1 + stage] = (int) odd;
-                    }
-                }
-            }
-            step<G::kTile>(load, p, items);
-            ++asked;
-            if (asked < count) find_rows();
+        within = -1;
+        if (lane < G::kCells && cell < load.cells) {
+            within = ((load.item / p.blocks) << p.layer.page_shift) + (int) (cell & ((1 << p.layer.page_shift) - 1));
+            entry = __ldg(p.layer.tables + (int64_t) load.seq * p.layer.table_stride + (cell >> p.layer.page_shift));
         }
-        commit_async();   // a group per call, empty ones too: the count of groups stands for the count of tiles
     };
-    find_rows();
+    int64_t found = 0, row = -1;     // tiles found so far; the row of the tile whose K was issued last
+    uint32_t held = 0, odd = 0;      // of that tile: the cells that are there, the rows that are odd
+    auto copy_plane = [&](int slot, const uint8_t* pool, const __half* scales) {
+        constexpr int kPer = 32 / G::kChunks;   // rows per trip of the warp
+        const uint32_t base = smem_at(smem) + slot * G::kSlotBytes, to = base + warp * G::kCells * G::kRowBytes;
+        const int64_t byte = row < 0 ? -1 : row * G::kRowBytes;
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue();
+        for (int i = 0; i < G::kCells / kPer; ++i) {
+            const int r = i * kPer + lane / G::kChunks, chunk = lane % G::kChunks;
+            const int64_t from_byte = __shfl_sync(0xffffffffu, byte, r);
+            copy_async<16>(to + chunk_at<G::kChunks>(r, chunk), pool + (from_byte < 0 ? 0 : from_byte) + chunk * 16, from_byte >= 0);
+        }
+        if constexpr (kInt8) {
+            // head_dim 64 has one two-byte scale per cell: the aligned word that holds it
+            if (lane < G::kCells)
+                copy_async<G::kScaleBytes>(base + G::kPlane + (warp * G::kCells + lane) * G::kScaleBytes,
+                                           reinterpret_cast<const uint8_t*>(scales) + (row < 0 ? 0 : (row * G::kGroups * 2) & ~(int64_t) 3), row >= 0);
+        }
+    };
+    // the next tile's rows and K, and the entries of the tile after it
+    auto issue_k = [&]() {
+        held = 0;
+        if (found < count) {
+            const bool there = within >= 0 && entry >= 0 && entry < p.layer.page_limit;
+            if (within >= 0 && !there) atomicOr(p.status, SKV_STATUS_BAD_SRC_PAGE);
+            row = there ? (((int64_t) entry * p.layer.n_head_kv) << p.layer.page_shift) + within : -1;
+            held = __ballot_sync(0xffffffffu, there);
+            odd = __ballot_sync(0xffffffffu, row & 1);
+            copy_plane(0, p.layer.k, p.layer.k_scale);
+            ++found;
+            if (found < count) {
+                step<G::kTile>(load, p, items);
+                find();
+            }
+        }
+        commit_async();   // a group per call, empty ones too: the count of groups stands for the count of planes
+    };
+    auto issue_v = [&](int slot, bool on) {
+        if (on) copy_plane(slot, p.layer.v, p.layer.v_scale);
+        commit_async();
+    };
+    find();
+    issue_k();
+    issue_v(1, true);
 
     // ---- the item's query, 16 heads x kDim, as the left operands of all its products
     uint32_t q[kDim / 16][4];
@@ -331,20 +336,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         for (int i = 0; i < G::kGroups; ++i) powers[i] = -24;
     };
     clear();
-    uint8_t* const weights = smem + kStages * G::kStageBytes;
+    uint8_t* const weights = smem + 3 * G::kSlotBytes;
     int first_tile = here.tile;   // of the item, in this share
 
-    int stage = kStages - 1;
-    for (int64_t n = 0; n < count; ++n) {
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-        const uint8_t* base = smem + stage * G::kStageBytes;
-        wait_async<kStages - 2>();
+    int v_slot = 1;
+    for (int64_t n = 0; n < count; ++n, v_slot = 3 - v_slot) {
+        const uint8_t* const v_base = smem + v_slot * G::kSlotBytes;
+        const uint32_t held_now = held, odd_now = odd;
+        wait_async<1>();          // K of this tile
         __syncwarp();
 
         // ---- scores of the warp's cells: rows g, g + 8; cells 8 t + 2c, 2c + 1
         constexpr int kTiles = G::kCells / 8;
         float score[kTiles][4];
-        const uint32_t k_at = smem_at(base) + warp * G::kCells * G::kRowBytes;
+        const uint32_t k_at = smem_at(smem) + warp * G::kCells * G::kRowBytes;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
             if constexpr (!kInt8) {
@@ -361,8 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             } else {
                 score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.0f;
                 const int cell = t * 8 + 2 * c;
-                const uint8_t* s_at = base + 2 * G::kPlane + (warp * G::kCells + cell) * G::kScaleBytes;
-                const uint32_t odd = kDim == 64 ? (uint32_t) s_power[warp][1 + stage] : 0u;
+                const uint8_t* s_at = smem + G::kPlane + (warp * G::kCells + cell) * G::kScaleBytes;
 #pragma unroll
                 for (int i = 0; i < G::kGroups; ++i) {
                     uint32_t b[4];
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         const uint32_t u = b[j] ^ 0x80808080u;
                         multiply(x, q[4 * i + j], codes_to_half<0x4140>(u), codes_to_half<0x4342>(u));
                     }
-                    const int h0 = kDim == 64 ? (odd >> cell) & 1 : i, h1 = kDim == 64 ? (odd >> (cell + 1)) & 1 : i;
+                    const int h0 = kDim == 64 ? (odd_now >> cell) & 1 : i, h1 = kDim == 64 ? (odd_now >> (cell + 1)) & 1 : i;
                     const float s0 = __half2float(reinterpret_cast<const __half*>(s_at)[h0]);
                     const float s1 = __half2float(reinterpret_cast<const __half*>(s_at + G::kScaleBytes)[h1]);
                     score[t][0] = fmaf(x[0], s0, score[t][0]);
@@ -383,13 +387,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
             }
         }
-        const uint32_t held = s_mask[stage][warp];
+        __syncwarp();
+        issue_k();
         float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bool on = (held >> (t * 8 + 2 * c + (j & 1))) & 1u;
+                const bool on = (held_now >> (t * 8 + 2 * c + (j & 1))) & 1u;
                 score[t][j] = on ? score[t][j] * factor[j >> 1] : -INFINITY;
                 most[j >> 1] = fmaxf(most[j >> 1], score[t][j]);   // fmaxf passes a NaN over; its weight is NaN all the same
             }
@@ -402,18 +407,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         }
         if constexpr (kInt8) {
             // the largest V scale of the warp's cells per group, as the power of two above it
-            const uint8_t* s_at = base + 2 * G::kPlane + (G::kTile + warp * G::kCells + (lane < G::kCells ? lane : 0)) * G::kScaleBytes;
-            const uint32_t odd = kDim == 64 ? (uint32_t) s_power[warp][1 + stage] : 0u;
+            wait_async<1>();              // V of this tile
+            __syncwarp();
+            const uint8_t* s_at = v_base + G::kPlane + (warp * G::kCells + (lane < G::kCells ? lane : 0)) * G::kScaleBytes;
 #pragma unroll
             for (int i = 0; i < G::kGroups; ++i) {
-                const float s = fabsf(__half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd >> lane) & 1 : i]));
+                const float s = fabsf(__half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd_now >> lane) & 1 : i]));
                 int e = s > 0.0f && lane < G::kCells ? ((__float_as_int(s) >> 23) & 0xff) - 126 : -24;
                 e = __reduce_max_sync(0xffffffffu, e);
-                if (lane == 0) s_power[warp][kDim == 64 ? 0 : i] = min(e, 17);
+                if (lane == 0) s_power[warp][i] = min(e, 17);
             }
         }
-        __syncthreads();   // row maxima; and every warp is done with the tile before, whose stage is filled again
-        issue();
+        __syncthreads();   // row maxima; and every warp is done with V of the tile before, whose slot is filled again
+        issue_v(3 - v_slot, n + 1 < count);
 
         float keep[2], now[2], shrink = 1.0f;
 #pragma unroll
@@ -453,21 +459,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 at[0] = Pair<__half>::down(w[0], w[1]);
                 at[8 * G::kWeightStride / 2] = Pair<__half>::down(w[2], w[3]);
             } else {
-                const uint8_t* s_at = base + 2 * G::kPlane + (G::kTile + cell) * G::kScaleBytes;
-                const uint32_t odd = kDim == 64 ? (uint32_t) s_power[warp][1 + stage] : 0u;
+                const uint8_t* s_at = v_base + G::kPlane + cell * G::kScaleBytes;
                 const int in = t * 8 + 2 * c;
 #pragma unroll
                 for (int i = 0; i < G::kGroups; ++i) {
                     const float down = power_of_two(-powers[i]);
-                    const float s0 = down * __half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd >> in) & 1 : i]);
-                    const float s1 = down * __half2float(reinterpret_cast<const __half*>(s_at + G::kScaleBytes)[kDim == 64 ? (odd >> (in + 1)) & 1 : i]);
+                    const float s0 = down * __half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd_now >> in) & 1 : i]);
+                    const float s1 = down * __half2float(reinterpret_cast<const __half*>(s_at + G::kScaleBytes)[kDim == 64 ? (odd_now >> (in + 1)) & 1 : i]);
                     uint32_t* at = reinterpret_cast<uint32_t*>(weights + ((i * kRows + g) * G::kWeightStride + cell) * 2);
                     at[0] = Pair<__half>::down(w[0] * s0, w[1] * s1);
                     at[8 * G::kWeightStride / 2] = Pair<__half>::down(w[2] * s0, w[3] * s1);
                 }
             }
         }
-        __syncthreads();   // weights; and all of V has landed
+        wait_async<2>();   // V of this tile
+        __syncthreads();   // weights, and everybody's part of V
 
         // ---- output: all cells x the warp's columns
 #pragma unroll
@@ -479,34 +485,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         }
         const int group = kInt8 ? warp * G::kCols / kInt8Group : 0;
         const uint32_t w_at = smem_at(weights) + ((group * kRows + (lane & 15)) * G::kWeightStride + (lane >> 4) * 8) * 2;
-        const uint32_t v_at = smem_at(base) + G::kPlane;
+        const uint32_t v_at = smem_at(v_base);
 #pragma unroll
         for (int k = 0; k < G::kTile / 32; ++k) {   // 32 cells: two products deep
             uint32_t w0[4], w1[4];
             load_matrices(w0, w_at + k * 64);
             load_matrices(w1, w_at + k * 64 + 32);
             if constexpr (kInt8) {
-                constexpr int kPieces = G::kCols >= 16 ? G::kCols / 16 : 1;
 #pragma unroll
-                for (int j = 0; j < kPieces; ++j) {
+                for (int j = 0; j < G::kCols / 16; ++j) {
                     uint32_t b[4];
                     load_matrices_t(b, v_at + chunk_at<G::kChunks>(k * 32 + lane, warp * G::kCols / 16 + j));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) b[i] ^= 0x80808080u;
-                    if constexpr (G::kCols >= 16) {   // even columns, odd columns
-                        multiply(out[2 * j], w0, codes_to_half<0x4240>(b[0]), codes_to_half<0x4240>(b[1]));
-                        multiply(out[2 * j + 1], w0, codes_to_half<0x4341>(b[0]), codes_to_half<0x4341>(b[1]));
-                        multiply(out[2 * j], w1, codes_to_half<0x4240>(b[2]), codes_to_half<0x4240>(b[3]));
-                        multiply(out[2 * j + 1], w1, codes_to_half<0x4341>(b[2]), codes_to_half<0x4341>(b[3]));
-                    } else if (warp & 1) {            // two warps share a chunk of 16 columns
-                        multiply(out[0], w0, codes_to_half<0x4341>(b[0]), codes_to_half<0x4341>(b[1]));
-                        multiply(out[0], w1, codes_to_half<0x4341>(b[2]), codes_to_half<0x4341>(b[3]));
-                    } else {
-                        multiply(out[0], w0, codes_to_half<0x4240>(b[0]), codes_to_half<0x4240>(b[1]));
-                        multiply(out[0], w1, codes_to_half<0x4240>(b[2]), codes_to_half<0x4240>(b[3]));
-                    }
+                    // even columns, odd columns
+                    multiply(out[2 * j], w0, codes_to_half<0x4240>(b[0]), codes_to_half<0x4240>(b[1]));
+                    multiply(out[2 * j + 1], w0, codes_to_half<0x4341>(b[0]), codes_to_half<0x4341>(b[1]));
+                    multiply(out[2 * j], w1, codes_to_half<0x4240>(b[2]), codes_to_half<0x4240>(b[3]));
+                    multiply(out[2 * j + 1], w1, codes_to_half<0x4341>(b[2]), codes_to_half<0x4341>(b[3]));
                 }
-            } else if constexpr (G::kOutTiles >= 2) {
+            } else {
 #pragma unroll
                 for (int j = 0; j < G::kOutTiles / 2; ++j) {
                     uint32_t b[4];
@@ -518,11 +516,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     multiply(out[2 * j], w1, b[0], b[1]);
                     multiply(out[2 * j + 1], w1, b[2], b[3]);
                 }
-            } else {
-                uint32_t b[4];
-                load_matrices_t(b, v_at + chunk_at<G::kChunks>(k * 32 + lane, warp));
-                multiply(out[0], w0, b[0], b[1]);
-                multiply(out[0], w1, b[2], b[3]);
             }
         }
 
@@ -561,8 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         for (int j = 0; j < 2; ++j) {
                             int d;
                             if constexpr (!kInt8) d = warp * G::kCols + i * 8 + 2 * c + j;
-                            else if constexpr (G::kCols >= 16) d = warp * G::kCols + (i >> 1) * 16 + 4 * c + 2 * j + (i & 1);
-                            else d = (warp >> 1) * 16 + 4 * c + 2 * j + (warp & 1);
+                            else d = warp * G::kCols + (i >> 1) * 16 + 4 * c + 2 * j + (i & 1);
                             // an empty row (nothing held, or minus infinity throughout) is zeros
                             const float x = whole && l == 0.0f ? 0.0f : out[i][h * 2 + j] * by;
                             if (whole) to[d] = Pair<T>::one(x);
@@ -597,10 +589,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 /// Joins the parts of the item that share blockIdx.x began and others went on with, head by head (blockIdx.y): each part
 /// counts by 2^(its maximum - the largest), in the order of the shares.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ AttnDev p) {
-    constexpr int kLanes = kDim / 4, kSets = kThreads / kLanes;
-    __shared__ float s_weight[kMaxCtas];
-    __shared__ float s_top[kWarps], s_sum[kWarps];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttnDev p) {
+    constexpr int kLanes = kDim / 4, kSets = kJoinThreads / kLanes;
+    __shared__ float s_weight[kMaxSms * 4];
+    __shared__ float s_top[kJoinThreads / 32], s_sum[kJoinThreads / 32];
     __shared__ float4 s_out[kSets][kLanes];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int2 cut = p.cut[blockIdx.x];
@@ -610,24 +602,28 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
     if (r >= p.group) return;
     const int tid = threadIdx.x, n = cut.y;
     const auto place = [&](int i) { return (((int64_t) blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + blockIdx.y; };
-    const float2 ml = tid < n ? p.part_ml[place(tid)] : make_float2(-INFINITY, 0.0f);
-    float top = ml.x;
+    float top = -INFINITY;
+    for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, p.part_ml[place(i)].x);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     if ((tid & 31) == 0) s_top[tid >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
-    const float weight = exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
-    if (tid < n) s_weight[tid] = weight;
-    float sum = weight * ml.y;
+    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_top[w]);
+    float sum = 0.0f;
+    for (int i = tid; i < n; i += kJoinThreads) {
+        const float2 ml = p.part_ml[place(i)];
+        const float weight = exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+        s_weight[i] = weight;
+        sum = fmaf(weight, ml.y, sum);
+    }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
     __syncthreads();
     sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += s_sum[w];
+    for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_sum[w];
     const int lane = tid % kLanes, set = tid / kLanes;
     float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 8
@@ -656,9 +652,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
 }
 
 template <typename T, int kDim, bool kInt8>
-cudaError_t launch(const AttnDev& p, int ctas, cudaStream_t stream) {
-    constexpr int kSmem = Geo<kDim, kInt8>::kSmem;
-    static_assert(kSmem + 4096 <= 227 * 1024, "the stages fit an SM");
+cudaError_t launch(const AttnDev& p, int sms, cudaStream_t stream) {
+    constexpr int kSmem = Geo<kDim, kInt8>::kSmem, kPerSm = Geo<kDim, kInt8>::kPerSm;
+    static_assert((kSmem + 3072) * kPerSm <= (int) kSmemPerSm && kPerSm <= 4, "the CTAs fit an SM");
+    const int ctas = sms * kPerSm;
     cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kDim, kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     attention_kernel<T, kDim, kInt8><<<ctas, kThreads, kSmem, stream>>>(p);
@@ -667,7 +664,7 @@ cudaError_t launch(const AttnDev& p, int ctas, cudaStream_t stream) {
     // the join is resident, or next in line, when the last share ends; it waits for all of them before its first read
     cudaLaunchConfig_t config{};
     config.gridDim = dim3((unsigned) ctas, (unsigned) (p.group < kRows ? p.group : kRows));
-    config.blockDim = dim3(kThreads);
+    config.blockDim = dim3(kJoinThreads);
     config.stream = stream;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -677,20 +674,24 @@ cudaError_t launch(const AttnDev& p, int ctas, cudaStream_t stream) {
     return cudaLaunchKernelEx(&config, join_kernel<T, kDim>, p);
 }
 template <typename T>
-cudaError_t launch(const AttnDev& p, int dim, bool int8, int ctas, cudaStream_t stream) {
-    if (dim == 64) return int8 ? launch<T, 64, true>(p, ctas, stream) : launch<T, 64, false>(p, ctas, stream);
-    if (dim == 128) return int8 ? launch<T, 128, true>(p, ctas, stream) : launch<T, 128, false>(p, ctas, stream);
-    return int8 ? launch<T, 256, true>(p, ctas, stream) : launch<T, 256, false>(p, ctas, stream);
+cudaError_t launch(const AttnDev& p, int dim, bool int8, int sms, cudaStream_t stream) {
+    if (dim == 64) return int8 ? launch<T, 64, true>(p, sms, stream) : launch<T, 64, false>(p, sms, stream);
+    if (dim == 128) return int8 ? launch<T, 128, true>(p, sms, stream) : launch<T, 128, false>(p, sms, stream);
+    return int8 ? launch<T, 256, true>(p, sms, stream) : launch<T, 256, false>(p, sms, stream);
 }
 
 /// The workspace: parts, their maxima and sums, the shares' cuts.
 struct Room {
     size_t ml, cut, bytes;
-    explicit Room(int dim) {
-        ml = (size_t) kMaxCtas * 2 * kRows * dim * sizeof(float);
-        cut = ml + (size_t) kMaxCtas * 2 * kRows * sizeof(float2);
-        bytes = (cut + kMaxCtas * sizeof(int2) + 255) / 256 * 256;
+    explicit Room(const skv_kv_layer& l) {
+        const bool int8 = l.format == SKV_KV_INT8;
+        const size_t shares = (size_t) kMaxSms * (l.head_dim == 64 ? per_sm<64>(int8) : l.head_dim == 128 ? per_sm<128>(int8) : per_sm<256>(int8));
+        ml = shares * 2 * kRows * l.head_dim * sizeof(float);
+        cut = ml + shares * 2 * kRows * sizeof(float2);
+        bytes = (cut + shares * sizeof(int2) + 255) / 256 * 256;
     }
+    template <int kDim>
+    static int per_sm(bool int8) { return int8 ? Geo<kDim, true>::kPerSm : Geo<kDim, false>::kPerSm; }
 };
 
 }  // namespace
@@ -704,7 +705,7 @@ int skv_decode_attention_workspace(const skv_kv_layer* layer, int n_seqs, int n_
     *out_bytes = 0;
     if (n_seqs < 0 || n_head < 1) return fail(SKV_EINVAL, "skv_decode_attention_workspace: bad counts");
     if (const int rc = check_layer(layer, n_seqs, "skv_decode_attention_workspace")) return rc;
-    *out_bytes = Room(layer->head_dim).bytes;
+    *out_bytes = Room(*layer).bytes;
     return SKV_OK;
 }
 
@@ -730,7 +731,7 @@ int skv_decode_attention(const skv_kv_layer* layer, const skv_attention_args* ar
     DeviceCtx* ctx = current_ctx();
     if (!ctx) return SKV_ECUDA;
     if (!ops_own_memory(layer->k_pool, ctx->device)) return no("the pool is not memory of the current device");
-    const Room room(layer->head_dim);
+    const Room room(*layer);
     AttnDev p{};
     p.layer = to_device(*layer);
     p.a = a;
@@ -740,11 +741,11 @@ int skv_decode_attention(const skv_kv_layer* layer, const skv_attention_args* ar
     p.part_o = static_cast<float*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.workspace) + room.ml);
     p.cut = reinterpret_cast<int2*>(static_cast<uint8_t*>(a.workspace) + room.cut);
-    const int ctas = ctx->sms < kMaxCtas ? ctx->sms : kMaxCtas;
+    const int sms = ctx->sms < kMaxSms ? ctx->sms : kMaxSms;
     const auto s = static_cast<cudaStream_t>(stream);
     const bool int8 = layer->format == SKV_KV_INT8;
-    const cudaError_t e = a.dtype == SKV_DTYPE_F16 ? launch<__half>(p, layer->head_dim, int8, ctas, s)
-                                                   : launch<__nv_bfloat16>(p, layer->head_dim, int8, ctas, s);
+    const cudaError_t e = a.dtype == SKV_DTYPE_F16 ? launch<__half>(p, layer->head_dim, int8, sms, s)
+                                                   : launch<__nv_bfloat16>(p, layer->head_dim, int8, sms, s);
     return e == cudaSuccess ? SKV_OK : cuda_fail(e, "skv_decode_attention");
 }
 
