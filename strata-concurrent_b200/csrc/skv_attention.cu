@@ -586,69 +586,94 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
     wait_async<0>();
 }
 
-/// Joins the parts of the item that share blockIdx.x began and others went on with, head by head (blockIdx.y): each part
-/// counts by 2^(its maximum - the largest), in the order of the shares.
+/// Joins the parts of the items that a share began and others went on with: each part counts by 2^(its maximum - the
+/// largest), in the order of the shares.  A task is one head of one cut item; where there are fewer tasks than CTAs (one
+/// long sequence leaves 148 parts or more of each of 24 heads) it is 64 of its columns.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttnDev p) {
-    constexpr int kLanes = kDim / 4, kSets = kJoinThreads / kLanes;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttnDev p, int shares) {
+    constexpr int kTrips = (kMaxSms * 4 + kJoinThreads - 1) / kJoinThreads, kJoinWarps = kJoinThreads / 32;
+    __shared__ int s_cut[kMaxSms * 4], s_count[kTrips * kJoinWarps];
     __shared__ float s_weight[kMaxSms * 4];
-    __shared__ float s_top[kJoinThreads / 32], s_sum[kJoinThreads / 32];
-    __shared__ float4 s_out[kSets][kLanes];
+    __shared__ float s_top[kJoinWarps], s_sum[kJoinWarps];
+    __shared__ float4 s_out[kJoinThreads];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = min(p.group, kRows), items = p.layer.n_head_kv * p.blocks;
+    if (tid < kTrips * kJoinWarps) s_count[tid] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int2 cut = p.cut[blockIdx.x];
-    if (cut.x < 0) return;
-    const int items = p.layer.n_head_kv * p.blocks, seq = cut.x / items, item = cut.x % items;
-    const int kv = item / p.blocks, r = (item % p.blocks) * kRows + blockIdx.y;
-    if (r >= p.group) return;
-    const int tid = threadIdx.x, n = cut.y;
-    const auto place = [&](int i) { return (((int64_t) blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + blockIdx.y; };
-    float top = -INFINITY;
-    for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, p.part_ml[place(i)].x);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if ((tid & 31) == 0) s_top[tid >> 5] = top;
     __syncthreads();
+    // the cut items, in order
+    uint32_t mask[kTrips];
 #pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_top[w]);
-    float sum = 0.0f;
-    for (int i = tid; i < n; i += kJoinThreads) {
-        const float2 ml = p.part_ml[place(i)];
-        const float weight = exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
-        s_weight[i] = weight;
-        sum = fmaf(weight, ml.y, sum);
+    for (int t = 0; t < kTrips; ++t) {
+        const int i = t * kJoinThreads + tid;
+        mask[t] = __ballot_sync(0xffffffffu, i < shares && p.cut[i].x >= 0);
+        if (lane == 0) s_count[t * kJoinWarps + warp] = __popc(mask[t]);
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
     __syncthreads();
-    sum = 0.0f;
+    int cuts = 0;
 #pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_sum[w];
-    const int lane = tid % kLanes, set = tid / kLanes;
-    float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-    for (int i = set; i < n; i += kSets) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + place(i) * kDim) + lane);
-        const float w = s_weight[i];
-        o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+    for (int j = 0; j < kTrips * kJoinWarps; ++j) {
+        if (j % kJoinWarps == warp && (mask[j / kJoinWarps] >> lane & 1u))
+            s_cut[cuts + __popc(mask[j / kJoinWarps] & ((1u << lane) - 1u))] = j / kJoinWarps * kJoinThreads + tid;
+        cuts += s_count[j];
     }
-    s_out[set][lane] = o;
     __syncthreads();
-    const int64_t head = (int64_t) kv * p.group + r;
-    if (set == 0) {
+    const int pieces = cuts * rows * (kDim / 64) <= (int) gridDim.x ? kDim / 64 : 1;
+    const int lanes = kDim / 4 / pieces, sets = kJoinThreads / lanes;   // four columns a lane
+    for (int task = blockIdx.x; task < cuts * rows * pieces; task += gridDim.x) {
+        const int begun = s_cut[task / (rows * pieces)], row = task / pieces % rows, piece = task % pieces;
+        const int2 cut = p.cut[begun];
+        const int seq = cut.x / items, item = cut.x % items, n = cut.y;
+        const int kv = item / p.blocks, r = (item % p.blocks) * kRows + row;
+        if (r >= p.group) continue;   // the same for the whole CTA
+        const auto place = [&](int i) { return (((int64_t) begun + i) * 2 + (i == 0 ? 1 : 0)) * kRows + row; };
+        float top = -INFINITY;
+        for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, p.part_ml[place(i)].x);
 #pragma unroll
-        for (int i = 1; i < kSets; ++i) {
-            const float4 x = s_out[i][lane];
-            o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_top[w]);
+        float sum = 0.0f;
+        for (int i = tid; i < n; i += kJoinThreads) {
+            const float2 ml = p.part_ml[place(i)];
+            const float weight = exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
+            s_weight[i] = weight;
+            sum = fmaf(weight, ml.y, sum);
         }
-        const float by = 1.0f / sum;
-        if (sum == 0.0f) o = make_float4(0, 0, 0, 0);
-        else o = make_float4(o.x * by, o.y * by, o.z * by, o.w * by);
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + (int64_t) seq * p.a.out_stride + head * kDim + lane * 4) =
-            make_uint2(Pair<T>::down(o.x, o.y), Pair<T>::down(o.z, o.w));
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) sum += s_sum[w];
+        const int at = tid % lanes, set = tid / lanes, column = (piece * lanes + at) * 4;
+        float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+        for (int i = set; i < n; i += sets) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + place(i) * kDim + column));
+            const float w = s_weight[i];
+            o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+        }
+        s_out[tid] = o;
+        __syncthreads();
+        const int64_t head = (int64_t) kv * p.group + r;
+        if (set == 0) {
+            for (int i = 1; i < min(sets, n); ++i) {
+                const float4 x = s_out[i * lanes + at];
+                o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+            }
+            const float by = 1.0f / sum;
+            if (sum == 0.0f) o = make_float4(0, 0, 0, 0);
+            else o = make_float4(o.x * by, o.y * by, o.z * by, o.w * by);
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + (int64_t) seq * p.a.out_stride + head * kDim + column) =
+                make_uint2(Pair<T>::down(o.x, o.y), Pair<T>::down(o.z, o.w));
+        }
+        if (tid == 0 && piece == 0 && p.a.lse)
+            p.a.lse[(int64_t) seq * p.a.n_head + head] = sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        __syncthreads();   // the next task writes s_top, s_weight and s_out again
     }
-    if (tid == 0 && p.a.lse)
-        p.a.lse[(int64_t) seq * p.a.n_head + head] = sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
 template <typename T, int kDim, bool kInt8>
@@ -663,7 +688,7 @@ cudaError_t launch(const AttnDev& p, int sms, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     // the join is resident, or next in line, when the last share ends; it waits for all of them before its first read
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned) ctas, (unsigned) (p.group < kRows ? p.group : kRows));
+    config.gridDim = dim3((unsigned) sms * 8);
     config.blockDim = dim3(kJoinThreads);
     config.stream = stream;
     cudaLaunchAttribute early{};
@@ -671,7 +696,7 @@ cudaError_t launch(const AttnDev& p, int sms, cudaStream_t stream) {
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, join_kernel<T, kDim>, p);
+    return cudaLaunchKernelEx(&config, join_kernel<T, kDim>, p, ctas);
 }
 template <typename T>
 cudaError_t launch(const AttnDev& p, int dim, bool int8, int sms, cudaStream_t stream) {
