@@ -22,10 +22,13 @@ constexpr int kSlice = 32;                       // value columns per CTA
 constexpr int kGroups = kThreads / (kSlice / 4); // row groups: 16
 constexpr int kChunksFrom = 32;                  // tokens of the longest sequence
 
+struct Record;
+
 struct DeltaDev {
     skv_gdn_args a;
     uint32_t* status;
-    int ratio;   // value heads per key head
+    Record* records;   // [slot][value head], when the call runs in chunks
+    int ratio;         // value heads per key head
 };
 
 /// The tokens [begin, end) of a sequence; false when it has none.
@@ -140,19 +143,21 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 //     (I + A) V' = beta (V - e^G K S),   A_ij = beta_i e^(G_i - G_j) k_i . k_j  (j < i)
 //     O  = scale (e^G Q S + P V'),       P_ij = e^(G_i - G_j) q_i . k_j         (j <= i)
 //     S <- e^(G_63) S + K^T (e^(G_63 - G) V')
-// A CTA takes one head's slice of 16 kConsumers value columns through all of its sequence's chunks.  Four producer warps
-// stay one chunk ahead: they stage K, Q and V, and work out P and T = (I + A)^-1, which need no state.  Each consumer warp
-// holds the transposed state of 16 columns in its accumulators and runs the recurrence alone: what a product leaves in
-// accumulators is the left operand of the next (S^T K^T, then V'^T = R^T T^T, then S^T += V'^T K), so nothing of
-// the chain passes through memory.  The chain bounds a single long sequence, so the slices are narrow when few CTAs
-// would run (2 consumers: 128 CTAs for 32 heads), wider when there are more than fill the GPU (4).
+// What needs no state, P and T = (I + A)^-1 with the decays, is worked out first, for all chunks at once: prepare_kernel
+// writes a record per chunk and head into the workspace.  Then chunk_kernel takes one head's slice of 16 kGroupsOf value
+// columns through all chunks of its sequence: four loader warps stay a chunk ahead, and a pair of consumer warps holds
+// the transposed state of 16 columns in accumulators, each warp one half of the keys.  What a product leaves in
+// accumulators is the left operand of the next (S^T K^T, then V'^T = R^T T^T, then S^T += V'^T K), so the chain from
+// chunk to chunk passes through memory once, where the halves' sums over the keys meet.  That chain, not the flops,
+// bounds a long sequence: hence the halves, and narrow slices where few CTAs would run (2 groups: 128 CTAs for 32
+// heads of one sequence), wider ones where there are more than fill the GPU (4).
 //
-// Precision.  Every product is fp16 with 32-bit sums.  A 32-bit operand (S, R, V', T) enters as the sum of two fp16 values
-// after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least; the state
-// therefore keeps 32-bit quality.  Only what goes to the 16-bit output alone (Q S, P V') takes the first of the two.  K and Q
-// are exact: fp16 as they are, bfloat16 scaled by a power of two (K by one per chunk, Q by one per row), up to values
-// 2^-24 of the largest.  The sums G are taken in 64 bits, so that a decay of e^-200 in a chunk (deeper ones are as good
-// as that) leaves the others' differences exact.
+// Precision.  Every product is fp16 with 32-bit sums.  A 32-bit operand (S, R, V', T, A) enters as the sum of two fp16
+// values after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least; the
+// state therefore keeps 32-bit quality.  Only what goes to the 16-bit output alone (Q S, P V') takes the first of the
+// two.  K and Q are exact: fp16 as they are, bfloat16 scaled by a power of two (K by one per chunk, Q by one per row), up
+// to values 2^-24 of the largest.  The sums G are taken in 64 bits and kept as two 32-bit parts, so that a decay of
+// e^-200 in a chunk (deeper ones are as good as that) leaves the others' differences exact.
 
 constexpr int kChunk = 64;
 constexpr int kProducers = 4;
@@ -215,346 +220,532 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t
     low = Pair<__half>::down(x - h.x, y - h.y);
 }
 
-/// Per token of a chunk, for the consumers.
+/// Per token of a chunk.
 struct Factors {
     float value[kChunk];    // 2^F beta
     float key[kChunk];      // 2^2F beta e^G
     float query[kChunk];    // e^G
     float out[kChunk];      // scale 2^(the query row's power)
     float update[kChunk];   // e^(G_63 - G)
+    float down[kChunk];     // 2^-(the query row's power)
     float whole;            // e^(G_63)
+    float key_down;         // 2^-F, F the power of the chunk's keys
+    float pad[2];
 };
+/// What prepare_kernel leaves of a chunk and head: the ten blocks of 16 x 16 on and below the diagonal of T (in two fp16
+/// parts, times kInverseScale) and of P, and the factors.
+constexpr int kBlockBytes = 512, kTriangleBytes = 10 * kBlockBytes;
+struct Record {
+    uint8_t t_high[kTriangleBytes], t_low[kTriangleBytes], mix[kTriangleBytes];
+    Factors f;
+};
+static_assert(sizeof(Record) % 16 == 0, "copied 16 bytes at a time");
+__host__ __device__ constexpr int block_of(int i, int j) { return i * (i + 1) / 2 + j; }
+/// The 16-byte half `chunk` of row `row` of a block, swizzled so that eight rows' equal halves lie in eight bank groups.
+__device__ __forceinline__ uint32_t half_row_at(int row, int chunk) { return (uint32_t) (row * 2 + (chunk ^ ((row >> 2) & 1))) * 16u; }
 
-template <int kDim, int kConsumers>
-struct ChunkRoom {
-    static constexpr int kTileBytes = kChunk * kDim * 2, kValueBytes = kChunk * kConsumers * 32, kSquareBytes = kChunk * kChunk * 2;
-    struct Buffer {
-        alignas(128) uint8_t k[kTileBytes], q[kTileBytes], v[kValueBytes], t_high[kSquareBytes], t_low[kSquareBytes], mix[kSquareBytes];
-        Factors f;
+/// The record slot of a sequence's first chunk: a sequence of n tokens from `begin` on takes ceil(n / 64) slots, at most
+/// floor((begin + n) / 64) - floor(begin / 64) + 1, so sequence s starts at floor(begin / 64) + s.
+__device__ __forceinline__ int64_t first_slot(int begin, int seq) { return begin / kChunk + seq; }
+
+int64_t record_slots(int n_tokens, int n_seqs) { return (int64_t) n_tokens / kChunk + n_seqs; }
+bool chunked(bool packed, int max_tokens) { return packed && max_tokens >= kChunksFrom; }
+
+/// fp16 parts of the left operand (16 x 16) at `at` in a 32-bit scratch matrix.
+__device__ __forceinline__ void left_parts(const float* at, float scale, uint32_t (&high)[4], uint32_t (&low)[4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 x = *reinterpret_cast<const float2*>(at + (g + (j & 1) * 8) * kScratch + 2 * c + (j >> 1) * 8);
+        split(x.x * scale, x.y * scale, high[j], low[j]);
+    }
+}
+/// ... and of the right operand (16 x 8).
+__device__ __forceinline__ void right_parts(const float* at, float scale, uint32_t (&high)[2], uint32_t (&low)[2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const float* x = at + (2 * c + j * 8) * kScratch + g;
+        split(x[0] * scale, x[kScratch] * scale, high[j], low[j]);
+    }
+}
+__device__ __forceinline__ void multiply_parts(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const uint32_t (&bh)[2], const uint32_t (&bl)[2]) {
+    multiply(c, ah, bl[0], bl[1]);
+    multiply(c, al, bh[0], bh[1]);
+    multiply(c, ah, bh[0], bh[1]);
+}
+__device__ __forceinline__ void store_product(float* at, float by, const float (&x)[4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    *reinterpret_cast<float2*>(at + g * kScratch + 2 * c) = make_float2(by * x[0], by * x[1]);
+    *reinterpret_cast<float2*>(at + (g + 8) * kScratch + 2 * c) = make_float2(by * x[2], by * x[3]);
+}
+
+template <int kDim>
+struct PrepareRoom {
+    union {
+        struct { uint8_t k[kChunk * kDim * 2], q[kChunk * kDim * 2]; } in;
+        struct { float a[kChunk * kScratch], t[kChunk * kScratch], x[kChunk / 2 * kScratch]; } work;
     };
-    Buffer buffer[2];
-    float a[kChunk * kScratch], t[kChunk * kScratch], x[kChunk / 2 * kScratch];
-    double sums[kChunk];
+    alignas(16) uint8_t mix[kTriangleBytes];
+    float2 sums[kChunk];      // G log2 e in two parts
+    double carry[2];          // the first 32 tokens' sum, and all
     float beta[kChunk];
-    float largest[kProducers];
+    float largest[4];
 };
 
-template <typename T, int kDim, int kConsumers>
-__device__ __forceinline__ void produce(const DeltaDev& p, ChunkRoom<kDim, kConsumers>& room, int begin, int end, int head, int slice) {
-    constexpr int kAll = kProducerThreads + kConsumers * 32, kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
-    constexpr int kValueChunks = kConsumers * 2;
+/// Blocks (kRow, kFrom .. kTo - 1) of K K^T and Q K^T: 16 tokens against 16 (kTo - kFrom).
+template <int kDim, int kBlocks>
+__device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, int row, int from, float (&kk)[2 * kBlocks][4], float (&qk)[2 * kBlocks][4]) {
+    constexpr int kChunks = kDim / 8;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int t = 0; t < 2 * kBlocks; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kk[t][j] = qk[t][j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kDim / 16; ++i) {
+        uint32_t x[4], y[4];
+        load_matrices(x, k_at + chunk_at<kChunks>(row * 16 + (lane & 15), 2 * i + (lane >> 4)));
+        load_matrices(y, q_at + chunk_at<kChunks>(row * 16 + (lane & 15), 2 * i + (lane >> 4)));
+#pragma unroll
+        for (int t = 0; t < kBlocks; ++t) {
+            uint32_t m[4];
+            load_matrices(m, k_at + chunk_at<kChunks>((from + t) * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+            multiply(kk[2 * t], x, m[0], m[1]);
+            multiply(kk[2 * t + 1], x, m[2], m[3]);
+            multiply(qk[2 * t], y, m[0], m[1]);
+            multiply(qk[2 * t + 1], y, m[2], m[3]);
+        }
+    }
+}
+/// A (32 bits) and P (fp16) of those blocks.
+template <int kDim, int kBlocks>
+__device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int block_row, int from, const float (&kk)[2 * kBlocks][4], const float (&qk)[2 * kBlocks][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int in = g + h * 8, row = block_row * 16 + in;
+        const float2 sum = room.sums[row];
+        const float by = fit2 * room.beta[row];
+#pragma unroll
+        for (int t = 0; t < 2 * kBlocks; ++t) {
+            const int col = from * 16 + t * 8 + 2 * c;
+            const float4 other = *reinterpret_cast<const float4*>(&room.sums[col]);   // of col and col + 1
+            // a decay of zero (and what lies above the diagonal) wipes out even an infinite product
+            const float d0 = exp2f((sum.x - other.x) + (sum.y - other.y)), d1 = exp2f((sum.x - other.z) + (sum.y - other.w));
+            *reinterpret_cast<float2*>(&room.work.a[row * kScratch + col]) =
+                make_float2(col < row ? by * d0 * kk[t][2 * h] : 0.0f, col + 1 < row ? by * d1 * kk[t][2 * h + 1] : 0.0f);
+            *reinterpret_cast<uint32_t*>(room.mix + block_of(block_row, from + t / 2) * kBlockBytes + half_row_at(in, t & 1) + c * 4) =
+                Pair<__half>::down(col <= row ? d0 * qk[t][2 * h] : 0.0f, col + 1 <= row ? d1 * qk[t][2 * h + 1] : 0.0f);
+        }
+    }
+}
+
+/// One chunk of one head.  Four warps; four CTAs an SM hide the short phases' latencies.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __grid_constant__ DeltaDev p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    auto& room = *reinterpret_cast<PrepareRoom<kDim>*>(smem);
+    constexpr int kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
     const skv_gdn_args& a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int head = (int) (blockIdx.x % a.n_v_heads);
+    const int64_t slot = blockIdx.x / a.n_v_heads;
+    // the last sequence whose slots begin at or before this one
+    int lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        const int at = a.seq_starts ? min(max(__ldg(a.seq_starts + mid), 0), a.n_tokens) : mid;
+        if (first_slot(at, mid) <= slot) lo = mid;
+        else hi = mid;
+    }
+    int begin, end;
+    if (!tokens_of(a, lo, begin, end)) return;
+    const int64_t chunk_of = slot - first_slot(begin, lo);
+    if (chunk_of < 0 || chunk_of * kChunk >= end - begin) return;
+    const int t0 = begin + (int) chunk_of * kChunk;
+    Record& record = p.records[slot * a.n_v_heads + head];
+
+    // ---- K and Q as fp16
     const T* qh = static_cast<const T*>(a.q) + (head / p.ratio) * kDim;
     const T* kh = static_cast<const T*>(a.k) + (head / p.ratio) * kDim;
-    const T* vh = static_cast<const T*>(a.v) + head * kDim + slice * kConsumers * 16;
-    uint4 next_k[kMine], next_q[kMine];
-    float next_g = 0.0f, next_beta = 0.0f;
-    const auto fetch = [&](int t0) {
+    uint4 k[kMine];
+    float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
-            const bool on = t0 + r < end;
-            const int64_t t = on ? t0 + r : begin;
-            next_k[i] = on ? __ldg(reinterpret_cast<const uint4*>(kh + t * a.k_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
-            next_q[i] = on ? __ldg(reinterpret_cast<const uint4*>(qh + t * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < kMine; ++i) {
+        const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+        const bool on = t0 + r < end;
+        k[i] = on ? __ldg(reinterpret_cast<const uint4*>(kh + (int64_t) (t0 + r) * a.k_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
+    }
+    float g = 0.0f, beta = 0.0f;
+    if (tid < kChunk && t0 + tid < end) {
+        g = __ldg(a.g + (int64_t) (t0 + tid) * a.g_stride + head);
+        beta = __ldg(a.beta + (int64_t) (t0 + tid) * a.beta_stride + head);
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+        const bool on = t0 + r < end;
+        uint4 q = on ? __ldg(reinterpret_cast<const uint4*>(qh + (int64_t) (t0 + r) * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
+        int power = 0;
+        if constexpr (!std::is_same<T, __half>::value) {
+            float x[8], most = 0.0f;
+            unpack8<T>(q, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+#pragma unroll
+            for (int m = 1; m < kChunks; m <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
+            power = most > 0.0f && most < INFINITY ? min(max(exponent_of(most), -126), 126) : 0;
+            const float down = power_of_two(-power);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= down;
+            q = pack8<__half>(x);
+            unpack8<T>(k[i], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
         }
-        if (tid < kChunk) {
-            const bool on = t0 + tid < end;
-            next_g = on ? __ldg(a.g + (int64_t) (t0 + tid) * a.g_stride + head) : 0.0f;
-            next_beta = on ? __ldg(a.beta + (int64_t) (t0 + tid) * a.beta_stride + head) : 0.0f;
+        *reinterpret_cast<uint4*>(room.in.q + chunk_at<kChunks>(r, chunk)) = q;
+        if (chunk == 0) {
+            record.f.out[r] = a.scale * power_of_two(power);
+            record.f.down[r] = power_of_two(-power);
         }
+    }
+    int key_power = 0;
+    if constexpr (!std::is_same<T, __half>::value) {
+        top = warp_largest(top);
+        if (lane == 0) room.largest[warp] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(room.largest[0], room.largest[1]), fmaxf(room.largest[2], room.largest[3]));
+        key_power = top > 0.0f && top < INFINITY ? min(max(exponent_of(top), -60), 60) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+        if constexpr (!std::is_same<T, __half>::value) {
+            float x[8];
+            unpack8<T>(k[i], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= power_of_two(-key_power);
+            k[i] = pack8<__half>(x);
+        }
+        *reinterpret_cast<uint4*>(room.in.k + chunk_at<kChunks>(r, chunk)) = k[i];
+    }
+    // ---- the decays: a token per lane of two warps, sums in 64 bits
+    const float fit = power_of_two(key_power);
+    double sum = g < -200.0f ? -200.0 : (double) g;
+    if (warp < 2) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const double o = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += o;
+        }
+        if (tid == 31) room.carry[0] = sum;
+    }
+    __syncthreads();
+    if (warp < 2) {
+        if (warp == 1) sum += room.carry[0];
+        if (tid == 63) room.carry[1] = sum;
+        const double turns = sum * 1.4426950408889634074;   // log2 e
+        const float high = (float) turns;
+        room.sums[tid] = make_float2(high, (float) (turns - (double) high));
+        room.beta[tid] = beta;
+    }
+    __syncthreads();
+    if (warp < 2) {
+        const double all = room.carry[1];
+        const float into = expf((float) sum);
+        record.f.value[tid] = fit * beta;
+        record.f.key[tid] = fit * fit * beta * into;
+        record.f.query[tid] = into;
+        record.f.update[tid] = expf((float) (all - sum));
+        if (tid == 0) {
+            record.f.whole = expf((float) all);
+            record.f.key_down = power_of_two(-key_power);
+        }
+    }
+    // ---- K K^T and Q K^T on and below the diagonal: ten blocks of 16 x 16, at most three a warp
+    const uint32_t k_at = smem_at(room.in.k), q_at = smem_at(room.in.q);
+    const float fit2 = fit * fit;
+    if (warp < 2) {            // row 3, two blocks each
+        float kk[4][4], qk[4][4];
+        products<kDim, 2>(k_at, q_at, 3, 2 * warp, kk, qk);
+        meet<kProducerThreads>(1);   // the scratch matrices lie where K and Q are
+        decayed<kDim, 2>(room, fit2, 3, 2 * warp, kk, qk);
+    } else if (warp == 2) {    // row 2
+        float kk[6][4], qk[6][4];
+        products<kDim, 3>(k_at, q_at, 2, 0, kk, qk);
+        meet<kProducerThreads>(1);
+        decayed<kDim, 3>(room, fit2, 2, 0, kk, qk);
+    } else {                   // rows 1 and 0
+        float kk[4][4], qk[4][4], kk0[2][4], qk0[2][4];
+        products<kDim, 2>(k_at, q_at, 1, 0, kk, qk);
+        products<kDim, 1>(k_at, q_at, 0, 0, kk0, qk0);
+        meet<kProducerThreads>(1);
+        decayed<kDim, 2>(room, fit2, 1, 0, kk, qk);
+        decayed<kDim, 1>(room, fit2, 0, 0, kk0, qk0);
+    }
+    __syncthreads();
+    // ---- T = (I + A)^-1: the diagonal blocks of 16 by substitution, a column per thread
+    auto& work = room.work;
+    if (tid < kChunk) {
+        const int base = tid & ~15, col = tid & 15;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float r[16];
+#pragma unroll
+            for (int j = 0; j < (i + 3) / 4; ++j)
+                *reinterpret_cast<float4*>(&r[4 * j]) = *reinterpret_cast<const float4*>(&work.a[(base + i) * kScratch + base + 4 * j]);
+            float s0 = i == col ? 1.0f : 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) {
+                if (j & 1) s1 = fmaf(-r[j], x[j], s1);
+                else s0 = fmaf(-r[j], x[j], s0);
+            }
+            x[i] = s0 + s1;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) work.t[(base + i) * kScratch + base + col] = x[i];
+    } else {
+        // above the diagonal blocks of each half the products below read zeros
+        for (int i = tid - kChunk; i < 2 * 16 * 16; i += kChunk)
+            work.t[(i / 256 * 32 + i % 256 / 16) * kScratch + i / 256 * 32 + 16 + i % 16] = 0.0f;
+    }
+    __syncthreads();
+    // below them T21 = -T22 (A21 T11): the blocks of 16 of each half, then the block of 32, eight columns a warp
+    constexpr float kUnit = kInverseScale, kDown = 1.0f / (kUnit * kUnit);
+    uint32_t ah[4], al[4], bh[2], bl[2];
+    {
+        const int at = (warp >> 1) * 32, col = (warp & 1) * 8;
+        float c[4] = {0, 0, 0, 0}, d[4] = {0, 0, 0, 0};
+        left_parts(&work.a[(at + 16) * kScratch + at], kUnit, ah, al);
+        right_parts(&work.t[at * kScratch + at + col], kUnit, bh, bl);
+        multiply_parts(c, ah, al, bh, bl);
+        store_product(&work.x[(warp >> 1) * 16 * kScratch + col], kDown, c);
+        __syncwarp();
+        left_parts(&work.t[(at + 16) * kScratch + at + 16], -kUnit, ah, al);
+        right_parts(&work.x[(warp >> 1) * 16 * kScratch + col], kUnit, bh, bl);
+        multiply_parts(d, ah, al, bh, bl);
+        store_product(&work.t[(at + 16) * kScratch + at + col], kDown, d);
+    }
+    __syncthreads();
+    {
+        const int col = warp * 8;
+        float c[2][4] = {}, d[2][4] = {};
+#pragma unroll
+        for (int k16 = 0; k16 < 2; ++k16) {
+            right_parts(&work.t[k16 * 16 * kScratch + col], kUnit, bh, bl);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                left_parts(&work.a[(32 + m * 16) * kScratch + k16 * 16], kUnit, ah, al);
+                multiply_parts(c[m], ah, al, bh, bl);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) store_product(&work.x[m * 16 * kScratch + col], kDown, c[m]);
+        __syncwarp();
+#pragma unroll
+        for (int k16 = 0; k16 < 2; ++k16) {
+            right_parts(&work.x[k16 * 16 * kScratch + col], kUnit, bh, bl);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                left_parts(&work.t[(32 + m * 16) * kScratch + 32 + k16 * 16], -kUnit, ah, al);
+                multiply_parts(d[m], ah, al, bh, bl);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) store_product(&work.t[(32 + m * 16) * kScratch + col], kDown, d[m]);
+    }
+    __syncthreads();
+    // ---- T in two fp16 parts, and P
+    for (int at = tid; at < kTriangleBytes / 16; at += kProducerThreads) {
+        const int block = at / 32, r = at % 32 / 2, chunk = at % 2;
+        const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3, j = block - block_of(i, 0);
+        const float4* x = reinterpret_cast<const float4*>(&work.t[(i * 16 + r) * kScratch + j * 16 + chunk * 8]);
+        const float4 u = x[0], v = x[1];
+        uint32_t high[4], low[4];
+        split(u.x * kUnit, u.y * kUnit, high[0], low[0]);
+        split(u.z * kUnit, u.w * kUnit, high[1], low[1]);
+        split(v.x * kUnit, v.y * kUnit, high[2], low[2]);
+        split(v.z * kUnit, v.w * kUnit, high[3], low[3]);
+        const uint32_t to = block * kBlockBytes + half_row_at(r, chunk);
+        *reinterpret_cast<uint4*>(record.t_high + to) = make_uint4(high[0], high[1], high[2], high[3]);
+        *reinterpret_cast<uint4*>(record.t_low + to) = make_uint4(low[0], low[1], low[2], low[3]);
+        *reinterpret_cast<uint4*>(record.mix + at * 16) = *reinterpret_cast<const uint4*>(room.mix + at * 16);
+    }
+}
+
+template <int kDim, int kGroupsOf>
+struct ChunkRoom {
+    struct Buffer {
+        alignas(128) uint8_t k[kChunk * kDim * 2], q[kChunk * kDim * 2], v[kChunk * kGroupsOf * 32];
+        Record record;
     };
-    fetch(begin);
+    Buffer buffer[2];
+    float4 meet[kGroupsOf * 2][12][32];   // what a consumer warp hands its partner: K S (8), Q S of the partner's tokens (4)
+    int power[kGroupsOf * 2];
+};
+
+template <typename T, int kDim, int kGroupsOf>
+__device__ __forceinline__ void load_chunks(const DeltaDev& p, ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int seq, int head, int slice) {
+    constexpr int kAll = kProducerThreads + kGroupsOf * 64, kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
+    constexpr int kValueChunks = kGroupsOf * 2;
+    constexpr bool kAsIs = std::is_same<T, __half>::value;
+    const skv_gdn_args& a = p.a;
+    const int tid = threadIdx.x;
+    const T* qh = static_cast<const T*>(a.q) + (head / p.ratio) * kDim;
+    const T* kh = static_cast<const T*>(a.k) + (head / p.ratio) * kDim;
+    const T* vh = static_cast<const T*>(a.v) + head * kDim + slice * kGroupsOf * 16;
+    const int64_t slot = first_slot(begin, seq);
     int b = 0;
     for (int t0 = begin, n = 0; t0 < end; t0 += kChunk, ++n, b ^= 1) {
         auto& buf = room.buffer[b];
+        const Record& record = p.records[(slot + n) * a.n_v_heads + head];
+        uint4 k[kAsIs ? 1 : kMine], q[kAsIs ? 1 : kMine];
+        float down[kAsIs ? 1 : kMine], key_down = 1.0f;
+        if constexpr (!kAsIs) {    // on their way while the buffer is still in use
+            key_down = __ldg(&record.f.key_down);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+                const bool on = t0 + r < end;
+                const int64_t t = on ? t0 + r : begin;
+                k[i] = on ? __ldg(reinterpret_cast<const uint4*>(kh + t * a.k_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
+                q[i] = on ? __ldg(reinterpret_cast<const uint4*>(qh + t * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
+                down[i] = __ldg(&record.f.down[r]);
+            }
+        }
         if (n >= 2) meet<kAll>(3 + b);   // the consumers are done with this buffer
-        // ---- V of the slice as it is; K and Q as fp16
         for (int at = tid; at < kChunk * kValueChunks; at += kProducerThreads) {
             const int r = at / kValueChunks, chunk = at % kValueChunks;
             const bool on = t0 + r < end;
             copy_async16(smem_at(buf.v) + chunk_at<kValueChunks>(r, chunk), vh + (int64_t) (on ? t0 + r : begin) * a.v_stride + chunk * 8, on);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        int key_power = 0;
-        if constexpr (!std::is_same<T, __half>::value) {
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-                float x[8];
-                unpack8<T>(next_k[i], x);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
-            }
-            top = warp_largest(top);
-            if (lane == 0) room.largest[warp] = top;
-            meet<kProducerThreads>(5);
-            top = fmaxf(fmaxf(room.largest[0], room.largest[1]), fmaxf(room.largest[2], room.largest[3]));
-            key_power = top > 0.0f && top < INFINITY ? min(max(exponent_of(top), -60), 60) : 0;
-        }
-        const float key_down = power_of_two(-key_power);
+        for (int at = tid; at < (int) (sizeof(Record) / 16); at += kProducerThreads)
+            copy_async16(smem_at(&buf.record) + at * 16, reinterpret_cast<const uint8_t*>(&record) + at * 16, true);
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
-            uint4 k = next_k[i], q = next_q[i];
-            int power = 0;
-            if constexpr (!std::is_same<T, __half>::value) {
-                float x[8], top = 0.0f;
-                unpack8<T>(k, x);
+            const uint32_t to = chunk_at<kChunks>(r, chunk);
+            if constexpr (kAsIs) {
+                const bool on = t0 + r < end;
+                const int64_t t = on ? t0 + r : begin;
+                copy_async16(smem_at(buf.k) + to, kh + t * a.k_stride + chunk * 8, on);
+                copy_async16(smem_at(buf.q) + to, qh + t * a.q_stride + chunk * 8, on);
+            } else {
+                float x[8];
+                unpack8<T>(k[i], x);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] *= key_down;
-                k = pack8<__half>(x);
-                unpack8<T>(q, x);
+                *reinterpret_cast<uint4*>(buf.k + to) = pack8<__half>(x);
+                unpack8<T>(q[i], x);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
-#pragma unroll
-                for (int m = 1; m < kChunks; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-                power = top > 0.0f && top < INFINITY ? min(max(exponent_of(top), -126), 126) : 0;
-                const float down = power_of_two(-power);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= down;
-                q = pack8<__half>(x);
-            }
-            *reinterpret_cast<uint4*>(buf.k + chunk_at<kChunks>(r, chunk)) = k;
-            *reinterpret_cast<uint4*>(buf.q + chunk_at<kChunks>(r, chunk)) = q;
-            if (chunk == 0) buf.f.out[r] = a.scale * power_of_two(power);
-        }
-        // ---- the decays: warp 0, two tokens a lane, sums in 64 bits
-        if (tid < kChunk) {
-            room.sums[tid] = next_g < -200.0f ? -200.0 : (double) next_g;
-            room.beta[tid] = next_beta;
-        }
-        meet<kProducerThreads>(5);
-        if (warp == 0) {
-            const double x = room.sums[2 * lane], y = room.sums[2 * lane + 1];
-            double up = x + y;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const double o = __shfl_up_sync(0xffffffffu, up, d);
-                if (lane >= d) up += o;
-            }
-            const double all = __shfl_sync(0xffffffffu, up, 31);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int t = 2 * lane + h;
-                const double sum = h ? up : up - y;
-                const float into = expf((float) sum), beta = room.beta[t], fit = power_of_two(key_power);
-                room.sums[t] = sum;
-                buf.f.value[t] = fit * beta;
-                buf.f.key[t] = fit * fit * beta * into;
-                buf.f.query[t] = into;
-                buf.f.update[t] = expf((float) (all - sum));
-                if (t == 0) buf.f.whole = expf((float) all);
+                for (int j = 0; j < 8; ++j) x[j] *= down[i];
+                *reinterpret_cast<uint4*>(buf.q + to) = pack8<__half>(x);
             }
         }
-        if (t0 + kChunk < end) fetch(t0 + kChunk);
-        meet<kProducerThreads>(5);
-        // ---- K K^T and Q K^T of 16 tokens per warp, up to the diagonal; A (32 bits) and P (fp16)
-        {
-            float kk[8][4], qk[8][4];
-#pragma unroll
-            for (int t = 0; t < 8; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) kk[t][j] = qk[t][j] = 0.0f;
-            const uint32_t k_at = smem_at(buf.k), q_at = smem_at(buf.q);
-#pragma unroll
-            for (int i = 0; i < kDim / 16; ++i) {
-                uint32_t x[4], y[4];
-                load_matrices(x, k_at + chunk_at<kChunks>(warp * 16 + (lane & 15), 2 * i + (lane >> 4)));
-                load_matrices(y, q_at + chunk_at<kChunks>(warp * 16 + (lane & 15), 2 * i + (lane >> 4)));
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (t <= warp) {
-                        uint32_t m[4];
-                        load_matrices(m, k_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
-                        multiply(kk[2 * t], x, m[0], m[1]);
-                        multiply(kk[2 * t + 1], x, m[2], m[3]);
-                        multiply(qk[2 * t], y, m[0], m[1]);
-                        multiply(qk[2 * t + 1], y, m[2], m[3]);
-                    }
-                }
-            }
-            const float fit = power_of_two(key_power), fit2 = fit * fit;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = warp * 16 + g + h * 8;
-                const double sum = room.sums[row];
-                const float by = fit2 * room.beta[row];
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    if (t < 2 * warp + 2) {
-                        const int col = t * 8 + 2 * c;
-                        const float d0 = col <= row ? expf((float) (sum - room.sums[col])) : 0.0f;
-                        const float d1 = col + 1 <= row ? expf((float) (sum - room.sums[col + 1])) : 0.0f;
-                        // a decay of zero wipes out even an infinite product
-                        *reinterpret_cast<float2*>(&room.a[row * kScratch + col]) =
-                            make_float2(col < row ? by * d0 * kk[t][2 * h] : 0.0f, col + 1 < row ? by * d1 * kk[t][2 * h + 1] : 0.0f);
-                        *reinterpret_cast<uint32_t*>(buf.mix + chunk_at<8>(row, t) + c * 4) =
-                            Pair<__half>::down(col <= row ? d0 * qk[t][2 * h] : 0.0f, col + 1 <= row ? d1 * qk[t][2 * h + 1] : 0.0f);
-                    }
-                }
-            }
-        }
-        meet<kProducerThreads>(5);
-        // ---- T = (I + A)^-1: the diagonal blocks of 16 by substitution, a column per thread
-        if (tid < kChunk) {
-            const int base = tid & ~15, col = tid & 15;
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float r[16];
-#pragma unroll
-                for (int j = 0; j < (i + 3) / 4; ++j)
-                    *reinterpret_cast<float4*>(&r[4 * j]) = *reinterpret_cast<const float4*>(&room.a[(base + i) * kScratch + base + 4 * j]);
-                float s0 = i == col ? 1.0f : 0.0f, s1 = 0.0f;
-#pragma unroll
-                for (int j = 0; j < i; ++j) {
-                    if (j & 1) s1 = fmaf(-r[j], x[j], s1);
-                    else s0 = fmaf(-r[j], x[j], s0);
-                }
-                x[i] = s0 + s1;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) room.t[(base + i) * kScratch + base + col] = x[i];
-        }
-        meet<kProducerThreads>(5);
-        // below them, T21 = -T22 (A21 T11): blocks of 16 in each half, then the block of 32
-        {
-            const int half_at = (tid >> 6) * 32, r = (tid & 63) >> 2, col = (tid & 3) * 4;
-            float4 s = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float w = room.a[(half_at + 16 + r) * kScratch + half_at + k];
-                const float4 y = *reinterpret_cast<const float4*>(&room.t[(half_at + k) * kScratch + half_at + col]);
-                s.x = fmaf(w, y.x, s.x); s.y = fmaf(w, y.y, s.y); s.z = fmaf(w, y.z, s.z); s.w = fmaf(w, y.w, s.w);
-            }
-            *reinterpret_cast<float4*>(&room.x[r * kScratch + (tid >> 6) * 16 + col]) = s;
-            meet<kProducerThreads>(5);
-            s = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float w = -room.t[(half_at + 16 + r) * kScratch + half_at + 16 + k];
-                const float4 y = *reinterpret_cast<const float4*>(&room.x[k * kScratch + (tid >> 6) * 16 + col]);
-                s.x = fmaf(w, y.x, s.x); s.y = fmaf(w, y.y, s.y); s.z = fmaf(w, y.z, s.z); s.w = fmaf(w, y.w, s.w);
-            }
-            *reinterpret_cast<float4*>(&room.t[(half_at + 16 + r) * kScratch + half_at + col]) = s;
-            // above the diagonal blocks of each half the sums below read zeros
-            *reinterpret_cast<float4*>(&room.t[(half_at + r) * kScratch + half_at + 16 + col]) = make_float4(0, 0, 0, 0);
-            meet<kProducerThreads>(5);
-        }
-        {
-            const int r = tid >> 2, col = (tid & 3) * 8;
-            float4 s = make_float4(0, 0, 0, 0), u = s;
-#pragma unroll 8
-            for (int k = 0; k < 32; ++k) {
-                const float w = room.a[(32 + r) * kScratch + k];
-                const float4 y = *reinterpret_cast<const float4*>(&room.t[k * kScratch + col]);
-                const float4 z = *reinterpret_cast<const float4*>(&room.t[k * kScratch + col + 4]);
-                s.x = fmaf(w, y.x, s.x); s.y = fmaf(w, y.y, s.y); s.z = fmaf(w, y.z, s.z); s.w = fmaf(w, y.w, s.w);
-                u.x = fmaf(w, z.x, u.x); u.y = fmaf(w, z.y, u.y); u.z = fmaf(w, z.z, u.z); u.w = fmaf(w, z.w, u.w);
-            }
-            *reinterpret_cast<float4*>(&room.x[r * kScratch + col]) = s;
-            *reinterpret_cast<float4*>(&room.x[r * kScratch + col + 4]) = u;
-            meet<kProducerThreads>(5);
-            s = u = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-            for (int k = 0; k < 32; ++k) {
-                const float w = -room.t[(32 + r) * kScratch + 32 + k];
-                const float4 y = *reinterpret_cast<const float4*>(&room.x[k * kScratch + col]);
-                const float4 z = *reinterpret_cast<const float4*>(&room.x[k * kScratch + col + 4]);
-                s.x = fmaf(w, y.x, s.x); s.y = fmaf(w, y.y, s.y); s.z = fmaf(w, y.z, s.z); s.w = fmaf(w, y.w, s.w);
-                u.x = fmaf(w, z.x, u.x); u.y = fmaf(w, z.y, u.y); u.z = fmaf(w, z.z, u.z); u.w = fmaf(w, z.w, u.w);
-            }
-            *reinterpret_cast<float4*>(&room.t[(32 + r) * kScratch + col]) = s;
-            *reinterpret_cast<float4*>(&room.t[(32 + r) * kScratch + col + 4]) = u;
-            meet<kProducerThreads>(5);
-        }
-        // ---- T in two fp16 parts; the blocks above the diagonal blocks are not read
-#pragma unroll
-        for (int i = 0; i < kChunk * 8 / kProducerThreads; ++i) {
-            const int at = i * kProducerThreads + tid, r = at >> 3, chunk = at & 7;
-            if (chunk / 2 <= r / 16) {
-                uint32_t high[4], low[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 x = *reinterpret_cast<const float2*>(&room.t[r * kScratch + chunk * 8 + 2 * j]);
-                    split(x.x * kInverseScale, x.y * kInverseScale, high[j], low[j]);
-                }
-                *reinterpret_cast<uint4*>(buf.t_high + chunk_at<8>(r, chunk)) = make_uint4(high[0], high[1], high[2], high[3]);
-                *reinterpret_cast<uint4*>(buf.t_low + chunk_at<8>(r, chunk)) = make_uint4(low[0], low[1], low[2], low[3]);
-            }
-        }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
         pass<kAll>(1 + b);   // the buffer is full
     }
 }
 
-template <typename T, int kDim, int kConsumers>
-__device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kConsumers>& room, int begin, int end, int head, int slice, float* state) {
-    constexpr int kAll = kProducerThreads + kConsumers * 32, kChunks = kDim / 8, kValueChunks = kConsumers * 2;
+template <typename T, int kDim, int kGroupsOf>
+__device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int head, int slice, float* state) {
+    constexpr int kAll = kProducerThreads + kGroupsOf * 64, kChunks = kDim / 8, kValueChunks = kGroupsOf * 2;
+    constexpr int kKeys = kDim / 2;                      // per warp of a pair
     const skv_gdn_args& a = p.a;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kProducers, g = lane >> 2, c = lane & 3;
-    const int col0 = (slice * kConsumers + warp) * 16;   // the warp's value columns
-    // S^T: rows (value columns) g, g + 8; columns (keys) 8 i + 2c, 2c + 1
-    float s[kDim / 8][4];
+    const int half = warp & 1, group = warp >> 1, key0 = half * kKeys;
+    const int col0 = (slice * kGroupsOf + group) * 16;   // the pair's value columns
+    // S^T: rows (value columns) g, g + 8; columns (keys from key0 on) 8 i + 2c, 2c + 1
+    float s[kKeys / 8][4];
 #pragma unroll
-    for (int i = 0; i < kDim / 8; ++i)
+    for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = state[(i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8];
+        for (int j = 0; j < 4; ++j) s[i][j] = state[(key0 + i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8];
     T* out = static_cast<T*>(a.out) + head * kDim + col0 + 2 * c;
     int b = 0;
     for (int t0 = begin; t0 < end; t0 += kChunk, b ^= 1) {
         const auto& buf = room.buffer[b];
         float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kDim / 8; ++i)
+        for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(s[i][j]));
         const int s_power = power_for(warp_largest(top));
         const float s_down = power_of_two(-s_power), s_up = power_of_two(s_power);
-        meet<kAll>(1 + b);       // the buffer is full
-        // ---- S^T K^T and S^T Q^T
-        float ks[8][4], o[8][4];
+        meet<kAll>(1 + b);       // the buffer is full; and both warps of a pair have read what they handed over
+        const uint32_t k_at = smem_at(buf.k);
+        // ---- S^T K^T and S^T Q^T over the warp's keys
+        float ks[8][4], o[4][4];
+        {
+            float qs[8][4];
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
+            for (int t = 0; t < 8; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ks[t][j] = o[t][j] = 0.0f;
-        const uint32_t k_at = smem_at(buf.k), q_at = smem_at(buf.q);
+                for (int j = 0; j < 4; ++j) ks[t][j] = qs[t][j] = 0.0f;
+            const uint32_t q_at = smem_at(buf.q);
 #pragma unroll
-        for (int i = 0; i < kDim / 16; ++i) {
-            uint32_t high[4], low[4];
-            split(s[2 * i][0] * s_down, s[2 * i][1] * s_down, high[0], low[0]);
-            split(s[2 * i][2] * s_down, s[2 * i][3] * s_down, high[1], low[1]);
-            split(s[2 * i + 1][0] * s_down, s[2 * i + 1][1] * s_down, high[2], low[2]);
-            split(s[2 * i + 1][2] * s_down, s[2 * i + 1][3] * s_down, high[3], low[3]);
+            for (int i = 0; i < kKeys / 16; ++i) {
+                uint32_t high[4], low[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    split(s[2 * i + (j >> 1)][2 * (j & 1)] * s_down, s[2 * i + (j >> 1)][2 * (j & 1) + 1] * s_down, high[j], low[j]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    uint32_t m[4];
+                    const uint32_t at = chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1));
+                    load_matrices(m, k_at + at);
+                    multiply(ks[2 * t], high, m[0], m[1]);
+                    multiply(ks[2 * t + 1], high, m[2], m[3]);
+                    multiply(ks[2 * t], low, m[0], m[1]);
+                    multiply(ks[2 * t + 1], low, m[2], m[3]);
+                    load_matrices(m, q_at + at);
+                    multiply(qs[2 * t], high, m[0], m[1]);
+                    multiply(qs[2 * t + 1], high, m[2], m[3]);
+                }
+            }
+            // ---- the other half of the keys: all of K S, and Q S of the 32 tokens whose output this warp writes
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                room.meet[warp][t][lane] = make_float4(ks[t][0] * s_up, ks[t][1] * s_up, ks[t][2] * s_up, ks[t][3] * s_up);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                uint32_t m[4];
-                const uint32_t at = chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1));
-                load_matrices(m, k_at + at);
-                multiply(ks[2 * t], high, m[0], m[1]);
-                multiply(ks[2 * t + 1], high, m[2], m[3]);
-                multiply(ks[2 * t], low, m[0], m[1]);
-                multiply(ks[2 * t + 1], low, m[2], m[3]);
-                load_matrices(m, q_at + at);
-                multiply(o[2 * t], high, m[0], m[1]);
-                multiply(o[2 * t + 1], high, m[2], m[3]);
+                room.meet[warp][8 + t][lane] =
+                    make_float4((half ? qs[t][0] : qs[4 + t][0]) * s_up, (half ? qs[t][1] : qs[4 + t][1]) * s_up,
+                                (half ? qs[t][2] : qs[4 + t][2]) * s_up, (half ? qs[t][3] : qs[4 + t][3]) * s_up);
+            }
+            if (lane == 0) room.power[warp] = s_power;
+            meet<64>(6 + group);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float4 x = room.meet[warp ^ 1][t][lane];
+                ks[t][0] = fmaf(ks[t][0], s_up, x.x);
+                ks[t][1] = fmaf(ks[t][1], s_up, x.y);
+                ks[t][2] = fmaf(ks[t][2], s_up, x.z);
+                ks[t][3] = fmaf(ks[t][3], s_up, x.w);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float4 x = room.meet[warp ^ 1][8 + t][lane];
+                o[t][0] = fmaf(half ? qs[4 + t][0] : qs[t][0], s_up, x.x);
+                o[t][1] = fmaf(half ? qs[4 + t][1] : qs[t][1], s_up, x.y);
+                o[t][2] = fmaf(half ? qs[4 + t][2] : qs[t][2], s_up, x.z);
+                o[t][3] = fmaf(half ? qs[4 + t][3] : qs[t][3], s_up, x.w);
             }
         }
+        const int o_least = max(max(s_power, room.power[warp ^ 1]) - 60, -120);
         // ---- R = beta (V - e^G K S), in place of K S
         top = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             uint32_t m[4];
-            load_matrices_t(m, smem_at(buf.v) + chunk_at<kValueChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), warp * 2 + ((lane >> 3) & 1)));
+            load_matrices_t(m, smem_at(buf.v) + chunk_at<kValueChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), group * 2 + ((lane >> 3) & 1)));
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int at = (2 * t + u) * 8 + 2 * c;
-                const float2 fv = *reinterpret_cast<const float2*>(&buf.f.value[at]);
-                float2 fk = *reinterpret_cast<const float2*>(&buf.f.key[at]);
-                fk.x *= s_up;
-                fk.y *= s_up;
+                const float2 fv = *reinterpret_cast<const float2*>(&buf.record.f.value[at]);
+                const float2 fk = *reinterpret_cast<const float2*>(&buf.record.f.key[at]);
                 const float2 v0 = Pair<T>::up(m[2 * u]), v1 = Pair<T>::up(m[2 * u + 1]);
                 float (&r)[4] = ks[2 * t + u];
                 r[0] = fv.x * v0.x - fk.x * r[0];
@@ -584,13 +775,13 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kCons
 #pragma unroll
                 for (int t = i; t < 4; ++t) {
                     uint32_t m[4];
-                    const uint32_t at = chunk_at<8>(t * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1));
-                    load_matrices(m, smem_at(buf.t_high) + at);
+                    const uint32_t at = block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+                    load_matrices(m, smem_at(buf.record.t_high) + at);
                     multiply(v[2 * t], high[i], m[0], m[1]);
                     multiply(v[2 * t + 1], high[i], m[2], m[3]);
                     multiply(v[2 * t], low[i], m[0], m[1]);
                     multiply(v[2 * t + 1], low[i], m[2], m[3]);
-                    load_matrices(m, smem_at(buf.t_low) + at);
+                    load_matrices(m, smem_at(buf.record.t_low) + at);
                     multiply(v[2 * t], high[i], m[0], m[1]);
                     multiply(v[2 * t + 1], high[i], m[2], m[3]);
                 }
@@ -606,7 +797,7 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kCons
             float w[8][4];
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                const float2 f = *reinterpret_cast<const float2*>(&buf.f.update[t * 8 + 2 * c]);
+                const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.update[t * 8 + 2 * c]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     w[t][j] = v[t][j] * (j & 1 ? f.y : f.x);
@@ -617,16 +808,16 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kCons
             // one power for S and the update: the update's, or 2^-60 of what S would need where the update is smaller yet
             int w_power = exponent_of(warp_largest(top)) - 14 + v_unit;
             w_power = min(max(w_power, max(s_power - 60, -120)), 120);
-            o_power = min(max(exponent_of(warp_largest(most)) - 14 + v_unit, max(s_power - 60, -120)), 120);
+            o_power = min(max(exponent_of(warp_largest(most)) - 14 + v_unit, o_least), 120);
             const float w_down = power_of_two(v_unit - w_power), v_down = power_of_two(v_unit - o_power);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     first[t][j] = Pair<__half>::down(v[2 * t + (j >> 1)][2 * (j & 1)] * v_down, v[2 * t + (j >> 1)][2 * (j & 1) + 1] * v_down);
-            const float keep = buf.f.whole * power_of_two(-w_power), up = power_of_two(w_power);
+            const float keep = buf.record.f.whole * power_of_two(-w_power), up = power_of_two(w_power);
 #pragma unroll
-            for (int i = 0; i < kDim / 8; ++i)
+            for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[i][j] *= keep;
 #pragma unroll
@@ -636,9 +827,9 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kCons
                 for (int j = 0; j < 4; ++j)
                     split(w[2 * t + (j >> 1)][2 * (j & 1)] * w_down, w[2 * t + (j >> 1)][2 * (j & 1) + 1] * w_down, high[j], low[j]);
 #pragma unroll
-                for (int i = 0; i < kDim / 16; ++i) {
+                for (int i = 0; i < kKeys / 16; ++i) {
                     uint32_t m[4];
-                    load_matrices_t(m, k_at + chunk_at<kChunks>(t * 16 + (lane & 15), 2 * i + (lane >> 4)));
+                    load_matrices_t(m, k_at + chunk_at<kChunks>(t * 16 + (lane & 15), key0 / 8 + 2 * i + (lane >> 4)));
                     multiply(s[2 * i], high, m[0], m[1]);
                     multiply(s[2 * i + 1], high, m[2], m[3]);
                     multiply(s[2 * i], low, m[0], m[1]);
@@ -646,38 +837,42 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kCons
                 }
             }
 #pragma unroll
-            for (int i = 0; i < kDim / 8; ++i)
+            for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[i][j] *= up;
         }
-        // ---- O = scale (e^G Q S + P V')
-        const float o_fit = power_of_two(s_power - o_power), o_up = power_of_two(o_power);
+        // ---- O = scale (e^G Q S + P V') of the warp's 32 tokens
+        const float o_down = power_of_two(-o_power), o_up = power_of_two(o_power);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const float2 f = *reinterpret_cast<const float2*>(&buf.f.query[t * 8 + 2 * c]);
-            o[t][0] *= f.x * o_fit;
-            o[t][1] *= f.y * o_fit;
-            o[t][2] *= f.x * o_fit;
-            o[t][3] *= f.y * o_fit;
+        for (int t = 0; t < 4; ++t) {
+            const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.query[half * 32 + t * 8 + 2 * c]);
+            o[t][0] *= f.x * o_down;
+            o[t][1] *= f.y * o_down;
+            o[t][2] *= f.x * o_down;
+            o[t][3] *= f.y * o_down;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int t = i; t < 4; ++t) {
-                uint32_t m[4];
-                load_matrices(m, smem_at(buf.mix) + chunk_at<8>(t * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
-                multiply(o[2 * t], first[i], m[0], m[1]);
-                multiply(o[2 * t + 1], first[i], m[2], m[3]);
+            for (int u = 0; u < 2; ++u) {
+                const int t = half * 2 + u;
+                if (i <= t) {
+                    uint32_t m[4];
+                    load_matrices(m, smem_at(buf.record.mix) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
+                    multiply(o[2 * u], first[i], m[0], m[1]);
+                    multiply(o[2 * u + 1], first[i], m[2], m[3]);
+                }
             }
         }
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            float2 f = *reinterpret_cast<const float2*>(&buf.f.out[t * 8 + 2 * c]);
+        for (int t = 0; t < 4; ++t) {
+            const int in = half * 32 + t * 8;
+            float2 f = *reinterpret_cast<const float2*>(&buf.record.f.out[in + 2 * c]);
             f.x *= o_up;
             f.y *= o_up;
             const uint32_t lo = transpose8(Pair<T>::down(o[t][0] * f.x, o[t][1] * f.y));
             const uint32_t hi = transpose8(Pair<T>::down(o[t][2] * f.x, o[t][3] * f.y));
-            const int token = t0 + t * 8 + g;
+            const int token = t0 + in + g;
             if (token < end) {
                 *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride) = lo;
                 *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride + 8) = hi;
@@ -686,16 +881,16 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kCons
         if (t0 + 2 * kChunk < end) pass<kAll>(3 + b);   // the buffer may be filled again
     }
 #pragma unroll
-    for (int i = 0; i < kDim / 8; ++i)
+    for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) state[(i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8] = s[i][j];
+        for (int j = 0; j < 4; ++j) state[(key0 + i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8] = s[i][j];
 }
 
-template <typename T, int kDim, int kConsumers>
-__global__ void __launch_bounds__(kProducerThreads + kConsumers * 32, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
+template <typename T, int kDim, int kGroupsOf>
+__global__ void __launch_bounds__(kProducerThreads + kGroupsOf * 64, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    auto& room = *reinterpret_cast<ChunkRoom<kDim, kConsumers>*>(smem);
-    constexpr int kSlices = kDim / (kConsumers * 16);
+    auto& room = *reinterpret_cast<ChunkRoom<kDim, kGroupsOf>*>(smem);
+    constexpr int kSlices = kDim / (kGroupsOf * 16);
     const skv_gdn_args& a = p.a;
     const int slice = blockIdx.x % kSlices;
     const int64_t item = blockIdx.x / kSlices;
@@ -704,8 +899,8 @@ __global__ void __launch_bounds__(kProducerThreads + kConsumers * 32, 1) chunk_k
     if (!tokens_of(a, seq, begin, end)) return;
     float* const state = state_of(p, seq, head, kDim);
     if (!state) return;
-    if (threadIdx.x < kProducerThreads) produce<T, kDim, kConsumers>(p, room, begin, end, head, slice);
-    else consume<T, kDim, kConsumers>(p, room, begin, end, head, slice, state);
+    if (threadIdx.x < kProducerThreads) load_chunks<T, kDim, kGroupsOf>(p, room, begin, end, seq, head, slice);
+    else consume<T, kDim, kGroupsOf>(p, room, begin, end, head, slice, state);
 }
 
 template <typename T>
@@ -716,20 +911,24 @@ cudaError_t launch_tokens(const DeltaDev& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <typename T, int kDim, int kConsumers>
+template <typename T, int kDim, int kGroupsOf>
 cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
-    constexpr int kSmem = sizeof(ChunkRoom<kDim, kConsumers>);
+    constexpr int kSmem = sizeof(ChunkRoom<kDim, kGroupsOf>), kPrepare = sizeof(PrepareRoom<kDim>);
     static_assert(kSmem <= 227 * 1024, "the buffers fit an SM");
-    const cudaError_t e = cudaFuncSetAttribute(chunk_kernel<T, kDim, kConsumers>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaError_t e = cudaFuncSetAttribute(prepare_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepare);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_kernel<T, kDim, kGroupsOf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    const unsigned grid = (unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * (kDim / (kConsumers * 16)));
-    chunk_kernel<T, kDim, kConsumers><<<grid, kProducerThreads + kConsumers * 32, kSmem, stream>>>(p);
+    prepare_kernel<T, kDim><<<(unsigned) (record_slots(p.a.n_tokens, p.a.n_seqs) * p.a.n_v_heads), kProducerThreads, kPrepare, stream>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const unsigned grid = (unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * (kDim / (kGroupsOf * 16)));
+    chunk_kernel<T, kDim, kGroupsOf><<<grid, kProducerThreads + kGroupsOf * 64, kSmem, stream>>>(p);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch(const DeltaDev& p, int sms, cudaStream_t stream) {
-    if (p.a.max_tokens < kChunksFrom) return launch_tokens<T>(p, stream);
+    if (!chunked(p.a.seq_starts != nullptr, p.a.max_tokens)) return launch_tokens<T>(p, stream);
     const bool few = (int64_t) p.a.n_seqs * p.a.n_v_heads * (p.a.head_dim / 32) <= sms;
     if (p.a.head_dim == 64) return few ? launch_chunks<T, 64, 2>(p, stream) : launch_chunks<T, 64, 4>(p, stream);
     return few ? launch_chunks<T, 128, 2>(p, stream) : launch_chunks<T, 128, 4>(p, stream);
@@ -747,6 +946,7 @@ int skv_gated_delta_workspace(int n_tokens, int n_seqs, int n_v_heads, int head_
     *out_bytes = 0;
     if (n_tokens < 0 || n_seqs < 0 || n_v_heads < 1 || max_tokens < 0 || (head_dim != 64 && head_dim != 128))
         return fail(SKV_EINVAL, "skv_gated_delta_workspace: bad sizes");
+    if (chunked(true, max_tokens)) *out_bytes = ((uint64_t) record_slots(n_tokens, n_seqs) * n_v_heads * sizeof(Record) + 255) / 256 * 256;
     return SKV_OK;
 }
 
@@ -774,7 +974,8 @@ int skv_gated_delta(const skv_gdn_args* args, void* stream) {
     if (a.state_rows < 1 || (a.state_rows > 1 && a.state_stride < vw * a.head_dim)) return no("the state rows overlap or are none");
     if (!a.state_index && a.state_rows < a.n_seqs) return no("fewer state rows than sequences");
     uint64_t need = 0;
-    if (const int rc = skv_gated_delta_workspace(a.n_tokens, a.n_seqs, a.n_v_heads, a.head_dim, a.max_tokens, &need)) return rc;
+    if (const int rc = skv_gated_delta_workspace(a.n_tokens, a.n_seqs, a.n_v_heads, a.head_dim, a.seq_starts ? a.max_tokens : 1, &need)) return rc;
+    if (need / sizeof(Record) > INT32_MAX) return fail(SKV_ERANGE, "skv_gated_delta: too many tokens and heads");
     if (need && (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255u) || a.workspace_bytes < need))
         return no("the workspace must be 256-byte aligned and as large as skv_gated_delta_workspace says");
     DeviceCtx* ctx = current_ctx();
@@ -783,6 +984,7 @@ int skv_gated_delta(const skv_gdn_args* args, void* stream) {
     DeltaDev p{};
     p.a = a;
     p.status = ctx->status;
+    p.records = static_cast<Record*>(a.workspace);
     p.ratio = a.n_v_heads / a.n_k_heads;
     const auto s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = a.dtype == SKV_DTYPE_F16 ? launch<__half>(p, ctx->sms, s) : launch<__nv_bfloat16>(p, ctx->sms, s);
