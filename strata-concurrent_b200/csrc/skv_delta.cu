@@ -178,13 +178,13 @@ __device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 template <int kThreadsOf>
@@ -290,18 +290,19 @@ struct PrepareRoom {
     float2 sums[kChunk];      // G log2 e in two parts
     double carry[2];          // the first 32 tokens' sum, and all
     float beta[kChunk];
+    int power[kChunk];        // of the query rows
     float largest[4];
 };
 
-/// Blocks (kRow, kFrom .. kTo - 1) of K K^T and Q K^T: 16 tokens against 16 (kTo - kFrom).
+/// Blocks (row, from), (row, from + 1) .. of K K^T and Q K^T, two tiles of eight tokens each from tile `at` on.
 template <int kDim, int kBlocks>
-__device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, int row, int from, float (&kk)[2 * kBlocks][4], float (&qk)[2 * kBlocks][4]) {
+__device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, int row, int from, int at, float (&kk)[6][4], float (&qk)[6][4]) {
     constexpr int kChunks = kDim / 8;
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int t = 0; t < 2 * kBlocks; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kk[t][j] = qk[t][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) kk[at + t][j] = qk[at + t][j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i) {
         uint32_t x[4], y[4];
@@ -311,16 +312,16 @@ __device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, int row, 
         for (int t = 0; t < kBlocks; ++t) {
             uint32_t m[4];
             load_matrices(m, k_at + chunk_at<kChunks>((from + t) * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
-            multiply(kk[2 * t], x, m[0], m[1]);
-            multiply(kk[2 * t + 1], x, m[2], m[3]);
-            multiply(qk[2 * t], y, m[0], m[1]);
-            multiply(qk[2 * t + 1], y, m[2], m[3]);
+            multiply(kk[at + 2 * t], x, m[0], m[1]);
+            multiply(kk[at + 2 * t + 1], x, m[2], m[3]);
+            multiply(qk[at + 2 * t], y, m[0], m[1]);
+            multiply(qk[at + 2 * t + 1], y, m[2], m[3]);
         }
     }
 }
 /// A (32 bits) and P (fp16) of those blocks.
 template <int kDim, int kBlocks>
-__device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int block_row, int from, const float (&kk)[2 * kBlocks][4], const float (&qk)[2 * kBlocks][4]) {
+__device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int block_row, int from, int at, const float (&kk)[6][4], const float (&qk)[6][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -334,14 +335,15 @@ __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int
             // a decay of zero (and what lies above the diagonal) wipes out even an infinite product
             const float d0 = exp2f((sum.x - other.x) + (sum.y - other.y)), d1 = exp2f((sum.x - other.z) + (sum.y - other.w));
             *reinterpret_cast<float2*>(&room.work.a[row * kScratch + col]) =
-                make_float2(col < row ? by * d0 * kk[t][2 * h] : 0.0f, col + 1 < row ? by * d1 * kk[t][2 * h + 1] : 0.0f);
+                make_float2(col < row ? by * d0 * kk[at + t][2 * h] : 0.0f, col + 1 < row ? by * d1 * kk[at + t][2 * h + 1] : 0.0f);
             *reinterpret_cast<uint32_t*>(room.mix + block_of(block_row, from + t / 2) * kBlockBytes + half_row_at(in, t & 1) + c * 4) =
-                Pair<__half>::down(col <= row ? d0 * qk[t][2 * h] : 0.0f, col + 1 <= row ? d1 * qk[t][2 * h + 1] : 0.0f);
+                Pair<__half>::down(col <= row ? d0 * qk[at + t][2 * h] : 0.0f, col + 1 <= row ? d1 * qk[at + t][2 * h + 1] : 0.0f);
         }
     }
 }
 
-/// One chunk of one head.  Four warps; four CTAs an SM hide the short phases' latencies.
+/// One chunk of one key head, for all of its value heads: K, Q and their products serve them all.  Four warps; four CTAs
+/// an SM hide the short phases' latencies.
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __grid_constant__ DeltaDev p) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -349,13 +351,13 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
     constexpr int kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
     const skv_gdn_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int head = (int) (blockIdx.x % a.n_v_heads);
-    const int64_t slot = blockIdx.x / a.n_v_heads;
+    const int key_head = (int) (blockIdx.x % a.n_k_heads);
+    const int64_t slot = blockIdx.x / a.n_k_heads;
     // the last sequence whose slots begin at or before this one
     int lo = 0, hi = a.n_seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        const int at = a.seq_starts ? min(max(__ldg(a.seq_starts + mid), 0), a.n_tokens) : mid;
+        const int at = min(max(__ldg(a.seq_starts + mid), 0), a.n_tokens);
         if (first_slot(at, mid) <= slot) lo = mid;
         else hi = mid;
     }
@@ -364,54 +366,28 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
     const int64_t chunk_of = slot - first_slot(begin, lo);
     if (chunk_of < 0 || chunk_of * kChunk >= end - begin) return;
     const int t0 = begin + (int) chunk_of * kChunk;
-    Record& record = p.records[slot * a.n_v_heads + head];
 
     // ---- K and Q as fp16
-    const T* qh = static_cast<const T*>(a.q) + (head / p.ratio) * kDim;
-    const T* kh = static_cast<const T*>(a.k) + (head / p.ratio) * kDim;
-    uint4 k[kMine];
-    float top = 0.0f;
+    const T* qh = static_cast<const T*>(a.q) + key_head * kDim;
+    const T* kh = static_cast<const T*>(a.k) + key_head * kDim;
+    uint4 k[kMine], q[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
         const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
         const bool on = t0 + r < end;
         k[i] = on ? __ldg(reinterpret_cast<const uint4*>(kh + (int64_t) (t0 + r) * a.k_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
+        q[i] = on ? __ldg(reinterpret_cast<const uint4*>(qh + (int64_t) (t0 + r) * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
     }
-    float g = 0.0f, beta = 0.0f;
-    if (tid < kChunk && t0 + tid < end) {
-        g = __ldg(a.g + (int64_t) (t0 + tid) * a.g_stride + head);
-        beta = __ldg(a.beta + (int64_t) (t0 + tid) * a.beta_stride + head);
-    }
+    int key_power = 0;
+    if constexpr (!std::is_same<T, __half>::value) {
+        float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
-        const bool on = t0 + r < end;
-        uint4 q = on ? __ldg(reinterpret_cast<const uint4*>(qh + (int64_t) (t0 + r) * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
-        int power = 0;
-        if constexpr (!std::is_same<T, __half>::value) {
-            float x[8], most = 0.0f;
-            unpack8<T>(q, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-#pragma unroll
-            for (int m = 1; m < kChunks; m <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-            power = most > 0.0f && most < INFINITY ? min(max(exponent_of(most), -126), 126) : 0;
-            const float down = power_of_two(-power);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= down;
-            q = pack8<__half>(x);
+        for (int i = 0; i < kMine; ++i) {
+            float x[8];
             unpack8<T>(k[i], x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
         }
-        *reinterpret_cast<uint4*>(room.in.q + chunk_at<kChunks>(r, chunk)) = q;
-        if (chunk == 0) {
-            record.f.out[r] = a.scale * power_of_two(power);
-            record.f.down[r] = power_of_two(-power);
-        }
-    }
-    int key_power = 0;
-    if constexpr (!std::is_same<T, __half>::value) {
         top = warp_largest(top);
         if (lane == 0) room.largest[warp] = top;
         __syncthreads();
@@ -421,157 +397,179 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
         const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+        int power = 0;
         if constexpr (!std::is_same<T, __half>::value) {
-            float x[8];
+            float x[8], most = 0.0f;
             unpack8<T>(k[i], x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] *= power_of_two(-key_power);
             k[i] = pack8<__half>(x);
+            unpack8<T>(q[i], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+#pragma unroll
+            for (int m = 1; m < kChunks; m <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
+            power = most > 0.0f && most < INFINITY ? min(max(exponent_of(most), -126), 126) : 0;
+            const float down = power_of_two(-power);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= down;
+            q[i] = pack8<__half>(x);
         }
         *reinterpret_cast<uint4*>(room.in.k + chunk_at<kChunks>(r, chunk)) = k[i];
-    }
-    // ---- the decays: a token per lane of two warps, sums in 64 bits
-    const float fit = power_of_two(key_power);
-    double sum = g < -200.0f ? -200.0 : (double) g;
-    if (warp < 2) {
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const double o = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += o;
-        }
-        if (tid == 31) room.carry[0] = sum;
+        *reinterpret_cast<uint4*>(room.in.q + chunk_at<kChunks>(r, chunk)) = q[i];
+        if (chunk == 0) room.power[r] = power;
     }
     __syncthreads();
-    if (warp < 2) {
-        if (warp == 1) sum += room.carry[0];
-        if (tid == 63) room.carry[1] = sum;
-        const double turns = sum * 1.4426950408889634074;   // log2 e
-        const float high = (float) turns;
-        room.sums[tid] = make_float2(high, (float) (turns - (double) high));
-        room.beta[tid] = beta;
-    }
-    __syncthreads();
-    if (warp < 2) {
-        const double all = room.carry[1];
-        const float into = expf((float) sum);
-        record.f.value[tid] = fit * beta;
-        record.f.key[tid] = fit * fit * beta * into;
-        record.f.query[tid] = into;
-        record.f.update[tid] = expf((float) (all - sum));
-        if (tid == 0) {
-            record.f.whole = expf((float) all);
-            record.f.key_down = power_of_two(-key_power);
-        }
-    }
     // ---- K K^T and Q K^T on and below the diagonal: ten blocks of 16 x 16, at most three a warp
     const uint32_t k_at = smem_at(room.in.k), q_at = smem_at(room.in.q);
-    const float fit2 = fit * fit;
-    if (warp < 2) {            // row 3, two blocks each
-        float kk[4][4], qk[4][4];
-        products<kDim, 2>(k_at, q_at, 3, 2 * warp, kk, qk);
-        meet<kProducerThreads>(1);   // the scratch matrices lie where K and Q are
-        decayed<kDim, 2>(room, fit2, 3, 2 * warp, kk, qk);
-    } else if (warp == 2) {    // row 2
-        float kk[6][4], qk[6][4];
-        products<kDim, 3>(k_at, q_at, 2, 0, kk, qk);
-        meet<kProducerThreads>(1);
-        decayed<kDim, 3>(room, fit2, 2, 0, kk, qk);
-    } else {                   // rows 1 and 0
-        float kk[4][4], qk[4][4], kk0[2][4], qk0[2][4];
-        products<kDim, 2>(k_at, q_at, 1, 0, kk, qk);
-        products<kDim, 1>(k_at, q_at, 0, 0, kk0, qk0);
-        meet<kProducerThreads>(1);
-        decayed<kDim, 2>(room, fit2, 1, 0, kk, qk);
-        decayed<kDim, 1>(room, fit2, 0, 0, kk0, qk0);
+    float kk[6][4], qk[6][4];
+    if (warp < 2) products<kDim, 2>(k_at, q_at, 3, 2 * warp, 0, kk, qk);   // row 3, two blocks each
+    else if (warp == 2) products<kDim, 3>(k_at, q_at, 2, 0, 0, kk, qk);    // row 2
+    else {
+        products<kDim, 2>(k_at, q_at, 1, 0, 0, kk, qk);                    // rows 1 and 0
+        products<kDim, 1>(k_at, q_at, 0, 0, 4, kk, qk);
     }
-    __syncthreads();
-    // ---- T = (I + A)^-1: the diagonal blocks of 16 by substitution, a column per thread
+    __syncthreads();   // the scratch matrices lie where K and Q are
+
+    const float fit = power_of_two(key_power), fit2 = fit * fit;
     auto& work = room.work;
-    if (tid < kChunk) {
-        const int base = tid & ~15, col = tid & 15;
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float r[16];
-#pragma unroll
-            for (int j = 0; j < (i + 3) / 4; ++j)
-                *reinterpret_cast<float4*>(&r[4 * j]) = *reinterpret_cast<const float4*>(&work.a[(base + i) * kScratch + base + 4 * j]);
-            float s0 = i == col ? 1.0f : 0.0f, s1 = 0.0f;
-#pragma unroll
-            for (int j = 0; j < i; ++j) {
-                if (j & 1) s1 = fmaf(-r[j], x[j], s1);
-                else s0 = fmaf(-r[j], x[j], s0);
+    for (int head = key_head * p.ratio; head < (key_head + 1) * p.ratio; ++head) {
+        Record& record = p.records[slot * a.n_v_heads + head];
+        // ---- the decays: a token per lane of two warps, sums in 64 bits
+        float g = 0.0f, beta = 0.0f;
+        double sum = 0.0;
+        if (warp < 2) {
+            if (t0 + tid < end) {
+                g = __ldg(a.g + (int64_t) (t0 + tid) * a.g_stride + head);
+                beta = __ldg(a.beta + (int64_t) (t0 + tid) * a.beta_stride + head);
             }
-            x[i] = s0 + s1;
-        }
+            sum = g < -200.0f ? -200.0 : (double) g;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) work.t[(base + i) * kScratch + base + col] = x[i];
-    } else {
-        // above the diagonal blocks of each half the products below read zeros
-        for (int i = tid - kChunk; i < 2 * 16 * 16; i += kChunk)
-            work.t[(i / 256 * 32 + i % 256 / 16) * kScratch + i / 256 * 32 + 16 + i % 16] = 0.0f;
-    }
-    __syncthreads();
-    // below them T21 = -T22 (A21 T11): the blocks of 16 of each half, then the block of 32, eight columns a warp
-    constexpr float kUnit = kInverseScale, kDown = 1.0f / (kUnit * kUnit);
-    uint32_t ah[4], al[4], bh[2], bl[2];
-    {
-        const int at = (warp >> 1) * 32, col = (warp & 1) * 8;
-        float c[4] = {0, 0, 0, 0}, d[4] = {0, 0, 0, 0};
-        left_parts(&work.a[(at + 16) * kScratch + at], kUnit, ah, al);
-        right_parts(&work.t[at * kScratch + at + col], kUnit, bh, bl);
-        multiply_parts(c, ah, al, bh, bl);
-        store_product(&work.x[(warp >> 1) * 16 * kScratch + col], kDown, c);
-        __syncwarp();
-        left_parts(&work.t[(at + 16) * kScratch + at + 16], -kUnit, ah, al);
-        right_parts(&work.x[(warp >> 1) * 16 * kScratch + col], kUnit, bh, bl);
-        multiply_parts(d, ah, al, bh, bl);
-        store_product(&work.t[(at + 16) * kScratch + at + col], kDown, d);
-    }
-    __syncthreads();
-    {
-        const int col = warp * 8;
-        float c[2][4] = {}, d[2][4] = {};
-#pragma unroll
-        for (int k16 = 0; k16 < 2; ++k16) {
-            right_parts(&work.t[k16 * 16 * kScratch + col], kUnit, bh, bl);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                left_parts(&work.a[(32 + m * 16) * kScratch + k16 * 16], kUnit, ah, al);
-                multiply_parts(c[m], ah, al, bh, bl);
+            for (int d = 1; d < 32; d <<= 1) {
+                const double o = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += o;
             }
+            if (tid == 31) room.carry[0] = sum;
         }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) store_product(&work.x[m * 16 * kScratch + col], kDown, c[m]);
-        __syncwarp();
-#pragma unroll
-        for (int k16 = 0; k16 < 2; ++k16) {
-            right_parts(&work.x[k16 * 16 * kScratch + col], kUnit, bh, bl);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                left_parts(&work.t[(32 + m * 16) * kScratch + 32 + k16 * 16], -kUnit, ah, al);
-                multiply_parts(d[m], ah, al, bh, bl);
+        __syncthreads();
+        if (warp < 2) {
+            if (warp == 1) sum += room.carry[0];
+            if (tid == 63) room.carry[1] = sum;
+            const double turns = sum * 1.4426950408889634074;   // log2 e
+            const float high = (float) turns;
+            room.sums[tid] = make_float2(high, (float) (turns - (double) high));
+            room.beta[tid] = beta;
+        }
+        __syncthreads();
+        if (warp < 2) {
+            const double all = room.carry[1];
+            const float into = expf((float) sum);
+            record.f.value[tid] = fit * beta;
+            record.f.key[tid] = fit2 * beta * into;
+            record.f.query[tid] = into;
+            record.f.update[tid] = expf((float) (all - sum));
+            record.f.out[tid] = a.scale * power_of_two(room.power[tid]);
+            record.f.down[tid] = power_of_two(-room.power[tid]);
+            if (tid == 0) {
+                record.f.whole = expf((float) all);
+                record.f.key_down = power_of_two(-key_power);
             }
+            decayed<kDim, 2>(room, fit2, 3, 2 * warp, 0, kk, qk);
+        } else if (warp == 2) {
+            decayed<kDim, 3>(room, fit2, 2, 0, 0, kk, qk);
+        } else {
+            decayed<kDim, 2>(room, fit2, 1, 0, 0, kk, qk);
+            decayed<kDim, 1>(room, fit2, 0, 0, 4, kk, qk);
         }
+        __syncthreads();
+        // ---- T = (I + A)^-1: the diagonal blocks of 16 by substitution, a column per thread
+        if (tid < kChunk) {
+            const int base = tid & ~15, col = tid & 15;
+            float x[16];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) store_product(&work.t[(32 + m * 16) * kScratch + col], kDown, d[m]);
-    }
-    __syncthreads();
-    // ---- T in two fp16 parts, and P
-    for (int at = tid; at < kTriangleBytes / 16; at += kProducerThreads) {
-        const int block = at / 32, r = at % 32 / 2, chunk = at % 2;
-        const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3, j = block - block_of(i, 0);
-        const float4* x = reinterpret_cast<const float4*>(&work.t[(i * 16 + r) * kScratch + j * 16 + chunk * 8]);
-        const float4 u = x[0], v = x[1];
-        uint32_t high[4], low[4];
-        split(u.x * kUnit, u.y * kUnit, high[0], low[0]);
-        split(u.z * kUnit, u.w * kUnit, high[1], low[1]);
-        split(v.x * kUnit, v.y * kUnit, high[2], low[2]);
-        split(v.z * kUnit, v.w * kUnit, high[3], low[3]);
-        const uint32_t to = block * kBlockBytes + half_row_at(r, chunk);
-        *reinterpret_cast<uint4*>(record.t_high + to) = make_uint4(high[0], high[1], high[2], high[3]);
-        *reinterpret_cast<uint4*>(record.t_low + to) = make_uint4(low[0], low[1], low[2], low[3]);
-        *reinterpret_cast<uint4*>(record.mix + at * 16) = *reinterpret_cast<const uint4*>(room.mix + at * 16);
+            for (int i = 0; i < 16; ++i) {
+                float r[16];
+#pragma unroll
+                for (int j = 0; j < (i + 3) / 4; ++j)
+                    *reinterpret_cast<float4*>(&r[4 * j]) = *reinterpret_cast<const float4*>(&work.a[(base + i) * kScratch + base + 4 * j]);
+                float s0 = i == col ? 1.0f : 0.0f, s1 = 0.0f;
+#pragma unroll
+                for (int j = 0; j < i; ++j) {
+                    if (j & 1) s1 = fmaf(-r[j], x[j], s1);
+                    else s0 = fmaf(-r[j], x[j], s0);
+                }
+                x[i] = s0 + s1;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) work.t[(base + i) * kScratch + base + col] = x[i];
+        } else {
+            // above the diagonal blocks of each half the products below read zeros
+            for (int i = tid - kChunk; i < 2 * 16 * 16; i += kChunk)
+                work.t[(i / 256 * 32 + i % 256 / 16) * kScratch + i / 256 * 32 + 16 + i % 16] = 0.0f;
+        }
+        __syncthreads();
+        // below them T21 = -T22 (A21 T11): the blocks of 16 of each half, then the block of 32, eight columns a warp
+        constexpr float kUnit = kInverseScale, kDown = 1.0f / (kUnit * kUnit);
+        uint32_t ah[4], al[4], bh[2], bl[2];
+        {
+            const int at = (warp >> 1) * 32, col = (warp & 1) * 8;
+            float c[4] = {0, 0, 0, 0}, d[4] = {0, 0, 0, 0};
+            left_parts(&work.a[(at + 16) * kScratch + at], kUnit, ah, al);
+            right_parts(&work.t[at * kScratch + at + col], kUnit, bh, bl);
+            multiply_parts(c, ah, al, bh, bl);
+            store_product(&work.x[(warp >> 1) * 16 * kScratch + col], kDown, c);
+            __syncwarp();
+            left_parts(&work.t[(at + 16) * kScratch + at + 16], -kUnit, ah, al);
+            right_parts(&work.x[(warp >> 1) * 16 * kScratch + col], kUnit, bh, bl);
+            multiply_parts(d, ah, al, bh, bl);
+            store_product(&work.t[(at + 16) * kScratch + at + col], kDown, d);
+        }
+        __syncthreads();
+        {
+            const int col = warp * 8;
+            float c[2][4] = {}, d[2][4] = {};
+#pragma unroll
+            for (int k16 = 0; k16 < 2; ++k16) {
+                right_parts(&work.t[k16 * 16 * kScratch + col], kUnit, bh, bl);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    left_parts(&work.a[(32 + m * 16) * kScratch + k16 * 16], kUnit, ah, al);
+                    multiply_parts(c[m], ah, al, bh, bl);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m) store_product(&work.x[m * 16 * kScratch + col], kDown, c[m]);
+            __syncwarp();
+#pragma unroll
+            for (int k16 = 0; k16 < 2; ++k16) {
+                right_parts(&work.x[k16 * 16 * kScratch + col], kUnit, bh, bl);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    left_parts(&work.t[(32 + m * 16) * kScratch + 32 + k16 * 16], -kUnit, ah, al);
+                    multiply_parts(d[m], ah, al, bh, bl);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m) store_product(&work.t[(32 + m * 16) * kScratch + col], kDown, d[m]);
+        }
+        __syncthreads();
+        // ---- T in two fp16 parts, and P
+        for (int at = tid; at < kTriangleBytes / 16; at += kProducerThreads) {
+            const int block = at / 32, r = at % 32 / 2, chunk = at % 2;
+            const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3, j = block - block_of(i, 0);
+            const float4* x = reinterpret_cast<const float4*>(&work.t[(i * 16 + r) * kScratch + j * 16 + chunk * 8]);
+            const float4 u = x[0], v = x[1];
+            uint32_t high[4], low[4];
+            split(u.x * kUnit, u.y * kUnit, high[0], low[0]);
+            split(u.z * kUnit, u.w * kUnit, high[1], low[1]);
+            split(v.x * kUnit, v.y * kUnit, high[2], low[2]);
+            split(v.z * kUnit, v.w * kUnit, high[3], low[3]);
+            const uint32_t to = block * kBlockBytes + half_row_at(r, chunk);
+            *reinterpret_cast<uint4*>(record.t_high + to) = make_uint4(high[0], high[1], high[2], high[3]);
+            *reinterpret_cast<uint4*>(record.t_low + to) = make_uint4(low[0], low[1], low[2], low[3]);
+            *reinterpret_cast<uint4*>(record.mix + at * 16) = *reinterpret_cast<const uint4*>(room.mix + at * 16);
+        }
+        __syncthreads();   // the next head writes A and P again
     }
 }
 
@@ -691,18 +689,23 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     split(s[2 * i + (j >> 1)][2 * (j & 1)] * s_down, s[2 * i + (j >> 1)][2 * (j & 1) + 1] * s_down, high[j], low[j]);
+                uint32_t m[4][4];   // products that add to the same sums are kept apart
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    uint32_t m[4];
-                    const uint32_t at = chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1));
-                    load_matrices(m, k_at + at);
-                    multiply(ks[2 * t], high, m[0], m[1]);
-                    multiply(ks[2 * t + 1], high, m[2], m[3]);
-                    multiply(ks[2 * t], low, m[0], m[1]);
-                    multiply(ks[2 * t + 1], low, m[2], m[3]);
-                    load_matrices(m, q_at + at);
-                    multiply(qs[2 * t], high, m[0], m[1]);
-                    multiply(qs[2 * t + 1], high, m[2], m[3]);
+                    load_matrices(m[t], k_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1)));
+                    multiply(ks[2 * t], high, m[t][0], m[t][1]);
+                    multiply(ks[2 * t + 1], high, m[t][2], m[t][3]);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    multiply(ks[2 * t], low, m[t][0], m[t][1]);
+                    multiply(ks[2 * t + 1], low, m[t][2], m[t][3]);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    load_matrices(m[t], q_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1)));
+                    multiply(qs[2 * t], high, m[t][0], m[t][1]);
+                    multiply(qs[2 * t + 1], high, m[t][2], m[t][3]);
                 }
             }
             // ---- the other half of the keys: all of K S, and Q S of the 32 tokens whose output this warp writes
@@ -772,18 +775,23 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
             for (int t = 0; t < 8; ++t) v[t][0] = v[t][1] = v[t][2] = v[t][3] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                uint32_t m[4][4];
 #pragma unroll
                 for (int t = i; t < 4; ++t) {
-                    uint32_t m[4];
-                    const uint32_t at = block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
-                    load_matrices(m, smem_at(buf.record.t_high) + at);
-                    multiply(v[2 * t], high[i], m[0], m[1]);
-                    multiply(v[2 * t + 1], high[i], m[2], m[3]);
-                    multiply(v[2 * t], low[i], m[0], m[1]);
-                    multiply(v[2 * t + 1], low[i], m[2], m[3]);
-                    load_matrices(m, smem_at(buf.record.t_low) + at);
-                    multiply(v[2 * t], high[i], m[0], m[1]);
-                    multiply(v[2 * t + 1], high[i], m[2], m[3]);
+                    load_matrices(m[t], smem_at(buf.record.t_high) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
+                    multiply(v[2 * t], high[i], m[t][0], m[t][1]);
+                    multiply(v[2 * t + 1], high[i], m[t][2], m[t][3]);
+                }
+#pragma unroll
+                for (int t = i; t < 4; ++t) {
+                    multiply(v[2 * t], low[i], m[t][0], m[t][1]);
+                    multiply(v[2 * t + 1], low[i], m[t][2], m[t][3]);
+                }
+#pragma unroll
+                for (int t = i; t < 4; ++t) {
+                    load_matrices(m[t], smem_at(buf.record.t_low) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
+                    multiply(v[2 * t], high[i], m[t][0], m[t][1]);
+                    multiply(v[2 * t + 1], high[i], m[t][2], m[t][3]);
                 }
             }
         }
@@ -826,14 +834,17 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     split(w[2 * t + (j >> 1)][2 * (j & 1)] * w_down, w[2 * t + (j >> 1)][2 * (j & 1) + 1] * w_down, high[j], low[j]);
+                uint32_t m[kKeys / 16][4];
 #pragma unroll
                 for (int i = 0; i < kKeys / 16; ++i) {
-                    uint32_t m[4];
-                    load_matrices_t(m, k_at + chunk_at<kChunks>(t * 16 + (lane & 15), key0 / 8 + 2 * i + (lane >> 4)));
-                    multiply(s[2 * i], high, m[0], m[1]);
-                    multiply(s[2 * i + 1], high, m[2], m[3]);
-                    multiply(s[2 * i], low, m[0], m[1]);
-                    multiply(s[2 * i + 1], low, m[2], m[3]);
+                    load_matrices_t(m[i], k_at + chunk_at<kChunks>(t * 16 + (lane & 15), key0 / 8 + 2 * i + (lane >> 4)));
+                    multiply(s[2 * i], high, m[i][0], m[i][1]);
+                    multiply(s[2 * i + 1], high, m[i][2], m[i][3]);
+                }
+#pragma unroll
+                for (int i = 0; i < kKeys / 16; ++i) {
+                    multiply(s[2 * i], low, m[i][0], m[i][1]);
+                    multiply(s[2 * i + 1], low, m[i][2], m[i][3]);
                 }
             }
 #pragma unroll
@@ -918,7 +929,7 @@ cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(prepare_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepare);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_kernel<T, kDim, kGroupsOf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    prepare_kernel<T, kDim><<<(unsigned) (record_slots(p.a.n_tokens, p.a.n_seqs) * p.a.n_v_heads), kProducerThreads, kPrepare, stream>>>(p);
+    prepare_kernel<T, kDim><<<(unsigned) (record_slots(p.a.n_tokens, p.a.n_seqs) * p.a.n_k_heads), kProducerThreads, kPrepare, stream>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const unsigned grid = (unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * (kDim / (kGroupsOf * 16)));
