@@ -575,83 +575,80 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
 
 template <int kDim, int kGroupsOf>
 struct ChunkRoom {
+    static constexpr int kThreadsOf = kProducerThreads + kGroupsOf * 96;   // loaders; state warps in pairs; output warps
     struct Buffer {
         alignas(128) uint8_t k[kChunk * kDim * 2], q[kChunk * kDim * 2], v[kChunk * kGroupsOf * 32];
         Record record;
     };
     Buffer buffer[2];
-    float4 meet[kGroupsOf * 2][12][32];   // what a consumer warp hands its partner: K S (8), Q S of the partner's tokens (4)
-    int power[kGroupsOf * 2];
+    float4 sums[kGroupsOf * 2][8][32];            // K S over its half of the keys, which a state warp hands its partner
+    uint4 states[kGroupsOf][kDim / 16][32];       // S as the output takes it: fp16 left operands, 16 keys each
+    uint4 values[2][kGroupsOf][4][32];            // V' as the output takes it, 16 tokens each
+    int state_power[kGroupsOf][2], value_power[2][kGroupsOf];
 };
+// Barriers.  A buffer is full (loaders arrive, the others wait) and empty again (the other way round); the two of a pair
+// hand over their sums; a pair's S is ready for its output warp (which waits), and its V' is (all three meet: so a
+// pair is never more than one chunk ahead of its output, whose reads of S are over by then).
+enum : int { kFull = 0, kEmpty = 2, kPair = 4, kStateReady = 8, kValueReady = 12 };
 
 template <typename T, int kDim, int kGroupsOf>
 __device__ __forceinline__ void load_chunks(const DeltaDev& p, ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int seq, int head, int slice) {
-    constexpr int kAll = kProducerThreads + kGroupsOf * 64, kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
+    constexpr int kAll = ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
     constexpr int kValueChunks = kGroupsOf * 2;
-    constexpr bool kAsIs = std::is_same<T, __half>::value;
     const skv_gdn_args& a = p.a;
     const int tid = threadIdx.x;
     const T* qh = static_cast<const T*>(a.q) + (head / p.ratio) * kDim;
     const T* kh = static_cast<const T*>(a.k) + (head / p.ratio) * kDim;
     const T* vh = static_cast<const T*>(a.v) + head * kDim + slice * kGroupsOf * 16;
-    const int64_t slot = first_slot(begin, seq);
+    const Record* record = p.records + first_slot(begin, seq) * a.n_v_heads + head;
     int b = 0;
-    for (int t0 = begin, n = 0; t0 < end; t0 += kChunk, ++n, b ^= 1) {
+    for (int t0 = begin, n = 0; t0 < end; t0 += kChunk, ++n, b ^= 1, record += a.n_v_heads) {
         auto& buf = room.buffer[b];
-        const Record& record = p.records[(slot + n) * a.n_v_heads + head];
-        uint4 k[kAsIs ? 1 : kMine], q[kAsIs ? 1 : kMine];
-        float down[kAsIs ? 1 : kMine], key_down = 1.0f;
-        if constexpr (!kAsIs) {    // on their way while the buffer is still in use
-            key_down = __ldg(&record.f.key_down);
+        if (n >= 2) meet<kAll>(kEmpty + b);
 #pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-                const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
-                const bool on = t0 + r < end;
-                const int64_t t = on ? t0 + r : begin;
-                k[i] = on ? __ldg(reinterpret_cast<const uint4*>(kh + t * a.k_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
-                q[i] = on ? __ldg(reinterpret_cast<const uint4*>(qh + t * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
-                down[i] = __ldg(&record.f.down[r]);
-            }
+        for (int i = 0; i < kMine; ++i) {
+            const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+            const uint32_t to = chunk_at<kChunks>(r, chunk);
+            const bool on = t0 + r < end;
+            const int64_t t = on ? t0 + r : begin;
+            copy_async16(smem_at(buf.k) + to, kh + t * a.k_stride + chunk * 8, on);
+            copy_async16(smem_at(buf.q) + to, qh + t * a.q_stride + chunk * 8, on);
         }
-        if (n >= 2) meet<kAll>(3 + b);   // the consumers are done with this buffer
         for (int at = tid; at < kChunk * kValueChunks; at += kProducerThreads) {
             const int r = at / kValueChunks, chunk = at % kValueChunks;
             const bool on = t0 + r < end;
             copy_async16(smem_at(buf.v) + chunk_at<kValueChunks>(r, chunk), vh + (int64_t) (on ? t0 + r : begin) * a.v_stride + chunk * 8, on);
         }
         for (int at = tid; at < (int) (sizeof(Record) / 16); at += kProducerThreads)
-            copy_async16(smem_at(&buf.record) + at * 16, reinterpret_cast<const uint8_t*>(&record) + at * 16, true);
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
-            const uint32_t to = chunk_at<kChunks>(r, chunk);
-            if constexpr (kAsIs) {
-                const bool on = t0 + r < end;
-                const int64_t t = on ? t0 + r : begin;
-                copy_async16(smem_at(buf.k) + to, kh + t * a.k_stride + chunk * 8, on);
-                copy_async16(smem_at(buf.q) + to, qh + t * a.q_stride + chunk * 8, on);
-            } else {
+            copy_async16(smem_at(&buf.record) + at * 16, reinterpret_cast<const uint8_t*>(record) + at * 16, true);
+        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+        if constexpr (!std::is_same<T, __half>::value) {
+            // bfloat16 becomes fp16 where it lies, each thread what it copied
+            const float key_down = __ldg(&record->f.key_down);
+#pragma unroll 2
+            for (int i = 0; i < kMine; ++i) {
+                const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+                const uint32_t to = chunk_at<kChunks>(r, chunk);
+                const float down = __ldg(&record->f.down[r]);
                 float x[8];
-                unpack8<T>(k[i], x);
+                unpack8<T>(*reinterpret_cast<const uint4*>(buf.k + to), x);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] *= key_down;
                 *reinterpret_cast<uint4*>(buf.k + to) = pack8<__half>(x);
-                unpack8<T>(q[i], x);
+                unpack8<T>(*reinterpret_cast<const uint4*>(buf.q + to), x);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= down[i];
+                for (int j = 0; j < 8; ++j) x[j] *= down;
                 *reinterpret_cast<uint4*>(buf.q + to) = pack8<__half>(x);
             }
         }
-        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-        pass<kAll>(1 + b);   // the buffer is full
+        pass<kAll>(kFull + b);
     }
 }
 
 template <typename T, int kDim, int kGroupsOf>
-__device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int head, int slice, float* state) {
-    constexpr int kAll = kProducerThreads + kGroupsOf * 64, kChunks = kDim / 8, kValueChunks = kGroupsOf * 2;
+__device__ __forceinline__ void advance(ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int head, int slice, float* state) {
+    constexpr int kAll = ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kChunks = kDim / 8, kValueChunks = kGroupsOf * 2;
     constexpr int kKeys = kDim / 2;                      // per warp of a pair
-    const skv_gdn_args& a = p.a;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kProducers, g = lane >> 2, c = lane & 3;
     const int half = warp & 1, group = warp >> 1, key0 = half * kKeys;
     const int col0 = (slice * kGroupsOf + group) * 16;   // the pair's value columns
@@ -661,7 +658,6 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
     for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = state[(key0 + i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8];
-    T* out = static_cast<T*>(a.out) + head * kDim + col0 + 2 * c;
     int b = 0;
     for (int t0 = begin; t0 < end; t0 += kChunk, b ^= 1) {
         const auto& buf = room.buffer[b];
@@ -672,72 +668,48 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
             for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(s[i][j]));
         const int s_power = power_for(warp_largest(top));
         const float s_down = power_of_two(-s_power), s_up = power_of_two(s_power);
-        meet<kAll>(1 + b);       // the buffer is full; and both warps of a pair have read what they handed over
+        meet<kAll>(kFull + b);   // and both warps of a pair have read what they handed over
         const uint32_t k_at = smem_at(buf.k);
-        // ---- S^T K^T and S^T Q^T over the warp's keys
-        float ks[8][4], o[4][4];
-        {
-            float qs[8][4];
+        // ---- S^T K^T over the warp's keys
+        float ks[8][4];
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
+        for (int t = 0; t < 8; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) ks[t][j] = qs[t][j] = 0.0f;
-            const uint32_t q_at = smem_at(buf.q);
+            for (int j = 0; j < 4; ++j) ks[t][j] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kKeys / 16; ++i) {
-                uint32_t high[4], low[4];
+        for (int i = 0; i < kKeys / 16; ++i) {
+            uint32_t high[4], low[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    split(s[2 * i + (j >> 1)][2 * (j & 1)] * s_down, s[2 * i + (j >> 1)][2 * (j & 1) + 1] * s_down, high[j], low[j]);
-                uint32_t m[4][4];   // products that add to the same sums are kept apart
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    load_matrices(m[t], k_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1)));
-                    multiply(ks[2 * t], high, m[t][0], m[t][1]);
-                    multiply(ks[2 * t + 1], high, m[t][2], m[t][3]);
-                }
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    multiply(ks[2 * t], low, m[t][0], m[t][1]);
-                    multiply(ks[2 * t + 1], low, m[t][2], m[t][3]);
-                }
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    load_matrices(m[t], q_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1)));
-                    multiply(qs[2 * t], high, m[t][0], m[t][1]);
-                    multiply(qs[2 * t + 1], high, m[t][2], m[t][3]);
-                }
-            }
-            // ---- the other half of the keys: all of K S, and Q S of the 32 tokens whose output this warp writes
-#pragma unroll
-            for (int t = 0; t < 8; ++t)
-                room.meet[warp][t][lane] = make_float4(ks[t][0] * s_up, ks[t][1] * s_up, ks[t][2] * s_up, ks[t][3] * s_up);
+            for (int j = 0; j < 4; ++j)
+                split(s[2 * i + (j >> 1)][2 * (j & 1)] * s_down, s[2 * i + (j >> 1)][2 * (j & 1) + 1] * s_down, high[j], low[j]);
+            room.states[group][half * (kKeys / 16) + i][lane] = make_uint4(high[0], high[1], high[2], high[3]);
+            uint32_t m[4][4];   // products that add to the same sums are kept apart
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                room.meet[warp][8 + t][lane] =
-                    make_float4((half ? qs[t][0] : qs[4 + t][0]) * s_up, (half ? qs[t][1] : qs[4 + t][1]) * s_up,
-                                (half ? qs[t][2] : qs[4 + t][2]) * s_up, (half ? qs[t][3] : qs[4 + t][3]) * s_up);
-            }
-            if (lane == 0) room.power[warp] = s_power;
-            meet<64>(6 + group);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const float4 x = room.meet[warp ^ 1][t][lane];
-                ks[t][0] = fmaf(ks[t][0], s_up, x.x);
-                ks[t][1] = fmaf(ks[t][1], s_up, x.y);
-                ks[t][2] = fmaf(ks[t][2], s_up, x.z);
-                ks[t][3] = fmaf(ks[t][3], s_up, x.w);
+                load_matrices(m[t], k_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1)));
+                multiply(ks[2 * t], high, m[t][0], m[t][1]);
+                multiply(ks[2 * t + 1], high, m[t][2], m[t][3]);
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const float4 x = room.meet[warp ^ 1][8 + t][lane];
-                o[t][0] = fmaf(half ? qs[4 + t][0] : qs[t][0], s_up, x.x);
-                o[t][1] = fmaf(half ? qs[4 + t][1] : qs[t][1], s_up, x.y);
-                o[t][2] = fmaf(half ? qs[4 + t][2] : qs[t][2], s_up, x.z);
-                o[t][3] = fmaf(half ? qs[4 + t][3] : qs[t][3], s_up, x.w);
+                multiply(ks[2 * t], low, m[t][0], m[t][1]);
+                multiply(ks[2 * t + 1], low, m[t][2], m[t][3]);
             }
         }
-        const int o_least = max(max(s_power, room.power[warp ^ 1]) - 60, -120);
+        if (lane == 0) room.state_power[group][half] = s_power;
+        pass<96>(kStateReady + group);
+        // ---- the other half of the keys
+#pragma unroll
+        for (int t = 0; t < 8; ++t) room.sums[warp][t][lane] = make_float4(ks[t][0] * s_up, ks[t][1] * s_up, ks[t][2] * s_up, ks[t][3] * s_up);
+        meet<64>(kPair + group);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const float4 x = room.sums[warp ^ 1][t][lane];
+            ks[t][0] = fmaf(ks[t][0], s_up, x.x);
+            ks[t][1] = fmaf(ks[t][1], s_up, x.y);
+            ks[t][2] = fmaf(ks[t][2], s_up, x.z);
+            ks[t][3] = fmaf(ks[t][3], s_up, x.w);
+        }
         // ---- R = beta (V - e^G K S), in place of K S
         top = 0.0f;
 #pragma unroll
@@ -796,33 +768,41 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
             }
         }
         const int v_unit = r_power - 10;   // V' = 2^v_unit v
+        // ---- V' for the output, from one warp of the pair
+        if (half == 0) {
+            top = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[t][j]));
+            const int least = max(max(s_power, room.state_power[group][1]) - 60, -120);
+            const int o_power = min(max(exponent_of(warp_largest(top)) - 14 + v_unit, least), 120);
+            const float v_down = power_of_two(v_unit - o_power);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                room.values[b][group][t][lane] =
+                    make_uint4(Pair<__half>::down(v[2 * t][0] * v_down, v[2 * t][1] * v_down), Pair<__half>::down(v[2 * t][2] * v_down, v[2 * t][3] * v_down),
+                               Pair<__half>::down(v[2 * t + 1][0] * v_down, v[2 * t + 1][1] * v_down),
+                               Pair<__half>::down(v[2 * t + 1][2] * v_down, v[2 * t + 1][3] * v_down));
+            if (lane == 0) room.value_power[b][group] = o_power;
+        }
+        meet<96>(kValueReady + group);
         // ---- S <- e^(G_63) S + K^T (e^(G_63 - G) V')
-        uint32_t first[4][4];              // V' as it enters the output
-        int o_power;
         {
             top = 0.0f;
-            float most = 0.0f;
-            float w[8][4];
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.update[t * 8 + 2 * c]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    w[t][j] = v[t][j] * (j & 1 ? f.y : f.x);
-                    top = fmaxf(top, fabsf(w[t][j]));
-                    most = fmaxf(most, fabsf(v[t][j]));
+                    v[t][j] *= j & 1 ? f.y : f.x;
+                    top = fmaxf(top, fabsf(v[t][j]));
                 }
             }
             // one power for S and the update: the update's, or 2^-60 of what S would need where the update is smaller yet
             int w_power = exponent_of(warp_largest(top)) - 14 + v_unit;
             w_power = min(max(w_power, max(s_power - 60, -120)), 120);
-            o_power = min(max(exponent_of(warp_largest(most)) - 14 + v_unit, o_least), 120);
-            const float w_down = power_of_two(v_unit - w_power), v_down = power_of_two(v_unit - o_power);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    first[t][j] = Pair<__half>::down(v[2 * t + (j >> 1)][2 * (j & 1)] * v_down, v[2 * t + (j >> 1)][2 * (j & 1) + 1] * v_down);
+            const float w_down = power_of_two(v_unit - w_power);
             const float keep = buf.record.f.whole * power_of_two(-w_power), up = power_of_two(w_power);
 #pragma unroll
             for (int i = 0; i < kKeys / 8; ++i)
@@ -833,7 +813,7 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
                 uint32_t high[4], low[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    split(w[2 * t + (j >> 1)][2 * (j & 1)] * w_down, w[2 * t + (j >> 1)][2 * (j & 1) + 1] * w_down, high[j], low[j]);
+                    split(v[2 * t + (j >> 1)][2 * (j & 1)] * w_down, v[2 * t + (j >> 1)][2 * (j & 1) + 1] * w_down, high[j], low[j]);
                 uint32_t m[kKeys / 16][4];
 #pragma unroll
                 for (int i = 0; i < kKeys / 16; ++i) {
@@ -852,44 +832,7 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[i][j] *= up;
         }
-        // ---- O = scale (e^G Q S + P V') of the warp's 32 tokens
-        const float o_down = power_of_two(-o_power), o_up = power_of_two(o_power);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.query[half * 32 + t * 8 + 2 * c]);
-            o[t][0] *= f.x * o_down;
-            o[t][1] *= f.y * o_down;
-            o[t][2] *= f.x * o_down;
-            o[t][3] *= f.y * o_down;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int t = half * 2 + u;
-                if (i <= t) {
-                    uint32_t m[4];
-                    load_matrices(m, smem_at(buf.record.mix) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
-                    multiply(o[2 * u], first[i], m[0], m[1]);
-                    multiply(o[2 * u + 1], first[i], m[2], m[3]);
-                }
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int in = half * 32 + t * 8;
-            float2 f = *reinterpret_cast<const float2*>(&buf.record.f.out[in + 2 * c]);
-            f.x *= o_up;
-            f.y *= o_up;
-            const uint32_t lo = transpose8(Pair<T>::down(o[t][0] * f.x, o[t][1] * f.y));
-            const uint32_t hi = transpose8(Pair<T>::down(o[t][2] * f.x, o[t][3] * f.y));
-            const int token = t0 + in + g;
-            if (token < end) {
-                *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride) = lo;
-                *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride + 8) = hi;
-            }
-        }
-        if (t0 + 2 * kChunk < end) pass<kAll>(3 + b);   // the buffer may be filled again
+        if (t0 + 2 * kChunk < end) pass<kAll>(kEmpty + b);
     }
 #pragma unroll
     for (int i = 0; i < kKeys / 8; ++i)
@@ -897,11 +840,98 @@ __device__ __forceinline__ void consume(const DeltaDev& p, ChunkRoom<kDim, kGrou
         for (int j = 0; j < 4; ++j) state[(key0 + i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8] = s[i][j];
 }
 
+/// O = scale (e^G Q S + P V') of one pair's columns.
 template <typename T, int kDim, int kGroupsOf>
-__global__ void __launch_bounds__(kProducerThreads + kGroupsOf * 64, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
+__device__ __forceinline__ void put_out(const DeltaDev& p, ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int head, int slice) {
+    constexpr int kAll = ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kChunks = kDim / 8;
+    const skv_gdn_args& a = p.a;
+    const int lane = threadIdx.x & 31, group = (threadIdx.x >> 5) - kProducers - 2 * kGroupsOf, g = lane >> 2, c = lane & 3;
+    T* const out = static_cast<T*>(a.out) + head * kDim + (slice * kGroupsOf + group) * 16 + 2 * c;
+    int b = 0;
+    for (int t0 = begin; t0 < end; t0 += kChunk, b ^= 1) {
+        const auto& buf = room.buffer[b];
+        float o[8][4];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+        meet<kAll>(kFull + b);
+        meet<96>(kStateReady + group);
+        // the half of the keys with the smaller power first: its sums are scaled down to the other's
+        const int power0 = room.state_power[group][0], power1 = room.state_power[group][1], first = power1 < power0;
+        const uint32_t q_at = smem_at(buf.q);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h == 1) {
+                const float down = power_of_two(-abs(power1 - power0));
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[t][j] *= down;
+            }
+#pragma unroll
+            for (int u = 0; u < kDim / 32; ++u) {
+                const int i = (first ^ h) * (kDim / 32) + u;
+                const uint4 x = room.states[group][i][lane];
+                const uint32_t high[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    uint32_t m[4];
+                    load_matrices(m, q_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+                    multiply(o[2 * t], high, m[0], m[1]);
+                    multiply(o[2 * t + 1], high, m[2], m[3]);
+                }
+            }
+        }
+        const int s_power = max(power0, power1);
+        meet<96>(kValueReady + group);
+        const int o_power = room.value_power[b][group];
+        const float fit = power_of_two(s_power - o_power), up = power_of_two(o_power);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.query[t * 8 + 2 * c]);
+            o[t][0] *= f.x * fit;
+            o[t][1] *= f.y * fit;
+            o[t][2] *= f.x * fit;
+            o[t][3] *= f.y * fit;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 x = room.values[b][group][i][lane];
+            const uint32_t high[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int t = i; t < 4; ++t) {
+                uint32_t m[4];
+                load_matrices(m, smem_at(buf.record.mix) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
+                multiply(o[2 * t], high, m[0], m[1]);
+                multiply(o[2 * t + 1], high, m[2], m[3]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            float2 f = *reinterpret_cast<const float2*>(&buf.record.f.out[t * 8 + 2 * c]);
+            f.x *= up;
+            f.y *= up;
+            const uint32_t lo = transpose8(Pair<T>::down(o[t][0] * f.x, o[t][1] * f.y));
+            const uint32_t hi = transpose8(Pair<T>::down(o[t][2] * f.x, o[t][3] * f.y));
+            const int token = t0 + t * 8 + g;
+            if (token < end) {
+                *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride) = lo;
+                *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride + 8) = hi;
+            }
+        }
+        if (t0 + 2 * kChunk < end) pass<kAll>(kEmpty + b);
+    }
+}
+
+/// Registers per thread of the roles where the CTA has 512 threads: they add up to what it was launched with.
+constexpr int kLoaderRegisters = 64, kStateRegisters = 176, kOutputRegisters = 96;
+static_assert(kLoaderRegisters * 128 + kStateRegisters * 256 + kOutputRegisters * 128 == 128 * 512, "the shares of 512 threads launched with 128 each");
+
+template <typename T, int kDim, int kGroupsOf>
+__global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf>::kThreadsOf, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
     extern __shared__ __align__(128) uint8_t smem[];
     auto& room = *reinterpret_cast<ChunkRoom<kDim, kGroupsOf>*>(smem);
     constexpr int kSlices = kDim / (kGroupsOf * 16);
+    constexpr bool kShares = kGroupsOf == 4;
     const skv_gdn_args& a = p.a;
     const int slice = blockIdx.x % kSlices;
     const int64_t item = blockIdx.x / kSlices;
@@ -910,8 +940,17 @@ __global__ void __launch_bounds__(kProducerThreads + kGroupsOf * 64, 1) chunk_ke
     if (!tokens_of(a, seq, begin, end)) return;
     float* const state = state_of(p, seq, head, kDim);
     if (!state) return;
-    if (threadIdx.x < kProducerThreads) load_chunks<T, kDim, kGroupsOf>(p, room, begin, end, seq, head, slice);
-    else consume<T, kDim, kGroupsOf>(p, room, begin, end, head, slice, state);
+    const int warp = threadIdx.x >> 5;
+    if (warp < kProducers) {
+        if constexpr (kShares) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegisters));
+        load_chunks<T, kDim, kGroupsOf>(p, room, begin, end, seq, head, slice);
+    } else if (warp < kProducers + 2 * kGroupsOf) {
+        if constexpr (kShares) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kStateRegisters));
+        advance<T, kDim, kGroupsOf>(room, begin, end, head, slice, state);
+    } else {
+        if constexpr (kShares) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOutputRegisters));
+        put_out<T, kDim, kGroupsOf>(p, room, begin, end, head, slice);
+    }
 }
 
 template <typename T>
@@ -926,6 +965,14 @@ template <typename T, int kDim, int kGroupsOf>
 cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
     constexpr int kSmem = sizeof(ChunkRoom<kDim, kGroupsOf>), kPrepare = sizeof(PrepareRoom<kDim>);
     static_assert(kSmem <= 227 * 1024, "the buffers fit an SM");
+    if constexpr (kGroupsOf == 4) {
+        // the roles' shares add up only if the CTA was launched with the registers they were made for
+        static const int registers = [] {
+            cudaFuncAttributes f{};
+            return cudaFuncGetAttributes(&f, chunk_kernel<T, kDim, kGroupsOf>) == cudaSuccess ? f.numRegs : 0;
+        }();
+        if (registers != 128) return cudaErrorInvalidConfiguration;
+    }
     cudaError_t e = cudaFuncSetAttribute(prepare_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepare);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_kernel<T, kDim, kGroupsOf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
@@ -933,7 +980,7 @@ cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const unsigned grid = (unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * (kDim / (kGroupsOf * 16)));
-    chunk_kernel<T, kDim, kGroupsOf><<<grid, kProducerThreads + kGroupsOf * 64, kSmem, stream>>>(p);
+    chunk_kernel<T, kDim, kGroupsOf><<<grid, ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kSmem, stream>>>(p);
     return cudaGetLastError();
 }
 
