@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -601,6 +602,12 @@ def unpack_segments(image, dst: PooledSequence) -> list:
 _CODES = {"torch.float16": DTYPE_F16, "torch.bfloat16": DTYPE_BF16}
 _KNOWN = {}     # dtype object -> (its name, its code or None), so that a call formats no text
 
+# The argument structures as the library reads them, packed: a third of the time of filling a ctypes structure.
+_APPEND = struct.Struct("@PPqqPPqqPPPPiiiiiifi")
+_ATTENTION = struct.Struct("@PPqqPPPQiiif")
+_DELTA = struct.Struct("@PPPPqqqqPPqqPqqPPPQiiiiiiif")
+assert (_APPEND.size, _ATTENTION.size, _DELTA.size) == tuple(C.sizeof(x) for x in (AppendArgs, AttentionArgs, GatedDeltaArgs))
+
 
 def _dtype(x) -> tuple:
     got = _KNOWN.get(x.dtype)
@@ -610,24 +617,29 @@ def _dtype(x) -> tuple:
     return got
 
 
-def _rows(x, what: str, like=None) -> tuple:
-    """(address, rows, heads, values, elements between rows) of a [row][head][value] tensor whose heads lie back to back."""
+def _rows(x, what: str, kind=None) -> tuple:
+    """(address, rows, heads, values, elements between rows) of a [row][head][value] tensor of dtype `kind` (None: a
+    float16 or bfloat16 one) whose heads lie back to back."""
     n, heads, dim = x.shape
-    step, between, one = x.stride()
-    if (between != dim and heads > 1) or (one != 1 and dim > 1):
-        raise ValueError(f"{what}: the heads of a row must lie back to back")
-    if _dtype(x)[1] is None or (like is not None and x.dtype != like.dtype):
+    if x.is_contiguous():
+        step = heads * dim
+    else:
+        step, between, one = x.stride()
+        if (between != dim and heads > 1) or (one != 1 and dim > 1):
+            raise ValueError(f"{what}: the heads of a row must lie back to back")
+        if n <= 1:
+            step = heads * dim
+    if (x.dtype is not kind) if kind is not None else _dtype(x)[1] is None:
         raise TypeError(f"{what}: {x.dtype} (all of a call's activations are float16, or all bfloat16)")
     if not x.is_cuda:
         raise ValueError(f"{what}: not on a GPU")
-    return x.data_ptr(), n, heads, dim, step if n > 1 else heads * dim
+    return x.data_ptr(), n, heads, dim, step
 
 
-def _vector(x, what: str, name: str, at_least: int):
-    """The address of a contiguous 1-d device tensor of `name` values; None for None."""
-    if x is None:
-        return None
-    if _dtype(x)[0] != name or x.dim() != 1 or not x.is_cuda or (x.shape[0] > 1 and x.stride(0) != 1):
+def _vector(x, what: str, name: str, at_least: int) -> int:
+    """The address of a contiguous 1-d device tensor of at least so many `name` values."""
+    got = _KNOWN.get(x.dtype) or _dtype(x)
+    if got[0] != name or x.dim() != 1 or not x.is_cuda or not x.is_contiguous():
         raise TypeError(f"{what}: a contiguous 1-d {name} tensor on the GPU")
     if x.shape[0] < at_least:
         raise ValueError(f"{what}: {x.shape[0]} entries, {at_least} needed")
@@ -685,25 +697,28 @@ def kv_append(layer: KvLayer, k, v, lengths, *, seq_starts=None, q=None, q_out=N
     """Write the K and V rows of new tokens ([token][kv_head][head_dim]) into cells lengths[s], lengths[s]+1, ... of
     their sequences, K rotated by its cell's number, and q rotated into q_out (skv_kv_append)."""
     kp, n, kv, dim, ks = _rows(k, "k")
-    vp, vn, vkv, vdim, vs = _rows(v, "v", k)
-    if (vn, vkv, vdim) != (n, kv, dim) or kv != layer.n_head_kv or dim != layer.head_dim:
+    kind = k.dtype
+    vp, vn, vkv, vdim, vs = _rows(v, "v", kind)
+    if vn != n or vkv != kv or vdim != dim or kv != layer.n_head_kv or dim != layer.head_dim:
         raise ValueError("kv_append: k and v are [token][kv_head][head_dim] of the layer")
     n_seqs = n if seq_starts is None else seq_starts.shape[0] - 1
-    qp = qo = None
-    qs = qos = heads = 0
+    qp = qo = qs = qos = heads = rot = 0
     if (q is None) != (q_out is None):
         raise ValueError("kv_append: q and q_out come together")
     if q is not None:
-        qp, qn, heads, qd, qs = _rows(q, "q", k)
-        qo, on, oh, od, qos = _rows(q_out, "q_out", k)
-        if (qn, qd) != (n, dim) or (on, oh, od) != (qn, heads, qd):
+        qp, qn, heads, qd, qs = _rows(q, "q", kind)
+        qo, on, oh, od, qos = _rows(q_out, "q_out", kind)
+        if qn != n or qd != dim or on != n or oh != heads or od != dim:
             raise ValueError("kv_append: q and q_out are [token][head][head_dim]")
-    args = AppendArgs(kp, vp, ks, vs, qp, qo, qs, qos, _vector(seq_starts, "seq_starts", "torch.int32", 1),
-                      _vector(lengths, "lengths", "torch.int32", n_seqs),
-                      _vector(lengths_out, "lengths_out", "torch.int32", n_seqs), _vector(inv_freq, "inv_freq", "torch.float32", 0),
-                      n, n_seqs, heads, 0 if inv_freq is None else 2 * inv_freq.shape[0], ROPE_STYLES[rope_style], _dtype(k)[1],
-                      rope_scale, 0)
-    check(lib().skv_kv_append(layer.at, C.addressof(args), _stream(stream)))
+    if inv_freq is not None:
+        rot = 2 * inv_freq.shape[0]
+    args = _APPEND.pack(kp, vp, ks, vs, qp, qo, qs, qos,
+                        0 if seq_starts is None else _vector(seq_starts, "seq_starts", "torch.int32", 1),
+                        _vector(lengths, "lengths", "torch.int32", n_seqs),
+                        0 if lengths_out is None else _vector(lengths_out, "lengths_out", "torch.int32", n_seqs),
+                        0 if inv_freq is None else _vector(inv_freq, "inv_freq", "torch.float32", 0),
+                        n, n_seqs, heads, rot, ROPE_STYLES[rope_style], _dtype(k)[1], rope_scale, 0)
+    check(lib().skv_kv_append(layer.at, args, _stream(stream)))
 
 
 def decode_attention_workspace(layer: KvLayer, n_seqs: int, n_head: int) -> int:
@@ -717,14 +732,17 @@ def decode_attention(layer: KvLayer, q, lengths, out, *, workspace, scale: float
     """out = softmax(scale * q K^T) V of one new token per sequence ([sequence][head][head_dim]) over the first
     lengths[s] cells of its cache (skv_decode_attention).  scale: head_dim ** -0.5 when None."""
     qp, n, heads, dim, qs = _rows(q, "q")
-    op, on, oh, od, os_ = _rows(out, "out", q)
-    if (on, oh, od) != (n, heads, dim) or dim != layer.head_dim:
+    op, on, oh, od, os_ = _rows(out, "out", q.dtype)
+    if on != n or oh != heads or od != dim or dim != layer.head_dim:
         raise ValueError("decode_attention: q and out are [sequence][head][head_dim] of the layer")
-    if lse is not None and (_dtype(lse)[0] != "torch.float32" or tuple(lse.shape) != (n, heads) or not lse.is_contiguous() or not lse.is_cuda):
-        raise TypeError("decode_attention: lse is a contiguous float32 [sequence][head] tensor on the GPU")
-    args = AttentionArgs(qp, op, qs, os_, _ptr(lse), _vector(lengths, "lengths", "torch.int32", n), _ptr(workspace),
-                         workspace.numel() * workspace.element_size(), n, heads, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
-    check(lib().skv_decode_attention(layer.at, C.addressof(args), _stream(stream)))
+    lp = 0
+    if lse is not None:
+        if _dtype(lse)[0] != "torch.float32" or lse.shape != (n, heads) or not lse.is_contiguous() or not lse.is_cuda:
+            raise TypeError("decode_attention: lse is a contiguous float32 [sequence][head] tensor on the GPU")
+        lp = lse.data_ptr()
+    args = _ATTENTION.pack(qp, op, qs, os_, lp, _vector(lengths, "lengths", "torch.int32", n), workspace.data_ptr(), workspace.nbytes,
+                           n, heads, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
+    check(lib().skv_decode_attention(layer.at, args, _stream(stream)))
 
 
 def gated_delta_workspace(n_tokens: int, n_seqs: int, n_v_heads: int, head_dim: int, max_tokens: int) -> int:
@@ -740,25 +758,38 @@ def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=No
     [token][v_head][dim], g, beta float32 [token][v_head], state float32 [row][v_head][dim key][dim value], updated in
     place.  max_tokens bounds the tokens of one sequence (all of them when None).  scale: dim ** -0.5 when None."""
     qp, n, kh, dim, qs = _rows(q, "q")
-    kp, kn, kkh, kd, ks = _rows(k, "k", q)
-    vp, vn, vh, vd, vs = _rows(v, "v", q)
-    op, on, oh, od, os_ = _rows(out, "out", q)
-    if (kn, kkh, kd) != (n, kh, dim) or (vn, vd) != (n, dim) or (on, oh, od) != (n, vh, dim):
+    kind = q.dtype
+    kp, kn, kkh, kd, ks = _rows(k, "k", kind)
+    vp, vn, vh, vd, vs = _rows(v, "v", kind)
+    op, on, oh, od, os_ = _rows(out, "out", kind)
+    if kn != n or kkh != kh or kd != dim or vn != n or vd != dim or on != n or oh != vh or od != dim:
         raise ValueError("gated_delta: q and k are [token][k_head][dim], v and out [token][v_head][dim]")
+    steps = []
     for x, what in ((g, "g"), (beta, "beta")):
-        if _dtype(x)[0] != "torch.float32" or tuple(x.shape) != (n, vh) or (vh > 1 and n and x.stride(1) != 1) or not x.is_cuda:
+        if _dtype(x)[0] != "torch.float32" or x.shape != (n, vh) or not x.is_cuda:
             raise TypeError(f"gated_delta: {what} is a float32 [token][v_head] tensor on the GPU")
+        if x.is_contiguous():
+            steps.append(vh)
+        else:
+            step, one = x.stride()
+            if one != 1 and vh > 1:
+                raise ValueError(f"gated_delta: the heads of {what} must lie back to back")
+            steps.append(step if n > 1 else vh)
     rows = state.shape[0]
-    if (_dtype(state)[0] != "torch.float32" or tuple(state.shape[1:]) != (vh, dim, dim) or not state.is_cuda
-            or (rows and not state[0].is_contiguous())):
-        raise TypeError("gated_delta: state is float32 [row][v_head][dim][dim] on the GPU, each row contiguous")
+    if _dtype(state)[0] != "torch.float32" or state.shape[1:] != (vh, dim, dim) or not state.is_cuda:
+        raise TypeError("gated_delta: state is float32 [row][v_head][dim][dim] on the GPU")
+    if state.is_contiguous():
+        row = vh * dim * dim
+    else:
+        if not state[0].is_contiguous():
+            raise ValueError("gated_delta: each row of the state must be contiguous")
+        row = state.stride(0) if rows > 1 else vh * dim * dim
     n_seqs = n if seq_starts is None else seq_starts.shape[0] - 1
     if max_tokens is None:
         max_tokens = 1 if seq_starts is None else n
-    args = GatedDeltaArgs(qp, kp, vp, op, qs, ks, vs, os_, g.data_ptr(), beta.data_ptr(), g.stride(0) if n > 1 else vh,
-                          beta.stride(0) if n > 1 else vh, state.data_ptr(), state.stride(0) if rows > 1 else vh * dim * dim, rows,
-                          _vector(state_index, "state_index", "torch.int32", n_seqs),
-                          _vector(seq_starts, "seq_starts", "torch.int32", 1), _ptr(workspace),
-                          0 if workspace is None else workspace.numel() * workspace.element_size(), n, n_seqs, kh, vh, dim,
-                          max_tokens, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
-    check(lib().skv_gated_delta(C.addressof(args), _stream(stream)))
+    args = _DELTA.pack(qp, kp, vp, op, qs, ks, vs, os_, g.data_ptr(), beta.data_ptr(), steps[0], steps[1], state.data_ptr(), row, rows,
+                       0 if state_index is None else _vector(state_index, "state_index", "torch.int32", n_seqs),
+                       0 if seq_starts is None else _vector(seq_starts, "seq_starts", "torch.int32", 1),
+                       0 if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes, n, n_seqs,
+                       kh, vh, dim, max_tokens, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
+    check(lib().skv_gated_delta(args, _stream(stream)))

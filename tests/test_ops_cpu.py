@@ -129,7 +129,7 @@ def test_the_binding_refuses_tensors_that_do_not_fit():
     with pytest.raises(TypeError, match="float16"):
         skv._rows(x.float(), "q")
     with pytest.raises(TypeError, match="all"):
-        skv._rows(x, "q", x.bfloat16())
+        skv._rows(x, "q", torch.bfloat16)
     with pytest.raises(ValueError, match="back to back"):
         skv._rows(x.transpose(1, 2), "q")
     with pytest.raises(TypeError, match="int32"):
