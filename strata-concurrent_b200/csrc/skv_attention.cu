@@ -35,7 +35,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;        // query heads per item: the rows of one matrix product
 constexpr int kMaxSms = 160;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 128;
 
 struct AttnDev {
     LayerDev layer;
@@ -83,14 +83,19 @@ template <int kLeft>
 __device__ __forceinline__ void wait_async() {
     asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
+/// Ordered by the waits and barriers around them (all volatile), not against the thread's own stores: what they read
+/// was copied or written before one of those, so they can run ahead between them.
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 __device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
+/// The CTA's barrier, a warp's meeting.
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 0;" ::: "memory"); }
+__device__ __forceinline__ void meet_warp() { asm volatile("bar.warp.sync 0xffffffff;" ::: "memory"); }
 /// c += a b, 16 x 8 x 16 in fp16 with 32-bit sums.
 __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -120,17 +125,24 @@ __device__ __forceinline__ int64_t cells_of(const AttnDev& p, int seq) {
     return n < 0 ? 0 : n > table ? table : n;
 }
 
-/// Sum over the CTA; every thread calls it.
-__device__ __forceinline__ int64_t cta_sum(int64_t v, int64_t* scratch) {
+/// `before` plus the sum of v over this thread and those before it; `before` grows by the CTA's sum.  Every thread calls it.
+__device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t& before, int64_t* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+    }
+    if (lane == 31) scratch[warp] = v;
     __syncthreads();
-    int64_t sum = 0;
+    v += before;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += scratch[w];
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) v += scratch[w];
+        before += scratch[w];
+    }
     __syncthreads();
-    return sum;
+    return v;
 }
 
 /// A place in the sequence of all tiles.
@@ -165,12 +177,15 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int items = p.layer.n_head_kv * p.blocks, n_seqs = p.a.n_seqs;
     const skv_attention_args& a = p.a;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // ---- the share: tiles [from, to) of all
-    int64_t mine = 0;
-    for (int s = tid; s < n_seqs; s += kThreads) mine += (cells_of(p, s) + G::kTile - 1) / G::kTile;
-    const int64_t total = cta_sum(mine, s_scan) * items;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // of whatever wrote the cache, the lengths and the queries
+    // ---- the share: tiles [from, to) of all.  The tiles of sequences 0 .. s, a thread per sequence, in trips
+    const auto tiles_of = [&](int s) { return s < n_seqs ? (cells_of(p, s) + G::kTile - 1) / G::kTile * items : 0; };
+    int64_t total = 0, end = 0, n = 0;   // of the trip's sequence: the tiles up to its end, and its own
+    for (int base = 0; base < n_seqs; base += kThreads) {
+        n = tiles_of(base + tid);
+        end = cta_scan(n, total, s_scan);
+    }
     const int64_t shares = total < (int64_t) gridDim.x ? total : (int64_t) gridDim.x;
     // sequences without cells
     for (int s = blockIdx.x; s < n_seqs; s += gridDim.x) {
@@ -187,33 +202,22 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         return;
     }
     const int64_t from = total * blockIdx.x / shares, to = total * (blockIdx.x + 1) / shares;
-    {
-        // the sequence that holds tile `from`: a running sum over the sequences, one per thread at a time
+    if (n_seqs <= kThreads) {   // the one trip is still at hand
+        if (n && from >= end - n && from < end) {
+            s_first[0] = tid;
+            s_first[1] = end - n;
+        }
+        meet();
+    } else {
         int64_t before = 0;
-        for (int base = 0; base < n_seqs; base += kThreads) {
-            const int s = base + tid;
-            const int64_t n = s < n_seqs ? (cells_of(p, s) + G::kTile - 1) / G::kTile * items : 0;
-            int64_t up = n;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int64_t o = __shfl_up_sync(0xffffffffu, up, d);
-                if (lane >= d) up += o;
-            }
-            if (lane == 31) s_scan[warp] = up;
-            __syncthreads();
-            int64_t at = before;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) at += s_scan[w];
-                before += s_scan[w];
-            }
-            const int64_t end = at + up;
+        for (int base = 0; base < n_seqs && before <= from; base += kThreads) {
+            n = tiles_of(base + tid);
+            end = cta_scan(n, before, s_scan);
             if (n && from >= end - n && from < end) {
-                s_first[0] = s;
+                s_first[0] = base + tid;
                 s_first[1] = end - n;
             }
-            __syncthreads();
-            if (from < before) break;
+            meet();
         }
     }
     Cursor load;
@@ -340,11 +344,11 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
     int first_tile = here.tile;   // of the item, in this share
 
     int v_slot = 1;
-    for (int64_t n = 0; n < count; ++n, v_slot = 3 - v_slot) {
+    for (n = 0; n < count; ++n, v_slot = 3 - v_slot) {
         const uint8_t* const v_base = smem + v_slot * G::kSlotBytes;
         const uint32_t held_now = held, odd_now = odd;
         wait_async<1>();          // K of this tile
-        __syncwarp();
+        meet_warp();
 
         // ---- scores of the warp's cells: rows g, g + 8; cells 8 t + 2c, 2c + 1
         constexpr int kTiles = G::kCells / 8;
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
                 }
             }
         }
-        __syncwarp();
+        meet_warp();
         issue_k();
         float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -408,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         if constexpr (kInt8) {
             // the largest V scale of the warp's cells per group, as the power of two above it
             wait_async<1>();              // V of this tile
-            __syncwarp();
+            meet_warp();
             const uint8_t* s_at = v_base + G::kPlane + (warp * G::kCells + (lane < G::kCells ? lane : 0)) * G::kScaleBytes;
 #pragma unroll
             for (int i = 0; i < G::kGroups; ++i) {
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
                 if (lane == 0) s_power[warp][i] = min(e, 17);
             }
         }
-        __syncthreads();   // row maxima; and every warp is done with V of the tile before, whose slot is filled again
+        meet();   // row maxima; and every warp is done with V of the tile before, whose slot is filled again
         issue_v(3 - v_slot, n + 1 < count);
 
         float keep[2], now[2], shrink = 1.0f;
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
             }
         }
         wait_async<2>();   // V of this tile
-        __syncthreads();   // weights, and everybody's part of V
+        meet();   // weights, and everybody's part of V
 
         // ---- output: all cells x the warp's columns
 #pragma unroll
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
                 sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
                 if (c == 0) s_sum[warp][g + h * 8] = sum[h];
             }
-            __syncthreads();
+            meet();
             const bool whole = first_tile == 0 && here.tile + 1 == here.tiles;
             const int slot = first_tile == 0 ? 1 : 0;
             const int kv = here.item / p.blocks, first = (here.item % p.blocks) * kRows;
@@ -587,47 +591,63 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
 }
 
 /// Joins the parts of the items that a share began and others went on with: each part counts by 2^(its maximum - the
-/// largest), in the order of the shares.  A task is one head of one cut item; where there are fewer tasks than CTAs (one
-/// long sequence leaves 148 parts or more of each of 24 heads) it is 64 of its columns.
+/// largest), in the order of the shares.  A task is one head of one cut item, or, where there are fewer of them than CTAs
+/// (one long sequence leaves 148 parts of each of 24 heads on 2 CTAs per SM), a piece of its columns.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttnDev p, int shares) {
-    constexpr int kTrips = (kMaxSms * 4 + kJoinThreads - 1) / kJoinThreads, kJoinWarps = kJoinThreads / 32;
-    __shared__ int s_cut[kMaxSms * 4], s_count[kTrips * kJoinWarps];
+__global__ void __launch_bounds__(kJoinThreads, 8) join_kernel(const __grid_constant__ AttnDev p, int shares) {
+    constexpr int kTrips = (kMaxSms * 4 + kJoinThreads - 1) / kJoinThreads, kJoinWarps = kJoinThreads / 32, kBatch = 6;
+    __shared__ int s_count[kTrips * kJoinWarps];
+    __shared__ int4 s_cut[kMaxSms * 4];   // the share that began it, the item, its parts
     __shared__ float s_weight[kMaxSms * 4];
     __shared__ float s_top[kJoinWarps], s_sum[kJoinWarps];
     __shared__ float4 s_out[kJoinThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = min(p.group, kRows), items = p.layer.n_head_kv * p.blocks;
-    if (tid < kTrips * kJoinWarps) s_count[tid] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __syncthreads();
     // the cut items, in order
+    int2 cut[kTrips];
     uint32_t mask[kTrips];
 #pragma unroll
     for (int t = 0; t < kTrips; ++t) {
         const int i = t * kJoinThreads + tid;
-        mask[t] = __ballot_sync(0xffffffffu, i < shares && p.cut[i].x >= 0);
+        cut[t] = i < shares ? __ldcg(p.cut + i) : make_int2(-1, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < kTrips; ++t) {
+        mask[t] = __ballot_sync(0xffffffffu, cut[t].x >= 0);
         if (lane == 0) s_count[t * kJoinWarps + warp] = __popc(mask[t]);
     }
     __syncthreads();
     int cuts = 0;
 #pragma unroll
-    for (int j = 0; j < kTrips * kJoinWarps; ++j) {
-        if (j % kJoinWarps == warp && (mask[j / kJoinWarps] >> lane & 1u))
-            s_cut[cuts + __popc(mask[j / kJoinWarps] & ((1u << lane) - 1u))] = j / kJoinWarps * kJoinThreads + tid;
-        cuts += s_count[j];
-    }
+    for (int t = 0; t < kTrips; ++t)
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            if (w == warp && cut[t].x >= 0)
+                s_cut[cuts + __popc(mask[t] & ((1u << lane) - 1u))] = make_int4(t * kJoinThreads + tid, cut[t].x, cut[t].y, 0);
+            cuts += s_count[t * kJoinWarps + w];
+        }
     __syncthreads();
-    const int pieces = cuts * rows * (kDim / 64) <= (int) gridDim.x ? kDim / 64 : 1;
+    int pieces = 1;
+    while (pieces < kDim / 32 && cuts * rows * pieces * 2 <= (int) gridDim.x) pieces *= 2;
     const int lanes = kDim / 4 / pieces, sets = kJoinThreads / lanes;   // four columns a lane
+    const int at = tid % lanes, set = tid / lanes;
     for (int task = blockIdx.x; task < cuts * rows * pieces; task += gridDim.x) {
-        const int begun = s_cut[task / (rows * pieces)], row = task / pieces % rows, piece = task % pieces;
-        const int2 cut = p.cut[begun];
-        const int seq = cut.x / items, item = cut.x % items, n = cut.y;
+        const int4 of = s_cut[task / (rows * pieces)];
+        const int row = task / pieces % rows, piece = task % pieces, n = of.z;
+        const int seq = of.y / items, item = of.y % items;
         const int kv = item / p.blocks, r = (item % p.blocks) * kRows + row;
         if (r >= p.group) continue;   // the same for the whole CTA
-        const auto place = [&](int i) { return (((int64_t) begun + i) * 2 + (i == 0 ? 1 : 0)) * kRows + row; };
+        const int column = (piece * lanes + at) * 4;
+        // part i of the head: the share's second place for the first, the first place of the shares after it
+        const auto place = [&](int i) { return (((int64_t) of.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + row; };
+        const auto load = [&](int i) {
+            return i < n ? __ldcg(reinterpret_cast<const float4*>(p.part_o + place(i) * kDim + column)) : make_float4(0, 0, 0, 0);
+        };
+        float4 ahead[kBatch];   // on their way while the weights are worked out
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) ahead[j] = load(set + j * sets);
         float top = -INFINITY;
-        for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, p.part_ml[place(i)].x);
+        for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, __ldcg(p.part_ml + place(i)).x);
 #pragma unroll
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         if (lane == 0) s_top[warp] = top;
@@ -636,7 +656,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_top[w]);
         float sum = 0.0f;
         for (int i = tid; i < n; i += kJoinThreads) {
-            const float2 ml = p.part_ml[place(i)];
+            const float2 ml = __ldcg(p.part_ml + place(i));
             const float weight = exp2f(ml.x - (top == -INFINITY ? 0.0f : top));
             s_weight[i] = weight;
             sum = fmaf(weight, ml.y, sum);
@@ -648,13 +668,18 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w) sum += s_sum[w];
-        const int at = tid % lanes, set = tid / lanes, column = (piece * lanes + at) * 4;
         float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-        for (int i = set; i < n; i += sets) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + place(i) * kDim + column));
-            const float w = s_weight[i];
-            o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+        for (int i = set; i < n; i += kBatch * sets) {
+            float4 x[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) x[j] = ahead[j];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) ahead[j] = load(i + (kBatch + j) * sets);
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const float w = i + j * sets < n ? s_weight[i + j * sets] : 0.0f;
+                o.x = fmaf(w, x[j].x, o.x); o.y = fmaf(w, x[j].y, o.y); o.z = fmaf(w, x[j].z, o.z); o.w = fmaf(w, x[j].w, o.w);
+            }
         }
         s_out[tid] = o;
         __syncthreads();
@@ -683,19 +708,23 @@ cudaError_t launch(const AttnDev& p, int sms, cudaStream_t stream) {
     const int ctas = sms * kPerSm;
     cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kDim, kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    attention_kernel<T, kDim, kInt8><<<ctas, kThreads, kSmem, stream>>>(p);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    // the join is resident, or next in line, when the last share ends; it waits for all of them before its first read
+    // Each kernel may be launched while the one before it ends, and waits for it before its first read: 11.5 us a call
+    // instead of 14.4 for 1,000 cells.  (Letting the join in any earlier, while shares still run, costs 2 us.)
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned) sms * 8);
-    config.blockDim = dim3(kJoinThreads);
-    config.stream = stream;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
+    config.stream = stream;
+    config.gridDim = dim3((unsigned) ctas);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kSmem;
+    e = cudaLaunchKernelEx(&config, attention_kernel<T, kDim, kInt8>, p);
+    if (e != cudaSuccess) return e;
+    config.gridDim = dim3((unsigned) sms * 8);
+    config.blockDim = dim3(kJoinThreads);
+    config.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&config, join_kernel<T, kDim>, p, ctas);
 }
 template <typename T>
