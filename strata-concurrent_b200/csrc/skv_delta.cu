@@ -173,9 +173,15 @@ __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
+/// The same without ordering against other memory accesses but the barriers below: for code that meets by those alone and
+/// reads what others wrote before them, so that its loads can run ahead.
+__device__ __forceinline__ void peek_matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void peek_matrices_t(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -213,12 +219,27 @@ template <int kChunks>
 __device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
     return (uint32_t) (row * kChunks + (kChunks >= 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3))) * 16u;
 }
+/// The largest magnitude of an accumulator array, in four chains.
+template <int kTiles>
+__device__ __forceinline__ float largest_of(const float (&x)[kTiles][4]) {
+    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], fabsf(x[i][j]));
+    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
 /// x and y as the sum of two pairs of fp16 values.
 __device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t& low) {
     high = Pair<__half>::down(x, y);
     const float2 h = Pair<__half>::up(high);
     low = Pair<__half>::down(x - h.x, y - h.y);
 }
+
+/// The eight rows of 16 tokens that a lane of the left and one of the right half of ldmatrix name: of a right operand
+/// [token][key], and of its transpose.
+__device__ __forceinline__ int right_row() { return (threadIdx.x & 7) + ((threadIdx.x >> 4) & 1) * 8; }
+__device__ __forceinline__ int right_half() { return (threadIdx.x >> 3) & 1; }
 
 /// Per token of a chunk.
 struct Factors {
@@ -288,6 +309,7 @@ struct PrepareRoom {
     };
     alignas(16) uint8_t mix[kTriangleBytes];
     float2 sums[kChunk];      // G log2 e in two parts
+    float rest[kChunk];       // e^(G_r - G), r the last token of the same 16
     double carry[2];          // the first 32 tokens' sum, and all
     float beta[kChunk];
     int power[kChunk];        // of the query rows
@@ -319,7 +341,8 @@ __device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, int row, 
         }
     }
 }
-/// A (32 bits) and P (fp16) of those blocks.
+/// A (32 bits) and P (fp16) of those blocks.  Below the diagonal block a decay e^(G_i - G_j) is the product of e^(G_i - G_r)
+/// and e^(G_r - G_j), r the last token of j's block: both at most 1, the second one per token.
 template <int kDim, int kBlocks>
 __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int block_row, int from, int at, const float (&kk)[6][4], const float (&qk)[6][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -329,15 +352,30 @@ __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int
         const float2 sum = room.sums[row];
         const float by = fit2 * room.beta[row];
 #pragma unroll
-        for (int t = 0; t < 2 * kBlocks; ++t) {
-            const int col = from * 16 + t * 8 + 2 * c;
-            const float4 other = *reinterpret_cast<const float4*>(&room.sums[col]);   // of col and col + 1
-            // a decay of zero (and what lies above the diagonal) wipes out even an infinite product
-            const float d0 = exp2f((sum.x - other.x) + (sum.y - other.y)), d1 = exp2f((sum.x - other.z) + (sum.y - other.w));
-            *reinterpret_cast<float2*>(&room.work.a[row * kScratch + col]) =
-                make_float2(col < row ? by * d0 * kk[at + t][2 * h] : 0.0f, col + 1 < row ? by * d1 * kk[at + t][2 * h + 1] : 0.0f);
-            *reinterpret_cast<uint32_t*>(room.mix + block_of(block_row, from + t / 2) * kBlockBytes + half_row_at(in, t & 1) + c * 4) =
-                Pair<__half>::down(col <= row ? d0 * qk[at + t][2 * h] : 0.0f, col + 1 <= row ? d1 * qk[at + t][2 * h + 1] : 0.0f);
+        for (int u = 0; u < kBlocks; ++u) {
+            const bool below = from + u < block_row;
+            const float2 ref = room.sums[(from + u) * 16 + 15];
+            const float part = below ? exp2f((sum.x - ref.x) + (sum.y - ref.y)) : 0.0f;
+#pragma unroll
+            for (int t = 2 * u; t < 2 * u + 2; ++t) {
+                const int col = from * 16 + t * 8 + 2 * c;
+                float d0, d1;
+                if (below) {
+                    const float2 rest = *reinterpret_cast<const float2*>(&room.rest[col]);
+                    d0 = part * rest.x;
+                    d1 = part * rest.y;
+                } else {
+                    // above the diagonal a decay of zero wipes out even an infinite product
+                    const float4 other = *reinterpret_cast<const float4*>(&room.sums[col]);   // of col and col + 1
+                    d0 = exp2f((sum.x - other.x) + (sum.y - other.y));
+                    d1 = exp2f((sum.x - other.z) + (sum.y - other.w));
+                }
+                const bool q0 = below || col <= row, q1 = below || col + 1 <= row, k0 = below || col < row, k1 = below || col + 1 < row;
+                *reinterpret_cast<float2*>(&room.work.a[row * kScratch + col]) =
+                    make_float2(k0 ? by * d0 * kk[at + t][2 * h] : 0.0f, k1 ? by * d1 * kk[at + t][2 * h + 1] : 0.0f);
+                *reinterpret_cast<uint32_t*>(room.mix + block_of(block_row, from + u) * kBlockBytes + half_row_at(in, t & 1) + c * 4) =
+                    Pair<__half>::down(q0 ? d0 * qk[at + t][2 * h] : 0.0f, q1 ? d1 * qk[at + t][2 * h + 1] : 0.0f);
+            }
         }
     }
 }
@@ -458,6 +496,7 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
             const double turns = sum * 1.4426950408889634074;   // log2 e
             const float high = (float) turns;
             room.sums[tid] = make_float2(high, (float) (turns - (double) high));
+            room.rest[tid] = exp2f((float) (__shfl_sync(0xffffffffu, turns, lane | 15) - turns));
             room.beta[tid] = beta;
         }
         __syncthreads();
@@ -573,33 +612,38 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
     }
 }
 
-template <int kDim, int kGroupsOf>
+/// A chunk CTA: kGroupsOf groups of 16 value columns, the keys of a group split over kSplit state warps, and the outputs of
+/// kTogether groups in one output warp.
+template <int kDim, int kGroupsOf, int kSplit, int kTogether>
 struct ChunkRoom {
-    static constexpr int kThreadsOf = kProducerThreads + kGroupsOf * 96;   // loaders; state warps in pairs; output warps
+    static constexpr int kStates = kGroupsOf * kSplit, kOutputs = kGroupsOf / kTogether;
+    static constexpr int kThreadsOf = (kProducers + kStates + kOutputs) * 32;   // loaders, state warps, output warps
+    static constexpr int kMeeting = (kSplit * kTogether + 1) * 32;              // the state warps of an output warp, and it
+    static constexpr int kSlices = kDim / (kGroupsOf * 16);
     struct Buffer {
         alignas(128) uint8_t k[kChunk * kDim * 2], q[kChunk * kDim * 2], v[kChunk * kGroupsOf * 32];
         Record record;
     };
     Buffer buffer[2];
-    float4 sums[kGroupsOf * 2][8][32];            // K S over its half of the keys, which a state warp hands its partner
+    float4 sums[kSplit == 1 ? 1 : kStates][8][32];   // K S over its part of the keys, which a state warp hands its partner
     uint4 states[kGroupsOf][kDim / 16][32];       // S as the output takes it: fp16 left operands, 16 keys each
     uint4 values[2][kGroupsOf][4][32];            // V' as the output takes it, 16 tokens each
-    int state_power[kGroupsOf][2], value_power[2][kGroupsOf];
+    int state_power[kGroupsOf][kSplit], value_power[2][kGroupsOf];
 };
 // Barriers.  A buffer is full (loaders arrive, the others wait) and empty again (the other way round); the two of a pair
-// hand over their sums; a pair's S is ready for its output warp (which waits), and its V' is (all three meet: so a
-// pair is never more than one chunk ahead of its output, whose reads of S are over by then).
+// hand over their sums; S is ready for its output warp (which waits), and V' is (all meet: so states are never more
+// than one chunk ahead of their output, whose reads of S are over by then).
 enum : int { kFull = 0, kEmpty = 2, kPair = 4, kStateReady = 8, kValueReady = 12 };
 
-template <typename T, int kDim, int kGroupsOf>
-__device__ __forceinline__ void load_chunks(const DeltaDev& p, ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int seq, int head, int slice) {
-    constexpr int kAll = ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
-    constexpr int kValueChunks = kGroupsOf * 2;
+template <typename T, int kDim, typename Room>
+__device__ __forceinline__ void load_chunks(const DeltaDev& p, Room& room, int begin, int end, int seq, int head, int slice) {
+    constexpr int kAll = Room::kThreadsOf, kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
+    constexpr int kValueChunks = sizeof(Room::Buffer::v) / (kChunk * 16);
     const skv_gdn_args& a = p.a;
     const int tid = threadIdx.x;
     const T* qh = static_cast<const T*>(a.q) + (head / p.ratio) * kDim;
     const T* kh = static_cast<const T*>(a.k) + (head / p.ratio) * kDim;
-    const T* vh = static_cast<const T*>(a.v) + head * kDim + slice * kGroupsOf * 16;
+    const T* vh = static_cast<const T*>(a.v) + head * kDim + slice * kValueChunks * 8;
     const Record* record = p.records + first_slot(begin, seq) * a.n_v_heads + head;
     int b = 0;
     for (int t0 = begin, n = 0; t0 < end; t0 += kChunk, ++n, b ^= 1, record += a.n_v_heads) {
@@ -625,7 +669,7 @@ __device__ __forceinline__ void load_chunks(const DeltaDev& p, ChunkRoom<kDim, k
         if constexpr (!std::is_same<T, __half>::value) {
             // bfloat16 becomes fp16 where it lies, each thread what it copied
             const float key_down = __ldg(&record->f.key_down);
-#pragma unroll 2
+#pragma unroll 4
             for (int i = 0; i < kMine; ++i) {
                 const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
                 const uint32_t to = chunk_at<kChunks>(r, chunk);
@@ -645,48 +689,44 @@ __device__ __forceinline__ void load_chunks(const DeltaDev& p, ChunkRoom<kDim, k
     }
 }
 
-template <typename T, int kDim, int kGroupsOf>
-__device__ __forceinline__ void advance(ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int head, int slice, float* state) {
-    constexpr int kAll = ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kChunks = kDim / 8, kValueChunks = kGroupsOf * 2;
-    constexpr int kKeys = kDim / 2;                      // per warp of a pair
+/// The chain of states of 16 value columns, over all keys or (a pair of warps) a half of them each.
+template <typename T, int kDim, int kSplit, int kTogether, typename Room>
+__device__ __forceinline__ void advance(Room& room, int begin, int end, int slice, float* state) {
+    constexpr int kAll = Room::kThreadsOf, kMeeting = Room::kMeeting, kChunks = kDim / 8;
+    constexpr int kValueChunks = sizeof(Room::Buffer::v) / (kChunk * 16);
+    constexpr int kKeys = kDim / kSplit;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kProducers, g = lane >> 2, c = lane & 3;
-    const int half = warp & 1, group = warp >> 1, key0 = half * kKeys;
-    const int col0 = (slice * kGroupsOf + group) * 16;   // the pair's value columns
+    const int part = kSplit == 1 ? 0 : warp & 1, group = kSplit == 1 ? warp : warp >> 1, key0 = part * kKeys;
+    const int output = group / kTogether;
+    const int col0 = slice * kValueChunks * 8 + group * 16;   // the group's value columns
     // S^T: rows (value columns) g, g + 8; columns (keys from key0 on) 8 i + 2c, 2c + 1
     float s[kKeys / 8][4];
 #pragma unroll
     for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = state[(key0 + i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8];
-    int b = 0;
+    int b = 0, unit = 0;         // S = 2^unit s
     for (int t0 = begin; t0 < end; t0 += kChunk, b ^= 1) {
         const auto& buf = room.buffer[b];
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kKeys / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(s[i][j]));
-        const int s_power = power_for(warp_largest(top));
-        const float s_down = power_of_two(-s_power), s_up = power_of_two(s_power);
+        const int s_power = max(exponent_of(warp_largest(largest_of(s))) - 14 + unit, -120);
+        const float s_down = power_of_two(unit - s_power), s_up = power_of_two(s_power);
         meet<kAll>(kFull + b);   // and both warps of a pair have read what they handed over
-        const uint32_t k_at = smem_at(buf.k);
         // ---- S^T K^T over the warp's keys
+        const uint32_t k_at = smem_at(buf.k);
         float ks[8][4];
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ks[t][j] = 0.0f;
+        for (int t = 0; t < 8; ++t) ks[t][0] = ks[t][1] = ks[t][2] = ks[t][3] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kKeys / 16; ++i) {
-            uint32_t high[4], low[4];
+            uint32_t high[4], low[4], m[4][4];   // products that add to the same sums are kept apart
+#pragma unroll
+            for (int t = 0; t < 4; ++t) peek_matrices(m[t], k_at + chunk_at<kChunks>(t * 16 + right_row(), key0 / 8 + 2 * i + right_half()));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 split(s[2 * i + (j >> 1)][2 * (j & 1)] * s_down, s[2 * i + (j >> 1)][2 * (j & 1) + 1] * s_down, high[j], low[j]);
-            room.states[group][half * (kKeys / 16) + i][lane] = make_uint4(high[0], high[1], high[2], high[3]);
-            uint32_t m[4][4];   // products that add to the same sums are kept apart
+            room.states[group][key0 / 16 + i][lane] = make_uint4(high[0], high[1], high[2], high[3]);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                load_matrices(m[t], k_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), key0 / 8 + 2 * i + ((lane >> 3) & 1)));
                 multiply(ks[2 * t], high, m[t][0], m[t][1]);
                 multiply(ks[2 * t + 1], high, m[t][2], m[t][3]);
             }
@@ -696,87 +736,79 @@ __device__ __forceinline__ void advance(ChunkRoom<kDim, kGroupsOf>& room, int be
                 multiply(ks[2 * t + 1], low, m[t][2], m[t][3]);
             }
         }
-        if (lane == 0) room.state_power[group][half] = s_power;
-        pass<96>(kStateReady + group);
-        // ---- the other half of the keys
+        if (lane == 0) room.state_power[group][part] = s_power;
+        pass<kMeeting>(kStateReady + output);
+        if constexpr (kSplit == 2) {
+            // ---- the other half of the keys
 #pragma unroll
-        for (int t = 0; t < 8; ++t) room.sums[warp][t][lane] = make_float4(ks[t][0] * s_up, ks[t][1] * s_up, ks[t][2] * s_up, ks[t][3] * s_up);
-        meet<64>(kPair + group);
+            for (int t = 0; t < 8; ++t) room.sums[warp][t][lane] = make_float4(ks[t][0] * s_up, ks[t][1] * s_up, ks[t][2] * s_up, ks[t][3] * s_up);
+            meet<64>(kPair + group);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const float4 x = room.sums[warp ^ 1][t][lane];
-            ks[t][0] = fmaf(ks[t][0], s_up, x.x);
-            ks[t][1] = fmaf(ks[t][1], s_up, x.y);
-            ks[t][2] = fmaf(ks[t][2], s_up, x.z);
-            ks[t][3] = fmaf(ks[t][3], s_up, x.w);
+            for (int t = 0; t < 8; ++t) {
+                const float4 x = room.sums[warp ^ 1][t][lane];
+                ks[t][0] = fmaf(ks[t][0], s_up, x.x);
+                ks[t][1] = fmaf(ks[t][1], s_up, x.y);
+                ks[t][2] = fmaf(ks[t][2], s_up, x.z);
+                ks[t][3] = fmaf(ks[t][3], s_up, x.w);
+            }
         }
         // ---- R = beta (V - e^G K S), in place of K S
-        top = 0.0f;
+        const float k_unit = kSplit == 1 ? s_up : 1.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             uint32_t m[4];
-            load_matrices_t(m, smem_at(buf.v) + chunk_at<kValueChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), group * 2 + ((lane >> 3) & 1)));
+            peek_matrices_t(m, smem_at(buf.v) + chunk_at<kValueChunks>(t * 16 + right_row(), group * 2 + right_half()));
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int at = (2 * t + u) * 8 + 2 * c;
                 const float2 fv = *reinterpret_cast<const float2*>(&buf.record.f.value[at]);
-                const float2 fk = *reinterpret_cast<const float2*>(&buf.record.f.key[at]);
+                float2 fk = *reinterpret_cast<const float2*>(&buf.record.f.key[at]);
+                fk.x *= k_unit;
+                fk.y *= k_unit;
                 const float2 v0 = Pair<T>::up(m[2 * u]), v1 = Pair<T>::up(m[2 * u + 1]);
                 float (&r)[4] = ks[2 * t + u];
                 r[0] = fv.x * v0.x - fk.x * r[0];
                 r[1] = fv.y * v0.y - fk.y * r[1];
                 r[2] = fv.x * v1.x - fk.x * r[2];
                 r[3] = fv.y * v1.y - fk.y * r[3];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(r[j]));
             }
         }
-        const int r_power = power_for(warp_largest(top));
+        const int r_power = power_for(warp_largest(largest_of(ks)));
         const float r_down = power_of_two(-r_power);
         // ---- V' = T R
         float v[8][4];
-        {
-            uint32_t high[4][4], low[4][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 8; ++t) v[t][0] = v[t][1] = v[t][2] = v[t][3] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    split(ks[2 * t + (j >> 1)][2 * (j & 1)] * r_down, ks[2 * t + (j >> 1)][2 * (j & 1) + 1] * r_down, high[t][j], low[t][j]);
+        for (int i = 0; i < 4; ++i) {
+            uint32_t high[4], low[4], m[4][4];
+#pragma unroll
+            for (int t = i; t < 4; ++t) peek_matrices(m[t], smem_at(buf.record.t_high) + block_of(t, i) * kBlockBytes + half_row_at(right_row(), right_half()));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                split(ks[2 * i + (j >> 1)][2 * (j & 1)] * r_down, ks[2 * i + (j >> 1)][2 * (j & 1) + 1] * r_down, high[j], low[j]);
+#pragma unroll
+            for (int t = i; t < 4; ++t) {
+                multiply(v[2 * t], high, m[t][0], m[t][1]);
+                multiply(v[2 * t + 1], high, m[t][2], m[t][3]);
             }
 #pragma unroll
-            for (int t = 0; t < 8; ++t) v[t][0] = v[t][1] = v[t][2] = v[t][3] = 0.0f;
+            for (int t = i; t < 4; ++t) {
+                multiply(v[2 * t], low, m[t][0], m[t][1]);
+                multiply(v[2 * t + 1], low, m[t][2], m[t][3]);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t m[4][4];
-#pragma unroll
-                for (int t = i; t < 4; ++t) {
-                    load_matrices(m[t], smem_at(buf.record.t_high) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
-                    multiply(v[2 * t], high[i], m[t][0], m[t][1]);
-                    multiply(v[2 * t + 1], high[i], m[t][2], m[t][3]);
-                }
-#pragma unroll
-                for (int t = i; t < 4; ++t) {
-                    multiply(v[2 * t], low[i], m[t][0], m[t][1]);
-                    multiply(v[2 * t + 1], low[i], m[t][2], m[t][3]);
-                }
-#pragma unroll
-                for (int t = i; t < 4; ++t) {
-                    load_matrices(m[t], smem_at(buf.record.t_low) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
-                    multiply(v[2 * t], high[i], m[t][0], m[t][1]);
-                    multiply(v[2 * t + 1], high[i], m[t][2], m[t][3]);
-                }
+            for (int t = i; t < 4; ++t) {
+                peek_matrices(m[t], smem_at(buf.record.t_low) + block_of(t, i) * kBlockBytes + half_row_at(right_row(), right_half()));
+                multiply(v[2 * t], high, m[t][0], m[t][1]);
+                multiply(v[2 * t + 1], high, m[t][2], m[t][3]);
             }
         }
-        const int v_unit = r_power - 10;   // V' = 2^v_unit v
-        // ---- V' for the output, from one warp of the pair
-        if (half == 0) {
-            top = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 8; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[t][j]));
-            const int least = max(max(s_power, room.state_power[group][1]) - 60, -120);
-            const int o_power = min(max(exponent_of(warp_largest(top)) - 14 + v_unit, least), 120);
+        const int v_unit = r_power - 10;   // V' = 2^v_unit v: T is kInverseScale = 2^10 times itself
+        // ---- V' for the output, from one warp of a pair
+        if (part == 0) {
+            const int most = kSplit == 1 ? s_power : max(s_power, room.state_power[group][kSplit - 1]);
+            const int o_power = min(max(exponent_of(warp_largest(largest_of(v))) - 14 + v_unit, max(most - 60, -120)), 120);
             const float v_down = power_of_two(v_unit - o_power);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -786,136 +818,163 @@ __device__ __forceinline__ void advance(ChunkRoom<kDim, kGroupsOf>& room, int be
                                Pair<__half>::down(v[2 * t + 1][2] * v_down, v[2 * t + 1][3] * v_down));
             if (lane == 0) room.value_power[b][group] = o_power;
         }
-        meet<96>(kValueReady + group);
+        meet<kMeeting>(kValueReady + output);
         // ---- S <- e^(G_63) S + K^T (e^(G_63 - G) V')
-        {
-            top = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.update[t * 8 + 2 * c]);
+        for (int t = 0; t < 8; ++t) {
+            const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.update[t * 8 + 2 * c]);
+            v[t][0] *= f.x;
+            v[t][1] *= f.y;
+            v[t][2] *= f.x;
+            v[t][3] *= f.y;
+        }
+        // one power for S and the update: the update's, or 2^-60 of what S would need where the update is smaller yet
+        int w_power = exponent_of(warp_largest(largest_of(v))) - 14 + v_unit;
+        w_power = min(max(w_power, max(s_power - 60, -120)), 120);
+        const float w_down = power_of_two(v_unit - w_power), keep = buf.record.f.whole * power_of_two(unit - w_power);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[t][j] *= j & 1 ? f.y : f.x;
-                    top = fmaxf(top, fabsf(v[t][j]));
+        for (int i = 0; i < kKeys / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] *= keep;
+        unit = w_power;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            uint32_t high[4], low[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                split(v[2 * t + (j >> 1)][2 * (j & 1)] * w_down, v[2 * t + (j >> 1)][2 * (j & 1) + 1] * w_down, high[j], low[j]);
+#pragma unroll
+            for (int h = 0; h < kKeys / 64 + (kKeys < 64); ++h) {   // 64 keys at a time
+                constexpr int kDeep = kKeys < 64 ? kKeys / 16 : 4;
+                uint32_t m[kDeep][4];
+#pragma unroll
+                for (int i = 0; i < kDeep; ++i)
+                    peek_matrices_t(m[i], k_at + chunk_at<kChunks>(t * 16 + (lane & 15), key0 / 8 + 2 * (h * 4 + i) + (lane >> 4)));
+#pragma unroll
+                for (int i = 0; i < kDeep; ++i) {
+                    multiply(s[2 * (h * 4 + i)], high, m[i][0], m[i][1]);
+                    multiply(s[2 * (h * 4 + i) + 1], high, m[i][2], m[i][3]);
+                }
+#pragma unroll
+                for (int i = 0; i < kDeep; ++i) {
+                    multiply(s[2 * (h * 4 + i)], low, m[i][0], m[i][1]);
+                    multiply(s[2 * (h * 4 + i) + 1], low, m[i][2], m[i][3]);
                 }
             }
-            // one power for S and the update: the update's, or 2^-60 of what S would need where the update is smaller yet
-            int w_power = exponent_of(warp_largest(top)) - 14 + v_unit;
-            w_power = min(max(w_power, max(s_power - 60, -120)), 120);
-            const float w_down = power_of_two(v_unit - w_power);
-            const float keep = buf.record.f.whole * power_of_two(-w_power), up = power_of_two(w_power);
-#pragma unroll
-            for (int i = 0; i < kKeys / 8; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[i][j] *= keep;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                uint32_t high[4], low[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    split(v[2 * t + (j >> 1)][2 * (j & 1)] * w_down, v[2 * t + (j >> 1)][2 * (j & 1) + 1] * w_down, high[j], low[j]);
-                uint32_t m[kKeys / 16][4];
-#pragma unroll
-                for (int i = 0; i < kKeys / 16; ++i) {
-                    load_matrices_t(m[i], k_at + chunk_at<kChunks>(t * 16 + (lane & 15), key0 / 8 + 2 * i + (lane >> 4)));
-                    multiply(s[2 * i], high, m[i][0], m[i][1]);
-                    multiply(s[2 * i + 1], high, m[i][2], m[i][3]);
-                }
-#pragma unroll
-                for (int i = 0; i < kKeys / 16; ++i) {
-                    multiply(s[2 * i], low, m[i][0], m[i][1]);
-                    multiply(s[2 * i + 1], low, m[i][2], m[i][3]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kKeys / 8; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[i][j] *= up;
         }
         if (t0 + 2 * kChunk < end) pass<kAll>(kEmpty + b);
     }
 #pragma unroll
     for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) state[(key0 + i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8] = s[i][j];
+        for (int j = 0; j < 4; ++j)
+            state[(key0 + i * 8 + 2 * c + (j & 1)) * kDim + col0 + g + (j >> 1) * 8] = s[i][j] * power_of_two(unit);
 }
 
-/// O = scale (e^G Q S + P V') of one pair's columns.
-template <typename T, int kDim, int kGroupsOf>
-__device__ __forceinline__ void put_out(const DeltaDev& p, ChunkRoom<kDim, kGroupsOf>& room, int begin, int end, int head, int slice) {
-    constexpr int kAll = ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kChunks = kDim / 8;
+/// O = scale (e^G Q S + P V') of kTogether groups' columns.
+template <typename T, int kDim, int kSplit, int kTogether, typename Room>
+__device__ __forceinline__ void put_out(const DeltaDev& p, Room& room, int begin, int end, int head, int slice) {
+    constexpr int kAll = Room::kThreadsOf, kMeeting = Room::kMeeting, kChunks = kDim / 8, kDeep = kDim / kSplit / 16;
+    constexpr int kValueChunks = sizeof(Room::Buffer::v) / (kChunk * 16);
     const skv_gdn_args& a = p.a;
-    const int lane = threadIdx.x & 31, group = (threadIdx.x >> 5) - kProducers - 2 * kGroupsOf, g = lane >> 2, c = lane & 3;
-    T* const out = static_cast<T*>(a.out) + head * kDim + (slice * kGroupsOf + group) * 16 + 2 * c;
+    const int lane = threadIdx.x & 31, output = (threadIdx.x >> 5) - kProducers - Room::kStates, g = lane >> 2, c = lane & 3;
+    T* const out = static_cast<T*>(a.out) + head * kDim + slice * kValueChunks * 8 + output * kTogether * 16 + 2 * c;
     int b = 0;
     for (int t0 = begin; t0 < end; t0 += kChunk, b ^= 1) {
         const auto& buf = room.buffer[b];
-        float o[8][4];
+        float o[kTogether][8][4];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+        for (int y = 0; y < kTogether; ++y)
+#pragma unroll
+            for (int t = 0; t < 8; ++t) o[y][t][0] = o[y][t][1] = o[y][t][2] = o[y][t][3] = 0.0f;
         meet<kAll>(kFull + b);
-        meet<96>(kStateReady + group);
-        // the half of the keys with the smaller power first: its sums are scaled down to the other's
-        const int power0 = room.state_power[group][0], power1 = room.state_power[group][1], first = power1 < power0;
+        meet<kMeeting>(kStateReady + output);
+        // of a pair, the part with the smaller power first: its sums are scaled down to the other's
+        int s_power[kTogether], first = 0;
+#pragma unroll
+        for (int y = 0; y < kTogether; ++y) s_power[y] = room.state_power[output * kTogether + y][0];
+        const int other = kSplit == 1 ? s_power[0] : room.state_power[output * kTogether][kSplit - 1];
+        static_assert(kSplit == 1 || kTogether == 1, "one order of the parts");
+        if constexpr (kSplit == 2) first = other < s_power[0];
         const uint32_t q_at = smem_at(buf.q);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kSplit; ++h) {
             if (h == 1) {
-                const float down = power_of_two(-abs(power1 - power0));
+                const float down = power_of_two(-abs(other - s_power[0]));
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[t][j] *= down;
+                    for (int j = 0; j < 4; ++j) o[0][t][j] *= down;
             }
 #pragma unroll
-            for (int u = 0; u < kDim / 32; ++u) {
-                const int i = (first ^ h) * (kDim / 32) + u;
-                const uint4 x = room.states[group][i][lane];
-                const uint32_t high[4] = {x.x, x.y, x.z, x.w};
+            for (int u = 0; u < kDeep; ++u) {
+                const int i = (first ^ h) * kDeep + u;
+                uint32_t high[kTogether][4];
+#pragma unroll
+                for (int y = 0; y < kTogether; ++y) {
+                    const uint4 x = room.states[output * kTogether + y][i][lane];
+                    high[y][0] = x.x; high[y][1] = x.y; high[y][2] = x.z; high[y][3] = x.w;
+                }
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     uint32_t m[4];
-                    load_matrices(m, q_at + chunk_at<kChunks>(t * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
-                    multiply(o[2 * t], high, m[0], m[1]);
-                    multiply(o[2 * t + 1], high, m[2], m[3]);
+                    peek_matrices(m, q_at + chunk_at<kChunks>(t * 16 + right_row(), 2 * i + right_half()));
+#pragma unroll
+                    for (int y = 0; y < kTogether; ++y) {
+                        multiply(o[y][2 * t], high[y], m[0], m[1]);
+                        multiply(o[y][2 * t + 1], high[y], m[2], m[3]);
+                    }
                 }
             }
         }
-        const int s_power = max(power0, power1);
-        meet<96>(kValueReady + group);
-        const int o_power = room.value_power[b][group];
-        const float fit = power_of_two(s_power - o_power), up = power_of_two(o_power);
+        if constexpr (kSplit == 2) s_power[0] = max(s_power[0], other);
+        meet<kMeeting>(kValueReady + output);
+        float up[kTogether];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.query[t * 8 + 2 * c]);
-            o[t][0] *= f.x * fit;
-            o[t][1] *= f.y * fit;
-            o[t][2] *= f.x * fit;
-            o[t][3] *= f.y * fit;
+        for (int y = 0; y < kTogether; ++y) {
+            const int o_power = room.value_power[b][output * kTogether + y];
+            const float fit = power_of_two(s_power[y] - o_power);
+            up[y] = power_of_two(o_power);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.query[t * 8 + 2 * c]);
+                o[y][t][0] *= f.x * fit;
+                o[y][t][1] *= f.y * fit;
+                o[y][t][2] *= f.x * fit;
+                o[y][t][3] *= f.y * fit;
+            }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 x = room.values[b][group][i][lane];
-            const uint32_t high[4] = {x.x, x.y, x.z, x.w};
+            uint32_t high[kTogether][4];
+#pragma unroll
+            for (int y = 0; y < kTogether; ++y) {
+                const uint4 x = room.values[b][output * kTogether + y][i][lane];
+                high[y][0] = x.x; high[y][1] = x.y; high[y][2] = x.z; high[y][3] = x.w;
+            }
 #pragma unroll
             for (int t = i; t < 4; ++t) {
                 uint32_t m[4];
-                load_matrices(m, smem_at(buf.record.mix) + block_of(t, i) * kBlockBytes + half_row_at((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1));
-                multiply(o[2 * t], high, m[0], m[1]);
-                multiply(o[2 * t + 1], high, m[2], m[3]);
+                peek_matrices(m, smem_at(buf.record.mix) + block_of(t, i) * kBlockBytes + half_row_at(right_row(), right_half()));
+#pragma unroll
+                for (int y = 0; y < kTogether; ++y) {
+                    multiply(o[y][2 * t], high[y], m[0], m[1]);
+                    multiply(o[y][2 * t + 1], high[y], m[2], m[3]);
+                }
             }
         }
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            float2 f = *reinterpret_cast<const float2*>(&buf.record.f.out[t * 8 + 2 * c]);
-            f.x *= up;
-            f.y *= up;
-            const uint32_t lo = transpose8(Pair<T>::down(o[t][0] * f.x, o[t][1] * f.y));
-            const uint32_t hi = transpose8(Pair<T>::down(o[t][2] * f.x, o[t][3] * f.y));
+            const float2 f = *reinterpret_cast<const float2*>(&buf.record.f.out[t * 8 + 2 * c]);
             const int token = t0 + t * 8 + g;
-            if (token < end) {
-                *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride) = lo;
-                *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride + 8) = hi;
+#pragma unroll
+            for (int y = 0; y < kTogether; ++y) {
+                const uint32_t lo = transpose8(Pair<T>::down(o[y][t][0] * up[y] * f.x, o[y][t][1] * up[y] * f.y));
+                const uint32_t hi = transpose8(Pair<T>::down(o[y][t][2] * up[y] * f.x, o[y][t][3] * up[y] * f.y));
+                if (token < end) {
+                    *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride + y * 16) = lo;
+                    *reinterpret_cast<uint32_t*>(out + (int64_t) token * a.out_stride + y * 16 + 8) = hi;
+                }
             }
         }
         if (t0 + 2 * kChunk < end) pass<kAll>(kEmpty + b);
@@ -923,18 +982,18 @@ __device__ __forceinline__ void put_out(const DeltaDev& p, ChunkRoom<kDim, kGrou
 }
 
 /// Registers per thread of the roles where the CTA has 512 threads: they add up to what it was launched with.
-constexpr int kLoaderRegisters = 64, kStateRegisters = 176, kOutputRegisters = 96;
+constexpr int kLoaderRegisters = 48, kStateRegisters = 176, kOutputRegisters = 112;
 static_assert(kLoaderRegisters * 128 + kStateRegisters * 256 + kOutputRegisters * 128 == 128 * 512, "the shares of 512 threads launched with 128 each");
 
-template <typename T, int kDim, int kGroupsOf>
-__global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf>::kThreadsOf, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
+template <typename T, int kDim, int kGroupsOf, int kSplit, int kTogether>
+__global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf, kSplit, kTogether>::kThreadsOf, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
+    using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether>;
     extern __shared__ __align__(128) uint8_t smem[];
-    auto& room = *reinterpret_cast<ChunkRoom<kDim, kGroupsOf>*>(smem);
-    constexpr int kSlices = kDim / (kGroupsOf * 16);
-    constexpr bool kShares = kGroupsOf == 4;
+    auto& room = *reinterpret_cast<Room*>(smem);
+    constexpr bool kShares = Room::kThreadsOf == 512;
     const skv_gdn_args& a = p.a;
-    const int slice = blockIdx.x % kSlices;
-    const int64_t item = blockIdx.x / kSlices;
+    const int slice = blockIdx.x % Room::kSlices;
+    const int64_t item = blockIdx.x / Room::kSlices;
     const int head = (int) (item % a.n_v_heads), seq = (int) (item / a.n_v_heads);
     int begin, end;
     if (!tokens_of(a, seq, begin, end)) return;
@@ -943,13 +1002,13 @@ __global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf>::kThreadsOf, 1) chu
     const int warp = threadIdx.x >> 5;
     if (warp < kProducers) {
         if constexpr (kShares) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegisters));
-        load_chunks<T, kDim, kGroupsOf>(p, room, begin, end, seq, head, slice);
-    } else if (warp < kProducers + 2 * kGroupsOf) {
+        load_chunks<T, kDim>(p, room, begin, end, seq, head, slice);
+    } else if (warp < kProducers + Room::kStates) {
         if constexpr (kShares) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kStateRegisters));
-        advance<T, kDim, kGroupsOf>(room, begin, end, head, slice, state);
+        advance<T, kDim, kSplit, kTogether>(room, begin, end, slice, state);
     } else {
         if constexpr (kShares) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOutputRegisters));
-        put_out<T, kDim, kGroupsOf>(p, room, begin, end, head, slice);
+        put_out<T, kDim, kSplit, kTogether>(p, room, begin, end, head, slice);
     }
 }
 
@@ -961,35 +1020,37 @@ cudaError_t launch_tokens(const DeltaDev& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <typename T, int kDim, int kGroupsOf>
+template <typename T, int kDim, int kGroupsOf, int kSplit, int kTogether>
 cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
-    constexpr int kSmem = sizeof(ChunkRoom<kDim, kGroupsOf>), kPrepare = sizeof(PrepareRoom<kDim>);
+    using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether>;
+    constexpr auto kKernel = chunk_kernel<T, kDim, kGroupsOf, kSplit, kTogether>;
+    constexpr int kSmem = sizeof(Room), kPrepare = sizeof(PrepareRoom<kDim>);
     static_assert(kSmem <= 227 * 1024, "the buffers fit an SM");
-    if constexpr (kGroupsOf == 4) {
+    if constexpr (Room::kThreadsOf == 512) {
         // the roles' shares add up only if the CTA was launched with the registers they were made for
         static const int registers = [] {
             cudaFuncAttributes f{};
-            return cudaFuncGetAttributes(&f, chunk_kernel<T, kDim, kGroupsOf>) == cudaSuccess ? f.numRegs : 0;
+            return cudaFuncGetAttributes(&f, kKernel) == cudaSuccess ? f.numRegs : 0;
         }();
         if (registers != 128) return cudaErrorInvalidConfiguration;
     }
     cudaError_t e = cudaFuncSetAttribute(prepare_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepare);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk_kernel<T, kDim, kGroupsOf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     prepare_kernel<T, kDim><<<(unsigned) (record_slots(p.a.n_tokens, p.a.n_seqs) * p.a.n_k_heads), kProducerThreads, kPrepare, stream>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const unsigned grid = (unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * (kDim / (kGroupsOf * 16)));
-    chunk_kernel<T, kDim, kGroupsOf><<<grid, ChunkRoom<kDim, kGroupsOf>::kThreadsOf, kSmem, stream>>>(p);
+    kKernel<<<(unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * Room::kSlices), Room::kThreadsOf, kSmem, stream>>>(p);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch(const DeltaDev& p, int sms, cudaStream_t stream) {
     if (!chunked(p.a.seq_starts != nullptr, p.a.max_tokens)) return launch_tokens<T>(p, stream);
+    // slices of 32 columns with the keys in halves while all of their CTAs run at once, else a CTA per head
     const bool few = (int64_t) p.a.n_seqs * p.a.n_v_heads * (p.a.head_dim / 32) <= sms;
-    if (p.a.head_dim == 64) return few ? launch_chunks<T, 64, 2>(p, stream) : launch_chunks<T, 64, 4>(p, stream);
-    return few ? launch_chunks<T, 128, 2>(p, stream) : launch_chunks<T, 128, 4>(p, stream);
+    if (p.a.head_dim == 64) return few ? launch_chunks<T, 64, 2, 2, 1>(p, stream) : launch_chunks<T, 64, 4, 1, 2>(p, stream);
+    return few ? launch_chunks<T, 128, 2, 2, 1>(p, stream) : launch_chunks<T, 128, 8, 1, 2>(p, stream);
 }
 
 }  // namespace

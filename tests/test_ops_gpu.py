@@ -433,6 +433,20 @@ def test_delta_ragged(torch_cuda, kind, kh, vh, d, counts):
     check_delta(torch, x, first, state, out, starts, list(range(len(counts))))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("kh,vh,d", [(8, 24, 128), (20, 40, 64)])
+def test_delta_fills_the_gpu(torch_cuda, kind, kh, vh, d):
+    """More heads and sequences than fit at once: a whole head per CTA."""
+    torch = torch_cuda
+    counts = [130, 1, 64, 65, 0, 200, 31]
+    x = delta_inputs(torch, 75, 1 + sum(counts) + 2, kh, vh, d, getattr(torch, kind))
+    state = normal(torch, 79, len(counts), vh, d, d, scale=0.1)
+    first = state.clone()
+    out, starts = run_delta(torch, x, state, counts, 1)
+    assert status(torch) == 0
+    check_delta(torch, x, first, state, out, starts, list(range(len(counts))))
+
+
 @pytest.mark.parametrize("n", [1, 5, 130])
 def test_delta_one_token_each(torch_cuda, n):
     """The decode form: no starts; the rows' order given by an index, strided inputs and rows."""
