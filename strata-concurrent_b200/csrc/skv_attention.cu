@@ -51,9 +51,9 @@ struct AttnDev {
 template <int kDim, bool kInt8>
 struct Geo {
     static constexpr int kRowBytes = kDim * (kInt8 ? 1 : 2);
-    // cells per tile: a plane (K or V of a tile) of 32 KiB, at most a lane per cell of a warp; 96 where four sets of weights
-    // lie beside it
-    static constexpr int kTile = kInt8 && kDim == 256 ? 96 : 32768 / kRowBytes < 128 ? 32768 / kRowBytes : 128;
+    // cells per tile: a plane (K or V of a tile) of 32 KiB, at most a lane per cell of a warp; 16 KiB where four sets of
+    // weights lie beside it
+    static constexpr int kTile = kInt8 && kDim == 256 ? 64 : 32768 / kRowBytes < 128 ? 32768 / kRowBytes : 128;
     static constexpr int kCells = kTile / kWarps;                                     // per warp
     static constexpr int kChunks = kRowBytes / 16;
     static constexpr int kGroups = kInt8 ? kDim / kInt8Group : 1;
@@ -62,7 +62,9 @@ struct Geo {
     static constexpr int kSlotBytes = kPlane + kTile * kScaleBytes;
     static constexpr int kWeightStride = kTile + 8;   // halves: rows 16 bytes apart modulo 128, ldmatrix meets no bank twice
     static constexpr int kWeightBytes = kGroups * kRows * kWeightStride * 2;
-    static constexpr int kSmem = 3 * kSlotBytes + kWeightBytes;   // K, and V twice
+    static constexpr int kQueryStride = kDim + 8;     // halves
+    static constexpr int kQueryBytes = kInt8 ? kRows * kQueryStride * 2 : 0;
+    static constexpr int kSmem = 3 * kSlotBytes + kWeightBytes + kQueryBytes;   // K, and V twice
     static constexpr int kPerSm = kPlane > 24000 ? 2 : kPlane > 12000 ? 3 : 4;   // CTAs: enough copies in flight
     static constexpr int kCols = kDim / kWarps;       // of the output, per warp
     static constexpr int kOutTiles = kCols / 8;
@@ -287,44 +289,97 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
     issue_k();
     issue_v(1, true);
 
-    // ---- the item's query, 16 heads x kDim, as the left operands of all its products
-    uint32_t q[kDim / 16][4];
+    // ---- the item's query, 16 heads x kDim, the left operand of all its products: of an fp16 cache in registers; of an int8
+    // one, whose conversions need those, in shared memory
+    uint32_t q[kInt8 ? 1 : kDim / 16][4];
     float factor[2];   // of rows g and g + 8: scale, log2 e, and the power of two the row was divided by
+    uint8_t* const queries = smem + 3 * G::kSlotBytes + G::kWeightBytes;
+    __shared__ float s_factor[kRows];
+    // the power of two that a row is divided by; in range for every finite row, 1 for one with an infinity
+    const auto power_of_row = [](float top) {
+        return top > 0.0f && top < INFINITY ? min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -126), 126) : 0;
+    };
     auto load_query = [&]() {
         const int kv = here.item / p.blocks, first = (here.item % p.blocks) * kRows;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = first + g + h * 8;
+        if constexpr (kInt8) {
+            // eight lanes a row; of each 16 values 4c, 4c+1 go to places 2c, 2c+1 and 4c+2, 4c+3 to 2c+8, 2c+9, so that
+            // the operand's columns meet K's as a register of four codes holds them
+            const int row = tid >> 3, r = first + row;
             const bool on = r < p.group;
             const T* src = static_cast<const T*>(a.q) + (int64_t) here.seq * a.q_stride + (int64_t) (kv * p.group + (on ? r : 0)) * kDim;
             float top = 0.0f;
+            constexpr int kPieces = kDim / 64;    // of 8 values, per lane
+            uint4 w[kPieces];
 #pragma unroll
-            for (int i = 0; i < kDim / 16; ++i) {
-                // fp16 cache: values 2c, 2c+1 and 2c+8, 2c+9 of each 16, as ldmatrix hands out K's rows;
-                // int8: values 4c .. 4c+3, as a register of four codes holds them
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(src + i * 16);
-                q[i][h] = on ? w[kInt8 ? 2 * c : c] : 0u;
-                q[i][h + 2] = on ? w[kInt8 ? 2 * c + 1 : c + 4] : 0u;
-                if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
-                    const float2 x = Pair<T>::up(q[i][h]), y = Pair<T>::up(q[i][h + 2]);
-                    top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+            for (int i = 0; i < kPieces; ++i) {
+                w[i] = on ? *reinterpret_cast<const uint4*>(src + ((tid & 7) * kPieces + i) * 8) : make_uint4(0, 0, 0, 0);
+                if constexpr (!std::is_same<T, __half>::value) {
+                    float x[8];
+                    unpack8<T>(w[i], x);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
                 }
             }
             int e = 0;
             if constexpr (!std::is_same<T, __half>::value) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // 2^-e in range for every finite row; a row with an infinity keeps it
-                e = top > 0.0f && top < INFINITY ? min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -126), 126) : 0;
+#pragma unroll
+                for (int m = 1; m < 8; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+                e = power_of_row(top);
                 const float down = power_of_two(-e);
 #pragma unroll
-                for (int i = 0; i < kDim / 16; ++i) {
-                    const float2 x = Pair<T>::up(q[i][h]), y = Pair<T>::up(q[i][h + 2]);
-                    q[i][h] = Pair<__half>::down(x.x * down, x.y * down);
-                    q[i][h + 2] = Pair<__half>::down(y.x * down, y.y * down);
+                for (int i = 0; i < kPieces; ++i) {
+                    float x[8];
+                    unpack8<T>(w[i], x);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] *= down;
+                    w[i] = pack8<__half>(x);
                 }
             }
-            factor[h] = a.scale * 1.4426950408889634f * power_of_two(e);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                // half of a block of 16: its pairs 0 and 2 go to the first eight places, 1 and 3 to the last eight
+                const int piece = (tid & 7) * kPieces + i;
+                uint2* to = reinterpret_cast<uint2*>(queries + (row * G::kQueryStride + piece / 2 * 16 + (piece & 1) * 4) * 2);
+                to[0] = make_uint2(w[i].x, w[i].z);
+                to[2] = make_uint2(w[i].y, w[i].w);
+            }
+            if ((tid & 7) == 0) s_factor[row] = a.scale * 1.4426950408889634f * power_of_two(e);
+            meet();
+            factor[0] = s_factor[g];
+            factor[1] = s_factor[g + 8];
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = first + g + h * 8;
+                const bool on = r < p.group;
+                const T* src = static_cast<const T*>(a.q) + (int64_t) here.seq * a.q_stride + (int64_t) (kv * p.group + (on ? r : 0)) * kDim;
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kDim / 16; ++i) {
+                    // values 2c, 2c+1 and 2c+8, 2c+9 of each 16, as ldmatrix hands out K's rows
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(src + i * 16);
+                    q[i][h] = on ? w[c] : 0u;
+                    q[i][h + 2] = on ? w[c + 4] : 0u;
+                    if constexpr (!std::is_same<T, __half>::value) {
+                        const float2 x = Pair<T>::up(q[i][h]), y = Pair<T>::up(q[i][h + 2]);
+                        top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+                    }
+                }
+                int e = 0;
+                if constexpr (!std::is_same<T, __half>::value) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    e = power_of_row(top);
+                    const float down = power_of_two(-e);
+#pragma unroll
+                    for (int i = 0; i < kDim / 16; ++i) {
+                        const float2 x = Pair<T>::up(q[i][h]), y = Pair<T>::up(q[i][h + 2]);
+                        q[i][h] = Pair<__half>::down(x.x * down, x.y * down);
+                        q[i][h + 2] = Pair<__half>::down(y.x * down, y.y * down);
+                    }
+                }
+                factor[h] = a.scale * 1.4426950408889634f * power_of_two(e);
+            }
         }
     };
     load_query();
@@ -354,9 +409,9 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         constexpr int kTiles = G::kCells / 8;
         float score[kTiles][4];
         const uint32_t k_at = smem_at(smem) + warp * G::kCells * G::kRowBytes;
+        if constexpr (!kInt8) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            if constexpr (!kInt8) {
+            for (int t = 0; t < kTiles; ++t) {
                 float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};   // two chains of sums
 #pragma unroll
                 for (int i = 0; i < kDim / 32; ++i) {
@@ -367,27 +422,36 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) score[t][j] = x[j] + y[j];
-            } else {
-                score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.0f;
-                const int cell = t * 8 + 2 * c;
-                const uint8_t* s_at = smem + G::kPlane + (warp * G::kCells + cell) * G::kScaleBytes;
+            }
+        } else {
+            const uint32_t q_at = smem_at(queries) + ((lane & 15) * G::kQueryStride + (lane >> 4) * 8) * 2;
 #pragma unroll
-                for (int i = 0; i < G::kGroups; ++i) {
+            for (int t = 0; t < kTiles; ++t) score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < G::kGroups; ++i) {
+                uint32_t w[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) load_matrices(w[j], q_at + (i * 4 + j) * 32);
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
                     uint32_t b[4];
                     load_matrices(b, k_at + chunk_at<G::kChunks>(t * 8 + (lane & 7), i * 4 + (lane >> 3)));
-                    float x[4] = {0, 0, 0, 0};
+                    float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t u = b[j] ^ 0x80808080u;
-                        multiply(x, q[4 * i + j], codes_to_half<0x4140>(u), codes_to_half<0x4342>(u));
-                    }
+                    for (int j = 0; j < 4; ++j) b[j] ^= 0x80808080u;
+                    multiply(x, w[0], codes_to_half<0x4140>(b[0]), codes_to_half<0x4342>(b[0]));
+                    multiply(y, w[1], codes_to_half<0x4140>(b[1]), codes_to_half<0x4342>(b[1]));
+                    multiply(x, w[2], codes_to_half<0x4140>(b[2]), codes_to_half<0x4342>(b[2]));
+                    multiply(y, w[3], codes_to_half<0x4140>(b[3]), codes_to_half<0x4342>(b[3]));
+                    const int cell = t * 8 + 2 * c;
+                    const uint8_t* s_at = smem + G::kPlane + (warp * G::kCells + cell) * G::kScaleBytes;
                     const int h0 = kDim == 64 ? (odd_now >> cell) & 1 : i, h1 = kDim == 64 ? (odd_now >> (cell + 1)) & 1 : i;
                     const float s0 = __half2float(reinterpret_cast<const __half*>(s_at)[h0]);
                     const float s1 = __half2float(reinterpret_cast<const __half*>(s_at + G::kScaleBytes)[h1]);
-                    score[t][0] = fmaf(x[0], s0, score[t][0]);
-                    score[t][1] = fmaf(x[1], s1, score[t][1]);
-                    score[t][2] = fmaf(x[2], s0, score[t][2]);
-                    score[t][3] = fmaf(x[3], s1, score[t][3]);
+                    score[t][0] = fmaf(x[0] + y[0], s0, score[t][0]);
+                    score[t][1] = fmaf(x[1] + y[1], s1, score[t][1]);
+                    score[t][2] = fmaf(x[2] + y[2], s0, score[t][2]);
+                    score[t][3] = fmaf(x[3] + y[3], s1, score[t][3]);
                 }
             }
         }
