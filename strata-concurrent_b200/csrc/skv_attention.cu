@@ -111,6 +111,25 @@ __device__ __forceinline__ uint32_t codes_to_half(uint32_t biased) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x6480)));   // 1152
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+/// The scales of a cell's groups; head_dim 64 has one, in the lower or the upper (`odd`) half of its word.
+template <int kGroups>
+__device__ __forceinline__ void load_scales(const uint8_t* at, bool odd, float (&x)[kGroups]) {
+    if constexpr (kGroups == 1) x[0] = __half2float(reinterpret_cast<const __half*>(at)[odd]);
+    else {
+        uint32_t w[kGroups / 2];
+        if constexpr (kGroups == 4) {
+            const uint2 y = *reinterpret_cast<const uint2*>(at);
+            w[0] = y.x;
+            w[1] = y.y;
+        } else w[0] = *reinterpret_cast<const uint32_t*>(at);
+#pragma unroll
+        for (int i = 0; i < kGroups / 2; ++i) {
+            const float2 f = Pair<__half>::up(w[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
 __device__ __forceinline__ float power_of_two(int e) {   // e clamped to the normal numbers
     return __int_as_float((min(max(e, -126), 127) + 127) << 23);
 }
@@ -173,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
     using G = Geo<kDim, kInt8>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_top[kWarps][kRows], s_sum[kWarps][kRows];
-    __shared__ int s_power[kWarps][4];   // int8: per V scale group
+    __shared__ alignas(16) int s_power[kWarps][4];   // int8: per V scale group
     __shared__ int64_t s_scan[kWarps];
     __shared__ int64_t s_first[2];   // the first sequence of the share, and the tiles before it
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -477,14 +496,16 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
             // the largest V scale of the warp's cells per group, as the power of two above it
             wait_async<1>();              // V of this tile
             meet_warp();
-            const uint8_t* s_at = v_base + G::kPlane + (warp * G::kCells + (lane < G::kCells ? lane : 0)) * G::kScaleBytes;
+            float scale[G::kGroups];
+            load_scales(v_base + G::kPlane + (warp * G::kCells + (lane < G::kCells ? lane : 0)) * G::kScaleBytes, (odd_now >> lane) & 1, scale);
+            int e[4] = {-24, -24, -24, -24};
 #pragma unroll
             for (int i = 0; i < G::kGroups; ++i) {
-                const float s = fabsf(__half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd_now >> lane) & 1 : i]));
-                int e = s > 0.0f && lane < G::kCells ? ((__float_as_int(s) >> 23) & 0xff) - 126 : -24;
-                e = __reduce_max_sync(0xffffffffu, e);
-                if (lane == 0) s_power[warp][i] = min(e, 17);
+                const float s = fabsf(scale[i]);
+                const int x = s > 0.0f && lane < G::kCells ? min(((__float_as_int(s) >> 23) & 0xff) - 126, 17) : -24;
+                e[i] = __reduce_max_sync(0xffffffffu, x);
             }
+            if (lane == 0) *reinterpret_cast<int4*>(s_power[warp]) = make_int4(e[0], e[1], e[2], e[3]);
         }
         meet();   // row maxima; and every warp is done with V of the tile before, whose slot is filled again
         issue_v(3 - v_slot, n + 1 < count);
@@ -503,11 +524,18 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         if constexpr (kInt8) {
             // within an item a power only grows: what was summed under a smaller one is scaled down
             const int mine = warp * G::kCols / kInt8Group;
+            int most[4] = {-24, -24, -24, -24};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const int4 x = *reinterpret_cast<const int4*>(s_power[w]);
+                most[0] = max(most[0], x.x);
+                most[1] = max(most[1], x.y);
+                most[2] = max(most[2], x.z);
+                most[3] = max(most[3], x.w);
+            }
 #pragma unroll
             for (int i = 0; i < G::kGroups; ++i) {
-                int x = powers[i];
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) x = max(x, s_power[w][i]);
+                const int x = max(powers[i], most[i]);
                 if (i == mine) shrink = power_of_two(powers[i] - x);
                 powers[i] = x;
             }
@@ -529,11 +557,12 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
             } else {
                 const uint8_t* s_at = v_base + G::kPlane + cell * G::kScaleBytes;
                 const int in = t * 8 + 2 * c;
+                float v0[G::kGroups], v1[G::kGroups];
+                load_scales(s_at, (odd_now >> in) & 1, v0);
+                load_scales(s_at + G::kScaleBytes, (odd_now >> (in + 1)) & 1, v1);
 #pragma unroll
                 for (int i = 0; i < G::kGroups; ++i) {
-                    const float down = power_of_two(-powers[i]);
-                    const float s0 = down * __half2float(reinterpret_cast<const __half*>(s_at)[kDim == 64 ? (odd_now >> in) & 1 : i]);
-                    const float s1 = down * __half2float(reinterpret_cast<const __half*>(s_at + G::kScaleBytes)[kDim == 64 ? (odd_now >> (in + 1)) & 1 : i]);
+                    const float down = power_of_two(-powers[i]), s0 = down * v0[i], s1 = down * v1[i];
                     uint32_t* at = reinterpret_cast<uint32_t*>(weights + ((i * kRows + g) * G::kWeightStride + cell) * 2);
                     at[0] = Pair<__half>::down(w[0] * s0, w[1] * s1);
                     at[8 * G::kWeightStride / 2] = Pair<__half>::down(w[2] * s0, w[3] * s1);
