@@ -305,7 +305,7 @@ template <int kDim>
 struct PrepareRoom {
     union {
         struct { uint8_t k[kChunk * kDim * 2], q[kChunk * kDim * 2]; } in;
-        struct { float a[kChunk * kScratch], t[kChunk * kScratch], x[kChunk / 2 * kScratch]; } work;
+        struct { float a[kChunk * kScratch], t[kChunk * kScratch]; } work;   // X lies in A's rows 0 - 31, columns 32 - 63, which hold nothing
     };
     alignas(16) uint8_t mix[kTriangleBytes];
     float2 sums[kChunk];      // G log2 e in two parts
@@ -316,49 +316,49 @@ struct PrepareRoom {
     float largest[4];
 };
 
-/// Blocks (row, from), (row, from + 1) .. of K K^T and Q K^T, two tiles of eight tokens each from tile `at` on.
-template <int kDim, int kBlocks>
-__device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, int row, int from, int at, float (&kk)[6][4], float (&qk)[6][4]) {
+/// Blocks (kRow, kFrom), (kRow, kFrom + 1) .. of K K^T and Q K^T, two tiles of eight tokens each from tile kAt on.
+template <int kDim, int kRow, int kFrom, int kBlocks, int kAt>
+__device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, float (&kk)[6][4], float (&qk)[6][4]) {
     constexpr int kChunks = kDim / 8;
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int t = 0; t < 2 * kBlocks; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kk[at + t][j] = qk[at + t][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) kk[kAt + t][j] = qk[kAt + t][j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i) {
         uint32_t x[4], y[4];
-        load_matrices(x, k_at + chunk_at<kChunks>(row * 16 + (lane & 15), 2 * i + (lane >> 4)));
-        load_matrices(y, q_at + chunk_at<kChunks>(row * 16 + (lane & 15), 2 * i + (lane >> 4)));
+        load_matrices(x, k_at + chunk_at<kChunks>(kRow * 16 + (lane & 15), 2 * i + (lane >> 4)));
+        load_matrices(y, q_at + chunk_at<kChunks>(kRow * 16 + (lane & 15), 2 * i + (lane >> 4)));
 #pragma unroll
         for (int t = 0; t < kBlocks; ++t) {
             uint32_t m[4];
-            load_matrices(m, k_at + chunk_at<kChunks>((from + t) * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
-            multiply(kk[at + 2 * t], x, m[0], m[1]);
-            multiply(kk[at + 2 * t + 1], x, m[2], m[3]);
-            multiply(qk[at + 2 * t], y, m[0], m[1]);
-            multiply(qk[at + 2 * t + 1], y, m[2], m[3]);
+            load_matrices(m, k_at + chunk_at<kChunks>((kFrom + t) * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+            multiply(kk[kAt + 2 * t], x, m[0], m[1]);
+            multiply(kk[kAt + 2 * t + 1], x, m[2], m[3]);
+            multiply(qk[kAt + 2 * t], y, m[0], m[1]);
+            multiply(qk[kAt + 2 * t + 1], y, m[2], m[3]);
         }
     }
 }
 /// A (32 bits) and P (fp16) of those blocks.  Below the diagonal block a decay e^(G_i - G_j) is the product of e^(G_i - G_r)
 /// and e^(G_r - G_j), r the last token of j's block: both at most 1, the second one per token.
-template <int kDim, int kBlocks>
-__device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int block_row, int from, int at, const float (&kk)[6][4], const float (&qk)[6][4]) {
+template <int kDim, int kRow, int kFrom, int kBlocks, int kAt>
+__device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, const float (&kk)[6][4], const float (&qk)[6][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int in = g + h * 8, row = block_row * 16 + in;
+        const int in = g + h * 8, row = kRow * 16 + in;
         const float2 sum = room.sums[row];
         const float by = fit2 * room.beta[row];
 #pragma unroll
         for (int u = 0; u < kBlocks; ++u) {
-            const bool below = from + u < block_row;
-            const float2 ref = room.sums[(from + u) * 16 + 15];
+            const bool below = kFrom + u < kRow;
+            const float2 ref = room.sums[(kFrom + u) * 16 + 15];
             const float part = below ? exp2f((sum.x - ref.x) + (sum.y - ref.y)) : 0.0f;
 #pragma unroll
             for (int t = 2 * u; t < 2 * u + 2; ++t) {
-                const int col = from * 16 + t * 8 + 2 * c;
+                const int col = kFrom * 16 + t * 8 + 2 * c;
                 float d0, d1;
                 if (below) {
                     const float2 rest = *reinterpret_cast<const float2*>(&room.rest[col]);
@@ -372,9 +372,9 @@ __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, int
                 }
                 const bool q0 = below || col <= row, q1 = below || col + 1 <= row, k0 = below || col < row, k1 = below || col + 1 < row;
                 *reinterpret_cast<float2*>(&room.work.a[row * kScratch + col]) =
-                    make_float2(k0 ? by * d0 * kk[at + t][2 * h] : 0.0f, k1 ? by * d1 * kk[at + t][2 * h + 1] : 0.0f);
-                *reinterpret_cast<uint32_t*>(room.mix + block_of(block_row, from + u) * kBlockBytes + half_row_at(in, t & 1) + c * 4) =
-                    Pair<__half>::down(q0 ? d0 * qk[at + t][2 * h] : 0.0f, q1 ? d1 * qk[at + t][2 * h + 1] : 0.0f);
+                    make_float2(k0 ? by * d0 * kk[kAt + t][2 * h] : 0.0f, k1 ? by * d1 * kk[kAt + t][2 * h + 1] : 0.0f);
+                *reinterpret_cast<uint32_t*>(room.mix + block_of(kRow, kFrom + u) * kBlockBytes + half_row_at(in, t & 1) + c * 4) =
+                    Pair<__half>::down(q0 ? d0 * qk[kAt + t][2 * h] : 0.0f, q1 ? d1 * qk[kAt + t][2 * h + 1] : 0.0f);
             }
         }
     }
@@ -461,11 +461,12 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
     // ---- K K^T and Q K^T on and below the diagonal: ten blocks of 16 x 16, at most three a warp
     const uint32_t k_at = smem_at(room.in.k), q_at = smem_at(room.in.q);
     float kk[6][4], qk[6][4];
-    if (warp < 2) products<kDim, 2>(k_at, q_at, 3, 2 * warp, 0, kk, qk);   // row 3, two blocks each
-    else if (warp == 2) products<kDim, 3>(k_at, q_at, 2, 0, 0, kk, qk);    // row 2
+    if (warp == 0) products<kDim, 3, 0, 2, 0>(k_at, q_at, kk, qk);
+    else if (warp == 1) products<kDim, 3, 2, 2, 0>(k_at, q_at, kk, qk);
+    else if (warp == 2) products<kDim, 2, 0, 3, 0>(k_at, q_at, kk, qk);
     else {
-        products<kDim, 2>(k_at, q_at, 1, 0, 0, kk, qk);                    // rows 1 and 0
-        products<kDim, 1>(k_at, q_at, 0, 0, 4, kk, qk);
+        products<kDim, 1, 0, 2, 0>(k_at, q_at, kk, qk);
+        products<kDim, 0, 0, 1, 4>(k_at, q_at, kk, qk);
     }
     __syncthreads();   // the scratch matrices lie where K and Q are
 
@@ -513,12 +514,13 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
                 record.f.whole = expf((float) all);
                 record.f.key_down = power_of_two(-key_power);
             }
-            decayed<kDim, 2>(room, fit2, 3, 2 * warp, 0, kk, qk);
+            if (warp == 0) decayed<kDim, 3, 0, 2, 0>(room, fit2, kk, qk);
+            else decayed<kDim, 3, 2, 2, 0>(room, fit2, kk, qk);
         } else if (warp == 2) {
-            decayed<kDim, 3>(room, fit2, 2, 0, 0, kk, qk);
+            decayed<kDim, 2, 0, 3, 0>(room, fit2, kk, qk);
         } else {
-            decayed<kDim, 2>(room, fit2, 1, 0, 0, kk, qk);
-            decayed<kDim, 1>(room, fit2, 0, 0, 4, kk, qk);
+            decayed<kDim, 1, 0, 2, 0>(room, fit2, kk, qk);
+            decayed<kDim, 0, 0, 1, 4>(room, fit2, kk, qk);
         }
         __syncthreads();
         // ---- T = (I + A)^-1: the diagonal blocks of 16 by substitution, a column per thread
@@ -556,10 +558,10 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
             left_parts(&work.a[(at + 16) * kScratch + at], kUnit, ah, al);
             right_parts(&work.t[at * kScratch + at + col], kUnit, bh, bl);
             multiply_parts(c, ah, al, bh, bl);
-            store_product(&work.x[(warp >> 1) * 16 * kScratch + col], kDown, c);
+            store_product(&work.a[(warp >> 1) * 16 * kScratch + 32 + col], kDown, c);
             __syncwarp();
             left_parts(&work.t[(at + 16) * kScratch + at + 16], -kUnit, ah, al);
-            right_parts(&work.x[(warp >> 1) * 16 * kScratch + col], kUnit, bh, bl);
+            right_parts(&work.a[(warp >> 1) * 16 * kScratch + 32 + col], kUnit, bh, bl);
             multiply_parts(d, ah, al, bh, bl);
             store_product(&work.t[(at + 16) * kScratch + at + col], kDown, d);
         }
@@ -577,11 +579,11 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
                 }
             }
 #pragma unroll
-            for (int m = 0; m < 2; ++m) store_product(&work.x[m * 16 * kScratch + col], kDown, c[m]);
+            for (int m = 0; m < 2; ++m) store_product(&work.a[m * 16 * kScratch + 32 + col], kDown, c[m]);
             __syncwarp();
 #pragma unroll
             for (int k16 = 0; k16 < 2; ++k16) {
-                right_parts(&work.x[k16 * 16 * kScratch + col], kUnit, bh, bl);
+                right_parts(&work.a[k16 * 16 * kScratch + 32 + col], kUnit, bh, bl);
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     left_parts(&work.t[(32 + m * 16) * kScratch + 32 + k16 * 16], -kUnit, ah, al);
