@@ -10,6 +10,7 @@
 #include "skv_ops.h"
 
 #include <cmath>
+#include <cstddef>
 #include <string>
 #include <type_traits>
 
@@ -259,8 +260,9 @@ constexpr int kBlockBytes = 512, kTriangleBytes = 10 * kBlockBytes;
 struct Record {
     uint8_t t_high[kTriangleBytes], t_low[kTriangleBytes], mix[kTriangleBytes];
     Factors f;
+    uint8_t mix_low[kTriangleBytes];   // P's second part, for fp16 outputs alone
 };
-static_assert(sizeof(Record) % 16 == 0, "copied 16 bytes at a time");
+static_assert(sizeof(Record) % 16 == 0 && offsetof(Record, mix_low) % 16 == 0, "copied 16 bytes at a time");
 __host__ __device__ constexpr int block_of(int i, int j) { return i * (i + 1) / 2 + j; }
 /// The 16-byte half `chunk` of row `row` of a block, swizzled so that eight rows' equal halves lie in eight bank groups.
 __device__ __forceinline__ uint32_t half_row_at(int row, int chunk) { return (uint32_t) (row * 2 + (chunk ^ ((row >> 2) & 1))) * 16u; }
@@ -308,6 +310,7 @@ struct PrepareRoom {
         struct { float a[kChunk * kScratch], t[kChunk * kScratch]; } work;   // X lies in A's rows 0 - 31, columns 32 - 63, which hold nothing
     };
     alignas(16) uint8_t mix[kTriangleBytes];
+    uint8_t mix_low[kTriangleBytes];
     float2 sums[kChunk];      // G log2 e in two parts
     float rest[kChunk];       // e^(G_r - G), r the last token of the same 16
     double carry[2];          // the first 32 tokens' sum, and all
@@ -343,7 +346,7 @@ __device__ __forceinline__ void products(uint32_t k_at, uint32_t q_at, float (&k
 }
 /// A (32 bits) and P (fp16) of those blocks.  Below the diagonal block a decay e^(G_i - G_j) is the product of e^(G_i - G_r)
 /// and e^(G_r - G_j), r the last token of j's block: both at most 1, the second one per token.
-template <int kDim, int kRow, int kFrom, int kBlocks, int kAt>
+template <int kDim, int kRow, int kFrom, int kBlocks, int kAt, bool kFine>
 __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, const float (&kk)[6][4], const float (&qk)[6][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -373,8 +376,11 @@ __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, con
                 const bool q0 = below || col <= row, q1 = below || col + 1 <= row, k0 = below || col < row, k1 = below || col + 1 < row;
                 *reinterpret_cast<float2*>(&room.work.a[row * kScratch + col]) =
                     make_float2(k0 ? by * d0 * kk[kAt + t][2 * h] : 0.0f, k1 ? by * d1 * kk[kAt + t][2 * h + 1] : 0.0f);
-                *reinterpret_cast<uint32_t*>(room.mix + block_of(kRow, kFrom + u) * kBlockBytes + half_row_at(in, t & 1) + c * 4) =
-                    Pair<__half>::down(q0 ? d0 * qk[kAt + t][2 * h] : 0.0f, q1 ? d1 * qk[kAt + t][2 * h + 1] : 0.0f);
+                uint32_t high, low;
+                split(q0 ? d0 * qk[kAt + t][2 * h] : 0.0f, q1 ? d1 * qk[kAt + t][2 * h + 1] : 0.0f, high, low);
+                const uint32_t to = block_of(kRow, kFrom + u) * kBlockBytes + half_row_at(in, t & 1) + c * 4;
+                *reinterpret_cast<uint32_t*>(room.mix + to) = high;
+                if constexpr (kFine) *reinterpret_cast<uint32_t*>(room.mix_low + to) = low;
             }
         }
     }
@@ -387,6 +393,7 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
     extern __shared__ __align__(128) uint8_t smem[];
     auto& room = *reinterpret_cast<PrepareRoom<kDim>*>(smem);
     constexpr int kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
+    constexpr bool kFine = std::is_same<T, __half>::value;
     const skv_gdn_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int key_head = (int) (blockIdx.x % a.n_k_heads);
@@ -514,13 +521,13 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
                 record.f.whole = expf((float) all);
                 record.f.key_down = power_of_two(-key_power);
             }
-            if (warp == 0) decayed<kDim, 3, 0, 2, 0>(room, fit2, kk, qk);
-            else decayed<kDim, 3, 2, 2, 0>(room, fit2, kk, qk);
+            if (warp == 0) decayed<kDim, 3, 0, 2, 0, kFine>(room, fit2, kk, qk);
+            else decayed<kDim, 3, 2, 2, 0, kFine>(room, fit2, kk, qk);
         } else if (warp == 2) {
-            decayed<kDim, 2, 0, 3, 0>(room, fit2, kk, qk);
+            decayed<kDim, 2, 0, 3, 0, kFine>(room, fit2, kk, qk);
         } else {
-            decayed<kDim, 1, 0, 2, 0>(room, fit2, kk, qk);
-            decayed<kDim, 0, 0, 1, 4>(room, fit2, kk, qk);
+            decayed<kDim, 1, 0, 2, 0, kFine>(room, fit2, kk, qk);
+            decayed<kDim, 0, 0, 1, 4, kFine>(room, fit2, kk, qk);
         }
         __syncthreads();
         // ---- T = (I + A)^-1: the diagonal blocks of 16 by substitution, a column per thread
@@ -609,14 +616,17 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
             *reinterpret_cast<uint4*>(record.t_high + to) = make_uint4(high[0], high[1], high[2], high[3]);
             *reinterpret_cast<uint4*>(record.t_low + to) = make_uint4(low[0], low[1], low[2], low[3]);
             *reinterpret_cast<uint4*>(record.mix + at * 16) = *reinterpret_cast<const uint4*>(room.mix + at * 16);
+            if constexpr (kFine) *reinterpret_cast<uint4*>(record.mix_low + at * 16) = *reinterpret_cast<const uint4*>(room.mix_low + at * 16);
         }
         __syncthreads();   // the next head writes A and P again
     }
 }
 
 /// A chunk CTA: kGroupsOf groups of 16 value columns, the keys of a group split over kSplit state warps, and the outputs of
-/// kTogether groups in one output warp.
-template <int kDim, int kGroupsOf, int kSplit, int kTogether>
+/// kTogether groups in one output warp.  kFine: P and V' enter the output in both of their parts (an fp16 output would
+/// otherwise be off by 1.7 times its own rounding, with them by at most 1.4; for a bfloat16 one the first parts are eight
+/// times finer than that).
+template <int kDim, int kGroupsOf, int kSplit, int kTogether, bool kFine>
 struct ChunkRoom {
     static constexpr int kStates = kGroupsOf * kSplit, kOutputs = kGroupsOf / kTogether;
     static constexpr int kThreadsOf = (kProducers + kStates + kOutputs) * 32;   // loaders, state warps, output warps
@@ -627,15 +637,19 @@ struct ChunkRoom {
         Record record;
     };
     Buffer buffer[2];
-    float4 sums[kSplit == 1 ? 1 : kStates][8][32];   // K S over its part of the keys, which a state warp hands its partner
+    float4 sums[kSplit == 1 ? 1 : kStates][kSplit == 1 ? 1 : 8][kSplit == 1 ? 1 : 32];   // K S over half of the keys, which a state warp hands its partner
     uint4 states[kGroupsOf][kDim / 16][32];       // S as the output takes it: fp16 left operands, 16 keys each
-    uint4 values[2][kGroupsOf][4][32];            // V' as the output takes it, 16 tokens each
-    int state_power[kGroupsOf][kSplit], value_power[2][kGroupsOf];
+    static constexpr int kCopies = kFine && kSplit == 1 ? 1 : 2;   // of V', by chunks: two where they fit
+    uint4 values[kCopies][kGroupsOf][4][32];      // V' as the output takes it, 16 tokens each
+    uint4 values_low[kFine ? kCopies : 1][kFine ? kGroupsOf : 1][kFine ? 4 : 1][kFine ? 32 : 1];   // and its second part
+    static constexpr bool kRest = kFine;
+    int state_power[kGroupsOf][kSplit], value_power[kCopies][kGroupsOf];
 };
 // Barriers.  A buffer is full (loaders arrive, the others wait) and empty again (the other way round); the two of a pair
 // hand over their sums; S is ready for its output warp (which waits), and V' is (all meet: so states are never more
-// than one chunk ahead of their output, whose reads of S are over by then).
-enum : int { kFull = 0, kEmpty = 2, kPair = 4, kStateReady = 8, kValueReady = 12 };
+// than one chunk ahead of their output, whose reads of S are over by then).  Where there is one copy of V', the output has
+// read it (state warps wait before they write the next).
+enum : int { kFull = 0, kEmpty = 2, kPair = 4, kValueFree = 4, kStateReady = 8, kValueReady = 12 };
 
 template <typename T, int kDim, typename Room>
 __device__ __forceinline__ void load_chunks(const DeltaDev& p, Room& room, int begin, int end, int seq, int head, int slice) {
@@ -665,7 +679,7 @@ __device__ __forceinline__ void load_chunks(const DeltaDev& p, Room& room, int b
             const bool on = t0 + r < end;
             copy_async16(smem_at(buf.v) + chunk_at<kValueChunks>(r, chunk), vh + (int64_t) (on ? t0 + r : begin) * a.v_stride + chunk * 8, on);
         }
-        for (int at = tid; at < (int) (sizeof(Record) / 16); at += kProducerThreads)
+        for (int at = tid; at < (int) ((Room::kRest ? sizeof(Record) : offsetof(Record, mix_low)) / 16); at += kProducerThreads)
             copy_async16(smem_at(&buf.record) + at * 16, reinterpret_cast<const uint8_t*>(record) + at * 16, true);
         asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
         if constexpr (!std::is_same<T, __half>::value) {
@@ -808,17 +822,25 @@ __device__ __forceinline__ void advance(Room& room, int begin, int end, int slic
         }
         const int v_unit = r_power - 10;   // V' = 2^v_unit v: T is kInverseScale = 2^10 times itself
         // ---- V' for the output, from one warp of a pair
+        const int copy = Room::kCopies == 1 ? 0 : b;
+        if constexpr (Room::kCopies == 1) {
+            static_assert(kSplit == 1, "the pairs' barriers are free");
+            if (t0 > begin) meet<kMeeting>(kValueFree + output);
+        }
         if (part == 0) {
             const int most = kSplit == 1 ? s_power : max(s_power, room.state_power[group][kSplit - 1]);
             const int o_power = min(max(exponent_of(warp_largest(largest_of(v))) - 14 + v_unit, max(most - 60, -120)), 120);
             const float v_down = power_of_two(v_unit - o_power);
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-                room.values[b][group][t][lane] =
-                    make_uint4(Pair<__half>::down(v[2 * t][0] * v_down, v[2 * t][1] * v_down), Pair<__half>::down(v[2 * t][2] * v_down, v[2 * t][3] * v_down),
-                               Pair<__half>::down(v[2 * t + 1][0] * v_down, v[2 * t + 1][1] * v_down),
-                               Pair<__half>::down(v[2 * t + 1][2] * v_down, v[2 * t + 1][3] * v_down));
-            if (lane == 0) room.value_power[b][group] = o_power;
+            for (int t = 0; t < 4; ++t) {
+                uint32_t high[4], low[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    split(v[2 * t + (j >> 1)][2 * (j & 1)] * v_down, v[2 * t + (j >> 1)][2 * (j & 1) + 1] * v_down, high[j], low[j]);
+                room.values[copy][group][t][lane] = make_uint4(high[0], high[1], high[2], high[3]);
+                if constexpr (Room::kRest) room.values_low[copy][group][t][lane] = make_uint4(low[0], low[1], low[2], low[3]);
+            }
+            if (lane == 0) room.value_power[copy][group] = o_power;
         }
         meet<kMeeting>(kValueReady + output);
         // ---- S <- e^(G_63) S + K^T (e^(G_63 - G) V')
@@ -931,10 +953,11 @@ __device__ __forceinline__ void put_out(const DeltaDev& p, Room& room, int begin
         }
         if constexpr (kSplit == 2) s_power[0] = max(s_power[0], other);
         meet<kMeeting>(kValueReady + output);
+        const int copy = Room::kCopies == 1 ? 0 : b;
         float up[kTogether];
 #pragma unroll
         for (int y = 0; y < kTogether; ++y) {
-            const int o_power = room.value_power[b][output * kTogether + y];
+            const int o_power = room.value_power[copy][output * kTogether + y];
             const float fit = power_of_two(s_power[y] - o_power);
             up[y] = power_of_two(o_power);
 #pragma unroll
@@ -948,22 +971,41 @@ __device__ __forceinline__ void put_out(const DeltaDev& p, Room& room, int begin
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t high[kTogether][4];
+            uint32_t high[kTogether][4], low[kTogether][4];
 #pragma unroll
             for (int y = 0; y < kTogether; ++y) {
-                const uint4 x = room.values[b][output * kTogether + y][i][lane];
+                const uint4 x = room.values[copy][output * kTogether + y][i][lane];
                 high[y][0] = x.x; high[y][1] = x.y; high[y][2] = x.z; high[y][3] = x.w;
+                if constexpr (Room::kRest) {
+                    const uint4 z = room.values_low[copy][output * kTogether + y][i][lane];
+                    low[y][0] = z.x; low[y][1] = z.y; low[y][2] = z.z; low[y][3] = z.w;
+                }
             }
 #pragma unroll
             for (int t = i; t < 4; ++t) {
                 uint32_t m[4];
-                peek_matrices(m, smem_at(buf.record.mix) + block_of(t, i) * kBlockBytes + half_row_at(right_row(), right_half()));
+                const uint32_t at = block_of(t, i) * kBlockBytes + half_row_at(right_row(), right_half());
+                peek_matrices(m, smem_at(buf.record.mix) + at);
 #pragma unroll
                 for (int y = 0; y < kTogether; ++y) {
                     multiply(o[y][2 * t], high[y], m[0], m[1]);
                     multiply(o[y][2 * t + 1], high[y], m[2], m[3]);
                 }
+                if constexpr (Room::kRest) {
+                    uint32_t n[4];
+                    peek_matrices(n, smem_at(buf.record.mix_low) + at);
+#pragma unroll
+                    for (int y = 0; y < kTogether; ++y) {
+                        multiply(o[y][2 * t], low[y], m[0], m[1]);
+                        multiply(o[y][2 * t + 1], low[y], m[2], m[3]);
+                        multiply(o[y][2 * t], high[y], n[0], n[1]);
+                        multiply(o[y][2 * t + 1], high[y], n[2], n[3]);
+                    }
+                }
             }
+        }
+        if constexpr (Room::kCopies == 1) {
+            if (t0 + kChunk < end) pass<kMeeting>(kValueFree + output);
         }
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
@@ -988,8 +1030,8 @@ constexpr int kLoaderRegisters = 48, kStateRegisters = 176, kOutputRegisters = 1
 static_assert(kLoaderRegisters * 128 + kStateRegisters * 256 + kOutputRegisters * 128 == 128 * 512, "the shares of 512 threads launched with 128 each");
 
 template <typename T, int kDim, int kGroupsOf, int kSplit, int kTogether>
-__global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf, kSplit, kTogether>::kThreadsOf, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
-    using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether>;
+__global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, std::is_same<T, __half>::value>::kThreadsOf, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
+    using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, std::is_same<T, __half>::value>;
     extern __shared__ __align__(128) uint8_t smem[];
     auto& room = *reinterpret_cast<Room*>(smem);
     constexpr bool kShares = Room::kThreadsOf == 512;
@@ -1024,7 +1066,7 @@ cudaError_t launch_tokens(const DeltaDev& p, cudaStream_t stream) {
 
 template <typename T, int kDim, int kGroupsOf, int kSplit, int kTogether>
 cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
-    using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether>;
+    using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, std::is_same<T, __half>::value>;
     constexpr auto kKernel = chunk_kernel<T, kDim, kGroupsOf, kSplit, kTogether>;
     constexpr int kSmem = sizeof(Room), kPrepare = sizeof(PrepareRoom<kDim>);
     static_assert(kSmem <= 227 * 1024, "the buffers fit an SM");
