@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
             }
         }
     };
+    wait_for_previous();
     fetch(lo);   // on their way while the angles are worked out
 
     if (blockIdx.y == 0 && a.lengths_out) {
@@ -251,15 +252,13 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 }
 
 template <typename T, int kDim>
-void launch(const AppendDev& p, dim3 grid, bool int8, cudaStream_t stream) {
-    if (int8) append_kernel<T, kDim, true><<<grid, kThreads, 0, stream>>>(p);
-    else append_kernel<T, kDim, false><<<grid, kThreads, 0, stream>>>(p);
+cudaError_t launch(const AppendDev& p, dim3 grid, bool int8, cudaStream_t stream) {
+    return int8 ? launch_early(append_kernel<T, kDim, true>, grid, kThreads, 0, stream, p)
+                : launch_early(append_kernel<T, kDim, false>, grid, kThreads, 0, stream, p);
 }
 template <typename T>
-void launch(const AppendDev& p, int dim, dim3 grid, bool int8, cudaStream_t stream) {
-    if (dim == 64) launch<T, 64>(p, grid, int8, stream);
-    else if (dim == 128) launch<T, 128>(p, grid, int8, stream);
-    else launch<T, 256>(p, grid, int8, stream);
+cudaError_t launch(const AppendDev& p, int dim, dim3 grid, bool int8, cudaStream_t stream) {
+    return dim == 64 ? launch<T, 64>(p, grid, int8, stream) : dim == 128 ? launch<T, 128>(p, grid, int8, stream) : launch<T, 256>(p, grid, int8, stream);
 }
 
 }  // namespace
@@ -314,8 +313,8 @@ extern "C" int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* a
     p.per_row = 1.0f / (float) (rows / kTokens > 0 ? rows / kTokens : 1);
     const dim3 grid((unsigned) blocks, (unsigned) ((rows + p.share - 1) / p.share));
     const auto s = static_cast<cudaStream_t>(stream);
-    if (a.dtype == SKV_DTYPE_F16) launch<__half>(p, layer->head_dim, grid, layer->format == SKV_KV_INT8, s);
-    else launch<__nv_bfloat16>(p, layer->head_dim, grid, layer->format == SKV_KV_INT8, s);
-    const cudaError_t e = cudaGetLastError();
+    const bool int8 = layer->format == SKV_KV_INT8;
+    const cudaError_t e = a.dtype == SKV_DTYPE_F16 ? launch<__half>(p, layer->head_dim, grid, int8, s)
+                                                   : launch<__nv_bfloat16>(p, layer->head_dim, grid, int8, s);
     return e == cudaSuccess ? SKV_OK : cuda_fail(e, "skv_kv_append");
 }

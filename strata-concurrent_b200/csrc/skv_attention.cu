@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
     const int items = p.layer.n_head_kv * p.blocks, n_seqs = p.a.n_seqs;
     const skv_attention_args& a = p.a;
 
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // of whatever wrote the cache, the lengths and the queries
+    wait_for_previous();
     // ---- the share: tiles [from, to) of all.  The tiles of sequences 0 .. s, a thread per sequence, in trips
     const auto tiles_of = [&](int s) { return s < n_seqs ? (cells_of(p, s) + G::kTile - 1) / G::kTile * items : 0; };
     int64_t total = 0, end = 0, n = 0;   // of the trip's sequence: the tiles up to its end, and its own
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) join_kernel(const __grid_cons
     __shared__ float s_top[kJoinWarps], s_sum[kJoinWarps];
     __shared__ float4 s_out[kJoinThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = min(p.group, kRows), items = p.layer.n_head_kv * p.blocks;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_previous();
     // the cut items, in order
     int2 cut[kTrips];
     uint32_t mask[kTrips];
@@ -801,24 +801,10 @@ cudaError_t launch(const AttnDev& p, int sms, cudaStream_t stream) {
     const int ctas = sms * kPerSm;
     cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kDim, kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    // Each kernel may be launched while the one before it ends, and waits for it before its first read: 11.5 us a call
-    // instead of 14.4 for 1,000 cells.  (Letting the join in any earlier, while shares still run, costs 2 us.)
-    cudaLaunchConfig_t config{};
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    config.stream = stream;
-    config.gridDim = dim3((unsigned) ctas);
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kSmem;
-    e = cudaLaunchKernelEx(&config, attention_kernel<T, kDim, kInt8>, p);
+    // (Letting the join in any earlier, while shares still run, costs 2 us a call.)
+    e = launch_early(attention_kernel<T, kDim, kInt8>, dim3((unsigned) ctas), kThreads, kSmem, stream, p);
     if (e != cudaSuccess) return e;
-    config.gridDim = dim3((unsigned) sms * 8);
-    config.blockDim = dim3(kJoinThreads);
-    config.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&config, join_kernel<T, kDim>, p, ctas);
+    return launch_early(join_kernel<T, kDim>, dim3((unsigned) sms * 8), kJoinThreads, 0, stream, p, ctas);
 }
 template <typename T>
 cudaError_t launch(const AttnDev& p, int dim, bool int8, int sms, cudaStream_t stream) {
