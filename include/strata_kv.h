@@ -260,7 +260,8 @@ SKV_API int skv_slice_segments(const skv_segment* segs, int n_segs, uint64_t lo,
  * device, allocate nothing and can be captured into a CUDA graph (after one call outside of capture has set up the
  * device).  Activations are fp16 or bf16 (`dtype`); sums, softmax statistics, states and angles are held in 32 bits or
  * more.  Row pointers are 16-byte aligned and strides (in elements, between tokens) multiples of 8; the heads of one
- * token lie back to back.  An output may not overlap an input unless an argument says so. */
+ * token lie back to back.  An output may not overlap an input unless an argument says so.  Everything they are given lies
+ * in the current device's own memory; a pool or a state elsewhere is refused (SKV_EINVAL). */
 #define SKV_DTYPE_F16 0
 #define SKV_DTYPE_BF16 1
 
@@ -296,8 +297,8 @@ typedef struct skv_kv_layer {
 /* skv_kv_append - write the K and V of new tokens into their cells, with the rotary positions applied to K on the way.
  *
  * Rows [seq_starts[s], seq_starts[s+1]) of k and v belong to sequence s and go to its cells lengths[s], lengths[s]+1, ...
- * (seq_starts null: one row per sequence).  Rows before the first or behind the last sequence are neither read nor
- * written.  A cell is rotated by its own number: pair j turns by cell * inv_freq[j], the product taken in 64 bits, and
+ * (seq_starts null: one row per sequence).  Rows before the first or behind the last sequence are padding: nothing comes
+ * of them, and q_out keeps what it held there.  A cell is rotated by its own number: pair j turns by cell * inv_freq[j], the product taken in 64 bits, and
  * is scaled by rope_scale.  SKV_ROPE_HALF pairs value j with j + n_rot/2, SKV_ROPE_PAIRS value 2j with 2j+1; values
  * from n_rot on pass through; n_rot 0 (inv_freq null) rotates nothing.  q, when given, is rotated the same way into
  * q_out, which may be q itself.  int8: scale = fp16(max |x| / 127) per 64 values, code = x / scale rounded to nearest
@@ -361,9 +362,11 @@ SKV_API int skv_decode_attention_workspace(const skv_kv_layer* layer, int n_seqs
  * with the fp32 state row of each sequence read before its first token and written after its last.  Row r of the
  * state is [n_v_heads][head_dim key][head_dim value] floats at state + r * state_stride; sequence s uses row
  * state_index[s] (null: s).  Each row at most once per call.  Value head h uses key head h / (n_v_heads / n_k_heads).
- * g is the logarithm of the decay (<= 0; -inf forgets everything), beta the write strength, k of about unit length.
- * seq_starts as in skv_kv_append; max_tokens bounds the tokens of one sequence (a longer one is cut there).  Few tokens
- * a sequence run token by token, long ones in chunks through the tensor cores; both hold S in 32 bits.
+ * g is the logarithm of the decay (<= 0; -inf forgets everything), beta the write strength; beta |k|^2 is at most 2, as
+ * for keys of unit length, and keys of one sequence are within a factor of 100 of each other in length.
+ * seq_starts as in skv_kv_append; max_tokens bounds the tokens of one sequence (a longer one is cut there).  Calls of
+ * few tokens a sequence (max_tokens below 16, or seq_starts null) run token by token, the others in chunks of 64 through the
+ * tensor cores; both hold S in 32 bits.
  * workspace: skv_gated_delta_workspace bytes of device memory, 256-byte aligned; as for skv_decode_attention. */
 typedef struct skv_gdn_args {
     const void* q;               /* [n_tokens][n_k_heads][head_dim] */

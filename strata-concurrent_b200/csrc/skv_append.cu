@@ -304,7 +304,7 @@ extern "C" int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* a
     p.a = a;
     p.status = ctx->status;
     // Few tokens: spread each CTA's rows over more CTAs, down to one trip each, until the GPU has two per SM.
-    const int blocks = (a.n_tokens + kTokens - 1) / kTokens > 0 ? (a.n_tokens + kTokens - 1) / kTokens : 1;
+    const int blocks = a.n_tokens ? (a.n_tokens - 1) / kTokens + 1 : 1;
     const int rows = ((a.q ? a.n_head : 0) + 2 * layer->n_head_kv) * kTokens, trip = kThreads * 8 / layer->head_dim;
     int split = (2 * ctx->sms + blocks - 1) / blocks;
     const int trips = (rows + trip - 1) / trip;

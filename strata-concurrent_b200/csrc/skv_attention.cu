@@ -166,12 +166,18 @@ __device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t& before, int64_t*
     return v;
 }
 
+/// a / b of non-negative numbers, in 32 bits where they fit.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return ((a | b) >> 31) == 0 ? (int64_t) ((uint32_t) a / (uint32_t) b) : a / b;
+}
+
 /// A place in the sequence of all tiles.
 struct Cursor {
     int seq, item;        // item: the K/V head and block of heads within the sequence
     int tile, tiles;      // of the sequence
     int64_t cells;
 };
+__device__ __forceinline__ int kv_of(const Cursor& c, const AttnDev& p) { return c.item / p.blocks; }
 template <int kTile>
 __device__ __forceinline__ void step(Cursor& c, const AttnDev& p, int items) {
     if (++c.tile < c.tiles) return;
@@ -195,12 +201,13 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
     __shared__ alignas(16) int s_power[kWarps][4];   // int8: per V scale group
     __shared__ int64_t s_scan[kWarps];
     __shared__ int64_t s_first[2];   // the first sequence of the share, and the tiles before it
+    __shared__ int64_t s_share[3];   // for the end: the share's first tile, all tiles, all shares
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int items = p.layer.n_head_kv * p.blocks, n_seqs = p.a.n_seqs;
     const skv_attention_args& a = p.a;
 
     wait_for_previous();
-    // ---- the share: tiles [from, to) of all.  The tiles of sequences 0 .. s, a thread per sequence, in trips
+    // ---- the share: `count` tiles from `from` on, of all.  The tiles of sequences 0 .. s, a thread per sequence, in trips
     const auto tiles_of = [&](int s) { return s < n_seqs ? (cells_of(p, s) + G::kTile - 1) / G::kTile * items : 0; };
     int64_t total = 0, end = 0, n = 0;   // of the trip's sequence: the tiles up to its end, and its own
     for (int base = 0; base < n_seqs; base += kThreads) {
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         if (tid == 0) p.cut[blockIdx.x] = make_int2(-1, 0);
         return;
     }
-    const int64_t from = total * blockIdx.x / shares, to = total * (blockIdx.x + 1) / shares;
+    const int64_t from = quotient(total * blockIdx.x, shares), count = quotient(total * (blockIdx.x + 1), shares) - from;
     if (n_seqs <= kThreads) {   // the one trip is still at hand
         if (n && from >= end - n && from < end) {
             s_first[0] = tid;
@@ -241,14 +248,18 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
             meet();
         }
     }
+    if (tid == 0) {
+        s_share[0] = from;
+        s_share[1] = total;
+        s_share[2] = shares;
+    }
     Cursor load;
     load.seq = (int) s_first[0];
     load.cells = cells_of(p, load.seq);
     load.tiles = (int) ((load.cells + G::kTile - 1) / G::kTile);
-    load.item = (int) ((from - s_first[1]) / load.tiles);
-    load.tile = (int) ((from - s_first[1]) % load.tiles);
+    load.item = (int) quotient(from - s_first[1], load.tiles);
+    load.tile = (int) (from - s_first[1] - (int64_t) load.item * load.tiles);
     Cursor here = load;
-    const int64_t count = to - from;
 
     // ---- loading.  Lane i of a warp knows the warp's cell i; its table entry is read a tile before its copies are issued.
     // A warp alone reads the K it copied, so the next tile's K follows as soon as it has its scores; V has two slots, and
@@ -259,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         const int64_t cell = (int64_t) load.tile * G::kTile + warp * G::kCells + lane;
         within = -1;
         if (lane < G::kCells && cell < load.cells) {
-            within = ((load.item / p.blocks) << p.layer.page_shift) + (int) (cell & ((1 << p.layer.page_shift) - 1));
+            within = (kv_of(load, p) << p.layer.page_shift) + (int) (cell & ((1 << p.layer.page_shift) - 1));
             entry = __ldg(p.layer.tables + (int64_t) load.seq * p.layer.table_stride + (cell >> p.layer.page_shift));
         }
     };
@@ -319,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         return top > 0.0f && top < INFINITY ? min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -126), 126) : 0;
     };
     auto load_query = [&]() {
-        const int kv = here.item / p.blocks, first = (here.item % p.blocks) * kRows;
+        const int kv = kv_of(here, p), first = (here.item - kv * p.blocks) * kRows;
         if constexpr (kInt8) {
             // eight lanes a row; of each 16 values 4c, 4c+1 go to places 2c, 2c+1 and 4c+2, 4c+3 to 2c+8, 2c+9, so that
             // the operand's columns meet K's as a register of four codes holds them
@@ -627,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
             meet();
             const bool whole = first_tile == 0 && here.tile + 1 == here.tiles;
             const int slot = first_tile == 0 ? 1 : 0;
-            const int kv = here.item / p.blocks, first = (here.item % p.blocks) * kRows;
+            const int kv = kv_of(here, p), first = (here.item - kv * p.blocks) * kRows;
             float fit = 1.0f / 32768.0f;
             if constexpr (kInt8) {
 #pragma unroll
@@ -666,8 +677,8 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
                 }
             }
             if (tid == 0 && n + 1 == count) {
-                const int64_t last = from + n + (here.tiles - 1 - here.tile);   // the item's last tile, and the share that has it
-                const int64_t holder = ((last + 1) * shares - 1) / total;
+                const int64_t last = s_share[0] + n + (here.tiles - 1 - here.tile);   // the item's last tile, and the share that has it
+                const int64_t holder = quotient((last + 1) * s_share[2] - 1, s_share[1]);
                 p.cut[blockIdx.x] = !whole && slot == 1 ? make_int2(here.seq * items + here.item, (int) (holder - blockIdx.x) + 1) : make_int2(-1, 0);
             }
             if (n + 1 < count) {

@@ -167,7 +167,10 @@ constexpr int kChunk = 64;
 constexpr int kProducers = 4;
 constexpr int kProducerThreads = kProducers * 32;
 constexpr int kScratch = 68;          // floats between rows of the 32-bit scratch matrices
-constexpr float kInverseScale = 1024.0f;   // T's entries are at most about 1: their fp16 parts keep clear of subnormals
+// T's entries are about 1 at most for keys of about unit length: 2^5 of them leaves their two fp16 parts 30 bits below 1,
+// and room for entries of 2,000 where keys differ in length.
+constexpr int kInversePower = 5;
+constexpr float kInverseScale = 1 << kInversePower;
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool on) {   // off: zeros, nothing is read
@@ -824,7 +827,7 @@ __device__ __forceinline__ void advance(Room& room, int begin, int end, int slic
                 multiply(v[2 * t + 1], high, m[t][2], m[t][3]);
             }
         }
-        const int v_unit = r_power - 10;   // V' = 2^v_unit v: T is kInverseScale = 2^10 times itself
+        const int v_unit = r_power - kInversePower;   // V' = 2^v_unit v
         // ---- V' for the output, from one warp of a pair
         const int copy = Room::kCopies == 1 ? 0 : b;
         if constexpr (Room::kCopies == 1) {

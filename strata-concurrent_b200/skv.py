@@ -617,9 +617,9 @@ def _dtype(x) -> tuple:
     return got
 
 
-def _rows(x, what: str, kind=None) -> tuple:
-    """(address, rows, heads, values, elements between rows) of a [row][head][value] tensor of dtype `kind` (None: a
-    float16 or bfloat16 one) whose heads lie back to back."""
+def _rows(x, what: str, device: int, kind=None) -> tuple:
+    """(address, rows, heads, values, elements between rows) of a [row][head][value] tensor on GPU `device`, of dtype `kind`
+    (None: a float16 or bfloat16 one), whose heads lie back to back."""
     n, heads, dim = x.shape
     if x.is_contiguous():
         step = heads * dim
@@ -631,19 +631,28 @@ def _rows(x, what: str, kind=None) -> tuple:
             step = heads * dim
     if (x.dtype is not kind) if kind is not None else _dtype(x)[1] is None:
         raise TypeError(f"{what}: {x.dtype} (all of a call's activations are float16, or all bfloat16)")
-    if not x.is_cuda:
-        raise ValueError(f"{what}: not on a GPU")
+    if x.get_device() != device or device < 0:
+        raise ValueError(f"{what}: not on the GPU of the others")
     return x.data_ptr(), n, heads, dim, step
 
 
-def _vector(x, what: str, name: str, at_least: int) -> int:
-    """The address of a contiguous 1-d device tensor of at least so many `name` values."""
+def _vector(x, what: str, device: int, name: str, at_least: int) -> int:
+    """The address of a contiguous 1-d tensor of at least so many `name` values on GPU `device`."""
     got = _KNOWN.get(x.dtype) or _dtype(x)
-    if got[0] != name or x.dim() != 1 or not x.is_cuda or not x.is_contiguous():
-        raise TypeError(f"{what}: a contiguous 1-d {name} tensor on the GPU")
+    if got[0] != name or x.dim() != 1 or x.get_device() != device or not x.is_contiguous():
+        raise TypeError(f"{what}: a contiguous 1-d {name} tensor on the GPU of the others")
     if x.shape[0] < at_least:
         raise ValueError(f"{what}: {x.shape[0]} entries, {at_least} needed")
     return x.data_ptr()
+
+
+def _room(x, device: int) -> tuple:
+    """(address, bytes) of a workspace; of none, nothing."""
+    if x is None:
+        return 0, 0
+    if x.get_device() != device or not x.is_contiguous():
+        raise TypeError("workspace: a contiguous tensor on the GPU of the others")
+    return x.data_ptr(), x.nbytes
 
 
 class KvLayer:
@@ -662,13 +671,14 @@ class KvLayer:
         for x in scales:
             if _dtype(x)[0] != "torch.float16" or tuple(x.shape) != (pages, n_head_kv, page_size, head_dim // 64):
                 raise TypeError("KvLayer: scales are float16, [page][kv_head][cell][head_dim / 64]")
+        self.device = k_pool.get_device()
         for x in (k_pool, v_pool, *scales):
-            if not x.is_contiguous() or not x.is_cuda:
-                raise ValueError("KvLayer: pools and scales must be contiguous and on the GPU")
+            if not x.is_contiguous() or x.get_device() != self.device or self.device < 0:
+                raise ValueError("KvLayer: pools and scales must be contiguous and on the GPU, all on one")
         self._init(k_pool, v_pool, k_scale, v_scale, page_tables, pages, n_head_kv, head_dim, page_size, fmt)
 
     def _init(self, k, v, k_scale, v_scale, tables, limit, n_head_kv, head_dim, page_size, fmt):
-        if _dtype(tables)[0] != "torch.int32" or tables.dim() != 2 or not tables.is_cuda or (tables.shape[1] > 1 and tables.stride(1) != 1):
+        if _dtype(tables)[0] != "torch.int32" or tables.dim() != 2 or tables.get_device() != self.device or (tables.shape[1] > 1 and tables.stride(1) != 1):
             raise TypeError("KvLayer: page tables are int32, [sequence][page], on the GPU, the pages of a row contiguous")
         n_tables, width = tables.shape
         step = tables.stride(0) if n_tables > 1 else width
@@ -686,6 +696,7 @@ class KvLayer:
         of a slot lies pages_per_block pages behind its K page."""
         self = cls.__new__(cls)
         shift = g.pages_per_block
+        self.device = pool.device
         self._init(pool.base, pool.base + shift * g.page_bytes, None, None, page_tables,
                    pool.n_blocks * g.slot_pages - shift, g.n_head_kv, g.head_dim, PAGE_CELLS, KV_F16)
         self.pool = pool
@@ -696,9 +707,10 @@ def kv_append(layer: KvLayer, k, v, lengths, *, seq_starts=None, q=None, q_out=N
               rope_style: str = "half", rope_scale: float = 1.0, lengths_out=None, stream=None) -> None:
     """Write the K and V rows of new tokens ([token][kv_head][head_dim]) into cells lengths[s], lengths[s]+1, ... of
     their sequences, K rotated by its cell's number, and q rotated into q_out (skv_kv_append)."""
-    kp, n, kv, dim, ks = _rows(k, "k")
+    dev = layer.device
+    kp, n, kv, dim, ks = _rows(k, "k", dev)
     kind = k.dtype
-    vp, vn, vkv, vdim, vs = _rows(v, "v", kind)
+    vp, vn, vkv, vdim, vs = _rows(v, "v", dev, kind)
     if vn != n or vkv != kv or vdim != dim or kv != layer.n_head_kv or dim != layer.head_dim:
         raise ValueError("kv_append: k and v are [token][kv_head][head_dim] of the layer")
     n_seqs = n if seq_starts is None else seq_starts.shape[0] - 1
@@ -706,17 +718,17 @@ def kv_append(layer: KvLayer, k, v, lengths, *, seq_starts=None, q=None, q_out=N
     if (q is None) != (q_out is None):
         raise ValueError("kv_append: q and q_out come together")
     if q is not None:
-        qp, qn, heads, qd, qs = _rows(q, "q", kind)
-        qo, on, oh, od, qos = _rows(q_out, "q_out", kind)
+        qp, qn, heads, qd, qs = _rows(q, "q", dev, kind)
+        qo, on, oh, od, qos = _rows(q_out, "q_out", dev, kind)
         if qn != n or qd != dim or on != n or oh != heads or od != dim:
             raise ValueError("kv_append: q and q_out are [token][head][head_dim]")
     if inv_freq is not None:
         rot = 2 * inv_freq.shape[0]
     args = _APPEND.pack(kp, vp, ks, vs, qp, qo, qs, qos,
-                        0 if seq_starts is None else _vector(seq_starts, "seq_starts", "torch.int32", 1),
-                        _vector(lengths, "lengths", "torch.int32", n_seqs),
-                        0 if lengths_out is None else _vector(lengths_out, "lengths_out", "torch.int32", n_seqs),
-                        0 if inv_freq is None else _vector(inv_freq, "inv_freq", "torch.float32", 0),
+                        0 if seq_starts is None else _vector(seq_starts, "seq_starts", dev, "torch.int32", 1),
+                        _vector(lengths, "lengths", dev, "torch.int32", n_seqs),
+                        0 if lengths_out is None else _vector(lengths_out, "lengths_out", dev, "torch.int32", n_seqs),
+                        0 if inv_freq is None else _vector(inv_freq, "inv_freq", dev, "torch.float32", 0),
                         n, n_seqs, heads, rot, ROPE_STYLES[rope_style], _dtype(k)[1], rope_scale, 0)
     check(lib().skv_kv_append(layer.at, args, _stream(stream)))
 
@@ -731,16 +743,17 @@ def decode_attention_workspace(layer: KvLayer, n_seqs: int, n_head: int) -> int:
 def decode_attention(layer: KvLayer, q, lengths, out, *, workspace, scale: float | None = None, lse=None, stream=None) -> None:
     """out = softmax(scale * q K^T) V of one new token per sequence ([sequence][head][head_dim]) over the first
     lengths[s] cells of its cache (skv_decode_attention).  scale: head_dim ** -0.5 when None."""
-    qp, n, heads, dim, qs = _rows(q, "q")
-    op, on, oh, od, os_ = _rows(out, "out", q.dtype)
+    dev = layer.device
+    qp, n, heads, dim, qs = _rows(q, "q", dev)
+    op, on, oh, od, os_ = _rows(out, "out", dev, q.dtype)
     if on != n or oh != heads or od != dim or dim != layer.head_dim:
         raise ValueError("decode_attention: q and out are [sequence][head][head_dim] of the layer")
     lp = 0
     if lse is not None:
-        if _dtype(lse)[0] != "torch.float32" or lse.shape != (n, heads) or not lse.is_contiguous() or not lse.is_cuda:
+        if _dtype(lse)[0] != "torch.float32" or lse.shape != (n, heads) or not lse.is_contiguous() or lse.get_device() != dev:
             raise TypeError("decode_attention: lse is a contiguous float32 [sequence][head] tensor on the GPU")
         lp = lse.data_ptr()
-    args = _ATTENTION.pack(qp, op, qs, os_, lp, _vector(lengths, "lengths", "torch.int32", n), workspace.data_ptr(), workspace.nbytes,
+    args = _ATTENTION.pack(qp, op, qs, os_, lp, _vector(lengths, "lengths", dev, "torch.int32", n), *_room(workspace, dev),
                            n, heads, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
     check(lib().skv_decode_attention(layer.at, args, _stream(stream)))
 
@@ -757,16 +770,17 @@ def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=No
     """The gated delta rule over packed sequences (skv_gated_delta): q, k [token][k_head][dim], v, out
     [token][v_head][dim], g, beta float32 [token][v_head], state float32 [row][v_head][dim key][dim value], updated in
     place.  max_tokens bounds the tokens of one sequence (all of them when None).  scale: dim ** -0.5 when None."""
-    qp, n, kh, dim, qs = _rows(q, "q")
+    dev = q.get_device()
+    qp, n, kh, dim, qs = _rows(q, "q", dev)
     kind = q.dtype
-    kp, kn, kkh, kd, ks = _rows(k, "k", kind)
-    vp, vn, vh, vd, vs = _rows(v, "v", kind)
-    op, on, oh, od, os_ = _rows(out, "out", kind)
+    kp, kn, kkh, kd, ks = _rows(k, "k", dev, kind)
+    vp, vn, vh, vd, vs = _rows(v, "v", dev, kind)
+    op, on, oh, od, os_ = _rows(out, "out", dev, kind)
     if kn != n or kkh != kh or kd != dim or vn != n or vd != dim or on != n or oh != vh or od != dim:
         raise ValueError("gated_delta: q and k are [token][k_head][dim], v and out [token][v_head][dim]")
     steps = []
     for x, what in ((g, "g"), (beta, "beta")):
-        if _dtype(x)[0] != "torch.float32" or x.shape != (n, vh) or not x.is_cuda:
+        if _dtype(x)[0] != "torch.float32" or x.shape != (n, vh) or x.get_device() != dev:
             raise TypeError(f"gated_delta: {what} is a float32 [token][v_head] tensor on the GPU")
         if x.is_contiguous():
             steps.append(vh)
@@ -776,7 +790,7 @@ def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=No
                 raise ValueError(f"gated_delta: the heads of {what} must lie back to back")
             steps.append(step if n > 1 else vh)
     rows = state.shape[0]
-    if _dtype(state)[0] != "torch.float32" or state.shape[1:] != (vh, dim, dim) or not state.is_cuda:
+    if _dtype(state)[0] != "torch.float32" or state.shape[1:] != (vh, dim, dim) or state.get_device() != dev:
         raise TypeError("gated_delta: state is float32 [row][v_head][dim][dim] on the GPU")
     if state.is_contiguous():
         row = vh * dim * dim
@@ -788,8 +802,8 @@ def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=No
     if max_tokens is None:
         max_tokens = 1 if seq_starts is None else n
     args = _DELTA.pack(qp, kp, vp, op, qs, ks, vs, os_, g.data_ptr(), beta.data_ptr(), steps[0], steps[1], state.data_ptr(), row, rows,
-                       0 if state_index is None else _vector(state_index, "state_index", "torch.int32", n_seqs),
-                       0 if seq_starts is None else _vector(seq_starts, "seq_starts", "torch.int32", 1),
-                       0 if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes, n, n_seqs,
+                       0 if state_index is None else _vector(state_index, "state_index", dev, "torch.int32", n_seqs),
+                       0 if seq_starts is None else _vector(seq_starts, "seq_starts", dev, "torch.int32", 1),
+                       *_room(workspace, dev), n, n_seqs,
                        kh, vh, dim, max_tokens, _dtype(q)[1], dim ** -0.5 if scale is None else scale)
     check(lib().skv_gated_delta(args, _stream(stream)))

@@ -124,13 +124,19 @@ def test_the_binding_refuses_tensors_that_do_not_fit():
     with pytest.raises(ValueError, match="scales"):
         skv.KvLayer(pool.to(torch.int8), pool.to(torch.int8), table)
     x = torch.zeros(1, 2, 256, dtype=torch.float16)
-    with pytest.raises(ValueError, match="not on a GPU"):
-        skv._rows(x, "q")
+    with pytest.raises(ValueError, match="not on the GPU"):
+        skv._rows(x, "q", 0)
+    with pytest.raises(ValueError, match="not on the GPU"):
+        skv._rows(x, "q", -1)          # a layer's or a first tensor's own place, when that is no GPU
     with pytest.raises(TypeError, match="float16"):
-        skv._rows(x.float(), "q")
+        skv._rows(x.float(), "q", 0)
     with pytest.raises(TypeError, match="all"):
-        skv._rows(x, "q", torch.bfloat16)
+        skv._rows(x, "q", 0, torch.bfloat16)
     with pytest.raises(ValueError, match="back to back"):
-        skv._rows(x.transpose(1, 2), "q")
+        skv._rows(x.transpose(1, 2), "q", 0)
     with pytest.raises(TypeError, match="int32"):
-        skv._vector(torch.zeros(3), "lengths", "torch.int32", 3)
+        skv._vector(torch.zeros(3), "lengths", 0, "torch.int32", 3)
+    with pytest.raises(TypeError, match="workspace"):
+        skv._room(torch.zeros(3), 0)
+    with pytest.raises(ValueError, match="not on the GPU"):
+        skv.gated_delta(x, x, x, torch.zeros(1, 2), torch.zeros(1, 2), torch.zeros(1, 2, 256, 256), x)

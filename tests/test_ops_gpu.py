@@ -179,6 +179,32 @@ def test_append_refuses_cells_on_the_device_and_writes_the_others(torch_cuda):
     assert after.tolist() == [1, 2, lengths[2] + 1, 1, 3]
 
 
+def test_append_of_nothing(torch_cuda):
+    """No rows at all: the lengths still come out."""
+    torch = torch_cuda
+    layer = make_layer(torch, 2, [4, 9, 1])
+    before = [x.clone() for x in layer.tensors[:2]]
+    none, after = torch.empty(0, 2, 256, dtype=torch.float16, device="cuda"), ints(torch, [-1] * 3)
+    skv.kv_append(layer, none, none, ints(torch, [4, 0, 7]), seq_starts=ints(torch, [0, 0, 0, 0]), lengths_out=after)
+    assert status(torch) == 0 and after.tolist() == [4, 0, 7]
+    assert torch.equal(layer.tensors[0], before[0]) and torch.equal(layer.tensors[1], before[1])
+
+
+def test_memory_of_another_place_is_refused(torch_cuda):
+    """A pool or a state in pinned host memory never reaches a kernel."""
+    torch = torch_cuda
+    layer = make_layer(torch, 2, [4])
+    x = normal(torch, 1, 1, 2, 256, dtype=torch.float16)
+    host = torch.zeros(layer.tensors[0].shape, dtype=torch.float16).pin_memory()
+    layer.args.k_pool = host.data_ptr()
+    with pytest.raises(skv.SkvError, match="current device"):
+        skv.kv_append(layer, x, x, ints(torch, [0]))
+    q = normal(torch, 1, 1, 24, 256, dtype=torch.float16)
+    with pytest.raises(skv.SkvError, match="current device"):
+        run_attention(torch, layer, q, [4], 0.0625)
+    assert (host == 0).all()
+
+
 def test_append_int8_edges(torch_cuda):
     """Zeros, one huge group, infinities and NaN: the other groups of the row are as without them."""
     torch = torch_cuda
@@ -447,6 +473,42 @@ def test_delta_fills_the_gpu(torch_cuda, kind, kh, vh, d):
     check_delta(torch, x, first, state, out, starts, list(range(len(counts))))
 
 
+@pytest.mark.parametrize("count", [5, 200])
+def test_delta_of_keys_and_queries_of_other_lengths(torch_cuda, count):
+    """Keys of a tenth to twice the unit length, queries 2^20 and 2^-30 of it, large values."""
+    torch = torch_cuda
+    q, k, v, g, beta = delta_inputs(torch, 95, count, 2, 4, 128, torch.bfloat16)
+    gen = np.random.default_rng(5)
+    size = torch.from_numpy(gen.uniform(0.1, 1.4, count).astype(np.float32)).cuda()
+    k = (k.float() * size[:, None, None]).to(torch.bfloat16)
+    q[::3] *= 2.0 ** 20
+    q[1::3] *= 2.0 ** -30
+    v *= 3000.0
+    state = normal(torch, 96, 1, 4, 128, 128, scale=10.0)
+    first = state.clone()
+    out, starts = run_delta(torch, (q, k, v, g, beta), state, [count])
+    check_delta(torch, (q, k, v, g, beta), first, state, out, starts, [0])
+
+
+def test_delta_on_two_streams_at_once(torch_cuda):
+    """Two prompts side by side, a workspace each: the bits of one after the other."""
+    torch = torch_cuda
+    runs = []
+    for i in range(2):
+        x = delta_inputs(torch, 105 + i, 400, 2, 4, 128, torch.bfloat16)
+        state = normal(torch, 107 + i, 1, 4, 128, 128, scale=0.1)
+        alone = state.clone()
+        want = run_delta(torch, x, alone, [400])[0]
+        work = torch.empty(skv.gated_delta_workspace(400, 1, 4, 128, 400), dtype=torch.uint8, device="cuda")
+        runs.append((x, state, alone, want, torch.full_like(want, 9.0), ints(torch, [0, 400]), work, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for x, state, _, _, out, starts, work, stream in runs:
+        skv.gated_delta(*x, state, out, seq_starts=starts, max_tokens=400, workspace=work, stream=stream)
+    torch.cuda.synchronize()
+    for _, state, alone, want, out, *_ in runs:
+        assert torch.equal(state, alone) and torch.equal(out, want)
+
+
 @pytest.mark.parametrize("n", [1, 5, 130])
 def test_delta_one_token_each(torch_cuda, n):
     """The decode form: no starts; the rows' order given by an index, strided inputs and rows."""
@@ -659,3 +721,49 @@ def test_a_conversation_is_prefilled_handed_over_and_continued(torch_cuda):
             # the query that was read is the rotated one
             turned, mag = R.rotated(torch, q[first[s] + n + i].double(), n + i, inv, "half")
             assert ((query - turned).abs() <= 6 * 2.0 ** -24 * mag + turned.abs() * 2.0 ** -8 * 1.01 + 2.0 ** -100).all()
+
+
+def test_a_decode_step_in_a_graph_goes_on(torch_cuda):
+    """Append, attention and a delta step captured once; each replay goes one cell further, with the bits of plain calls."""
+    torch = torch_cuda
+    cells, steps = [30, 257, 4], 5
+    layers = [make_layer(torch, 121, [n + steps for n in cells]) for _ in range(2)]
+    inv = 1e4 ** (-torch.arange(32, device="cuda") / 32)
+    inputs = [[normal(torch, 130 + 10 * i + j, 3, h, 256, dtype=torch.bfloat16) for j, h in enumerate((24, 2, 2))] for i in range(steps)]
+    deltas = [delta_inputs(torch, 200 + i, 3, 2, 4, 128, torch.bfloat16) for i in range(steps)]
+    results = []
+    for captured, layer in enumerate(layers):
+        q, k, v = (torch.empty_like(x) for x in inputs[0])
+        d = [torch.empty_like(x) for x in deltas[0]]
+        have, then = ints(torch, cells), ints(torch, [0] * 3)
+        state = normal(torch, 140, 3, 4, 128, 128, scale=0.1)
+        out, delta_out = torch.empty_like(q), torch.empty(3, 4, 128, dtype=torch.bfloat16, device="cuda")
+        work = torch.empty(skv.decode_attention_workspace(layer, 3, 24), dtype=torch.uint8, device="cuda")
+
+        def step():
+            on = torch.cuda.current_stream()
+            skv.kv_append(layer, k, v, have, q=q, q_out=q, inv_freq=inv, lengths_out=then, stream=on)
+            skv.decode_attention(layer, q, then, out, workspace=work, stream=on)
+            skv.gated_delta(*d, state, delta_out, stream=on)
+            have.copy_(then)
+
+        graph = None
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+        outs = []
+        for i in range(steps):
+            for to, new in zip((q, k, v, *d), (*inputs[i], *deltas[i])):
+                to.copy_(new)
+            graph.replay() if captured else step()
+            outs += [out.clone(), delta_out.clone(), q.clone()]
+        assert have.tolist() == [n + steps for n in cells]
+        results.append((outs, state, layer.tensors[0], layer.tensors[1]))
+    assert status(torch) == 0
+    assert all(torch.equal(a, b) for a, b in zip(results[0][0], results[1][0]))
+    assert all(torch.equal(a, b) for a, b in zip(results[0][1:], results[1][1:]))
+    # and the first step's attention is the 64-bit one's over what the cache held then
+    layer, lengths = layers[0], [n + 1 for n in cells]
+    want, _, far, _ = R.attention(torch, layer, results[0][0][2], lengths, 0.0625)
+    assert ((results[0][0][0].double() - want).abs() <= far).all()
