@@ -9,6 +9,7 @@
 // bytes of S, read and written once; 32 columns are 128 bytes of a row, whole lines.
 #include "skv_ops.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstddef>
 #include <string>
@@ -1096,8 +1097,12 @@ cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
 template <typename T>
 cudaError_t launch(const DeltaDev& p, int sms, cudaStream_t stream) {
     if (!chunked(p.a.seq_starts != nullptr, p.a.max_tokens)) return launch_tokens<T>(p, stream);
-    // slices of 32 columns with the keys in halves while all of their CTAs run at once, else a CTA per head
-    const bool few = (int64_t) p.a.n_seqs * p.a.n_v_heads * (p.a.head_dim / 32) <= sms;
+    // Slices of 32 columns with the keys in halves, or a CTA per head: a chunk takes the first 4/7 of the time of the second
+    // (4/5 at head_dim 64), but they are dim / 32 times as many CTAs, one to an SM.  Either ends with its longest sequence or, if
+    // that is later, when the SMs have been through all tokens.  32 heads of 128, sequences of 2,048 tokens: one 116 and
+    // 204 us, two 218 and 220, three 318 and 237, eight 736 and 486.
+    const int64_t longest = std::min(p.a.max_tokens, p.a.n_tokens), all = (int64_t) p.a.n_tokens * p.a.n_v_heads / sms;
+    const bool few = std::max(longest, all * (p.a.head_dim / 32)) * 4 <= std::max(longest, all) * (p.a.head_dim == 64 ? 5 : 7);
     if (p.a.head_dim == 64) return few ? launch_chunks<T, 64, 2, 2, 1>(p, stream) : launch_chunks<T, 64, 4, 1, 2>(p, stream);
     return few ? launch_chunks<T, 128, 2, 2, 1>(p, stream) : launch_chunks<T, 128, 8, 1, 2>(p, stream);
 }
