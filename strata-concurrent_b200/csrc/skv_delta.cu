@@ -1094,17 +1094,29 @@ cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
     return launch_early(kKernel, dim3((unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * Room::kSlices)), Room::kThreadsOf, kSmem, stream, p);
 }
 
+/// How long a launch of so many CTAs per sequence and head takes, one CTA per SM, in tokens of one CTA: the longest sequence
+/// when all run at once; else what the longest ones take in their rounds or, if that is more, all tokens over the SMs and half
+/// of another sequence for the uneven end.
+int64_t span_of(const skv_gdn_args& a, int sms, int slices) {
+    const int64_t ctas = (int64_t) a.n_v_heads * slices, longest = std::min(a.max_tokens, a.n_tokens);
+    if (ctas * a.n_seqs <= sms) return longest;
+    const int64_t other = a.n_seqs > 1 ? std::min((a.n_tokens - longest) / (a.n_seqs - 1), longest) : 0;
+    return std::max((ctas + sms - 1) / sms * longest, a.n_tokens * ctas / sms + other / 2);
+}
+
 template <typename T>
 cudaError_t launch(const DeltaDev& p, int sms, cudaStream_t stream) {
     if (!chunked(p.a.seq_starts != nullptr, p.a.max_tokens)) return launch_tokens<T>(p, stream);
-    // Slices of 32 columns with the keys in halves, or a CTA per head: a chunk takes the first 4/7 of the time of the second
-    // (4/5 at head_dim 64), but they are dim / 32 times as many CTAs, one to an SM.  Either ends with its longest sequence or, if
-    // that is later, when the SMs have been through all tokens.  32 heads of 128, sequences of 2,048 tokens: one 116 and
-    // 204 us, two 218 and 220, three 318 and 237, eight 736 and 486.
-    const int64_t longest = std::min(p.a.max_tokens, p.a.n_tokens), all = (int64_t) p.a.n_tokens * p.a.n_v_heads / sms;
-    const bool few = std::max(longest, all * (p.a.head_dim / 32)) * 4 <= std::max(longest, all) * (p.a.head_dim == 64 ? 5 : 7);
-    if (p.a.head_dim == 64) return few ? launch_chunks<T, 64, 2, 2, 1>(p, stream) : launch_chunks<T, 64, 4, 1, 2>(p, stream);
-    return few ? launch_chunks<T, 128, 2, 2, 1>(p, stream) : launch_chunks<T, 128, 8, 1, 2>(p, stream);
+    // A chunk takes CTAs of 32 columns with the keys in halves, CTAs of 64, and CTAs of all 128 about 2, 3 and 4 units of time
+    // (at head_dim 64, 32 and 64 columns: 3 and 4); the wider, the fewer CTAs.  In us, bfloat16, 2,048 tokens a sequence,
+    // 128 wide: one sequence of 32 heads 116, 157, 204; of 48 heads 206, 165, 208; two of 32 216, 175, 218; of 48 314, 316,
+    // 234; eight of 32 736, 658, 486.  One of 8K and 15 of 100 tokens, 32 heads: 482, 622, 797; 64 heads: 919, 747, 845.
+    const int64_t narrow = span_of(p.a, sms, p.a.head_dim / 32);
+    if (p.a.head_dim == 64)
+        return narrow * 3 <= span_of(p.a, sms, 1) * 4 ? launch_chunks<T, 64, 2, 2, 1>(p, stream) : launch_chunks<T, 64, 4, 1, 2>(p, stream);
+    const int64_t middle = span_of(p.a, sms, 2) * 3, wide = span_of(p.a, sms, 1) * 4;
+    if (narrow * 2 <= std::min(middle, wide)) return launch_chunks<T, 128, 2, 2, 1>(p, stream);
+    return middle <= wide ? launch_chunks<T, 128, 4, 2, 1>(p, stream) : launch_chunks<T, 128, 8, 1, 2>(p, stream);
 }
 
 }  // namespace

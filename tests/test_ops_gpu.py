@@ -473,6 +473,19 @@ def test_delta_fills_the_gpu(torch_cuda, kind, kh, vh, d):
     check_delta(torch, x, first, state, out, starts, list(range(len(counts))))
 
 
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("vh,d,counts", [(32, 128, [190]), (48, 128, [190]), (32, 128, [70, 190]), (48, 128, [70, 129, 100]), (32, 64, [190]), (64, 64, [190, 64, 70])])
+def test_delta_of_each_width(torch_cuda, kind, vh, d, counts):
+    """On 148 SMs: CTAs of 32 columns, of 64 (twice), of a head; of 32 and of a head of 64."""
+    torch = torch_cuda
+    x = delta_inputs(torch, 85, sum(counts), 16, vh, d, getattr(torch, kind))
+    state = normal(torch, 86, len(counts), vh, d, d, scale=0.1)
+    first = state.clone()
+    out, starts = run_delta(torch, x, state, counts)
+    assert status(torch) == 0
+    check_delta(torch, x, first, state, out, starts, list(range(len(counts))))
+
+
 @pytest.mark.parametrize("count", [5, 200])
 def test_delta_of_keys_and_queries_of_other_lengths(torch_cuda, count):
     """Keys of a tenth to twice the unit length, queries 2^20 and 2^-30 of it, large values."""
