@@ -89,11 +89,26 @@ __device__ __forceinline__ uint2 quantize(const float (&x)[8], __half& scale) {
     for (int m = 1; m < 8; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
     scale = __float2half_rn(fminf(top / 127.0f, 65504.0f));
     const float step = __half2float(scale), by = step > 0.0f ? 1.0f / step : 0.0f, half = 0.5f * step;
-    uint32_t w[2] = {0, 0};
+    // The quotient by a reciprocal, rounded as it is added to 1.5 * 2^23, whose low byte is then the code.  What it leaves over
+    // is exact (a code and a scale have 18 bits together) and, where it is less than half a step, proves the code.
+    constexpr float kWhole = 12582912.0f;
+    uint32_t w[2] = {0, 0}, code[8];
+    bool sure = top <= 127.25f * step;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // the quotient by a reciprocal, clamped and rounded, then put right by what it leaves over (exact: a code and a scale
-        // have 18 bits together): a third of the time of a division, and the same code, ties included
+        const float c = fmaf(x[i], by, kWhole);
+        code[i] = __float_as_uint(c);
+        sure = sure && fabsf(fmaf(kWhole - c, step, x[i])) < half;   // not for a NaN, nor where the step is zero
+    }
+    if (sure) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040), __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410);
+        return make_uint2(w[0], w[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // ties, codes off by one, and values far past the scale
         float c = rintf(fminf(fmaxf(x[i] * by, -127.0f), 127.0f));   // a NaN becomes -127 here ...
         const float left = fmaf(-c, step, x[i]);
         if (left > half && c < 127.0f) c += 1.0f;
