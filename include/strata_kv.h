@@ -298,9 +298,9 @@ typedef struct skv_kv_layer {
  *
  * Rows [seq_starts[s], seq_starts[s+1]) of k and v belong to sequence s and go to its cells lengths[s], lengths[s]+1, ...
  * (seq_starts null: one row per sequence).  Rows before the first or behind the last sequence are padding: nothing comes
- * of them, and q_out keeps what it held there.  A cell is rotated by its own number: pair j turns by cell * inv_freq[j], the product taken in 64 bits, and
- * is scaled by rope_scale.  SKV_ROPE_HALF pairs value j with j + n_rot/2, SKV_ROPE_PAIRS value 2j with 2j+1; values
- * from n_rot on pass through; n_rot 0 (inv_freq null) rotates nothing.  q, when given, is rotated the same way into
+ * of them, and q_out keeps what it held there.  A cell is rotated by its own number: pair j turns by cell * inv_freq[j],
+ * the product taken in 64 bits, and is scaled by rope_scale.  SKV_ROPE_HALF pairs value j with j + n_rot/2, SKV_ROPE_PAIRS
+ * value 2j with 2j+1; values from n_rot on pass through; n_rot 0 (inv_freq null) rotates nothing.  q, when given, is rotated the same way into
  * q_out, which may be q itself.  int8: scale = fp16(max |x| / 127) per 64 values, code = x / scale rounded to nearest
  * even, within +-127 (a zero scale gives codes 0; a scale past fp16 saturates; a NaN takes code 0).
  * lengths_out, when given, gets lengths[s] + the number of its rows.
@@ -366,7 +366,9 @@ SKV_API int skv_decode_attention_workspace(const skv_kv_layer* layer, int n_seqs
  * for keys of unit length, and keys of one sequence are within a factor of 100 of each other in length.
  * seq_starts as in skv_kv_append; max_tokens bounds the tokens of one sequence (a longer one is cut there).  Calls of
  * few tokens a sequence (max_tokens below 16, or seq_starts null) run token by token, the others in chunks of 64 through the
- * tensor cores; both hold S in 32 bits.
+ * tensor cores; both hold S in 32 bits.  In chunks a value counts down to 2^-39 of the largest it is summed with, and an
+ * infinity or a NaN in a token or a state leaves nothing to rely on of the output and state of the value heads that use it, from
+ * the first token of its chunk on; other heads and sequences are as without it.
  * workspace: skv_gated_delta_workspace bytes of device memory, 256-byte aligned; as for skv_decode_attention. */
 typedef struct skv_gdn_args {
     const void* q;               /* [n_tokens][n_k_heads][head_dim] */

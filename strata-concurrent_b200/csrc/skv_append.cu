@@ -6,6 +6,11 @@
 // once (the angle cell * inv_freq in 64 bits, reduced by whole turns, then a 32-bit sincos of at most pi) and every row
 // uses them from shared memory; head_dim / 8 lanes hold a row, 16 bytes each, so a warp's loads and stores are whole
 // lines.  The half-style pair of a lane's values lies in another lane of the same row: one shuffle.
+//
+// Measured (24 + 4 heads of 256, 64 turned, in a graph): 32K tokens into an fp16 cache 166 us, 5.7 TB/s; into an int8 cache
+// 190 us, 4.7 TB/s, where finding the codes costs issue slots.  A ragged batch of 7,948 tokens into an int8 cache 52 us: its
+// 994 CTAs are 1.3 times what runs at once, and cutting them finer repeats the angles (47 to 57 us more or less at two, eight
+// and 48 CTAs per SM).  One token 2.8 us: a launch.
 #include "skv_ops.h"
 
 #include <string>

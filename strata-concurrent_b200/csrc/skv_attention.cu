@@ -6,16 +6,22 @@
 // go through the tensor cores (the up to 16 query heads that share a K/V head are the 16 rows of an m16n8k16 product, as
 // 12 of them on CUDA cores would take 12 flops per byte, more than the cores have at this bandwidth).
 //
-// Split.  The work is the tiles of all (sequence, K/V head) items laid end to end; one CTA per SM takes an equal,
-// contiguous share of them, worked out from the lengths on the device.  So one long sequence and many ragged ones load
-// the GPU alike.  An item that lies inside one share is finished there; an item cut by a share's border leaves parts
-// (its unnormalised output, maximum and sum) that join_kernel adds up in a fixed order.
+// Split.  The work is the tiles of all (sequence, K/V head) items laid end to end; each CTA takes an equal, contiguous share
+// of them, worked out from the lengths on the device, so one long sequence and many ragged ones load the GPU alike.  An
+// item that lies inside one share is finished there; an item cut by a share's border leaves parts (its unnormalised
+// output, maximum and sum) that join_kernel adds up in a fixed order.
 //
-// A tile is 32 KiB of K and as much of V (64 cells of 256 fp16 values): three stages fill the shared memory and keep at
-// least 64 KiB per SM in flight, twice what bandwidth x latency asks for.  Each warp copies (16-byte cp.async, chunks
-// swizzled by the row so that ldmatrix meets no bank twice), then scores, its own eighth of the cells; the warps
-// exchange row maxima and weights through shared memory and each multiplies all weights with its own eighth of V's
-// columns.  So no warp holds an output that another has to add, and a tile costs two barriers.
+// A tile is 32 KiB of K and as much of V (64 cells of 256 fp16 values; 64 int8 cells are half of that).  A CTA of four warps
+// holds one tile of K and two of V, and two to four CTAs share an SM: 192 KiB of copies on their way per SM, and one CTA's
+// products run under another's barriers (one CTA of eight warps and three tiles: 128K cells 76 us, 32 ragged sequences 101,
+// against 63 and 75).  Each warp copies its own quarter of the cells (16-byte cp.async, chunks swizzled by the row so that
+// ldmatrix meets no bank twice) and scores it; the warps exchange row maxima and weights through shared memory and each
+// multiplies all weights with its own quarter of V's columns.  So no warp holds an output that another has to add, and a
+// tile costs two barriers.
+//
+// Measured (24 heads on 2 K/V heads of 256, both kernels, in a graph): 131,072 fp16 cells 53 us, 5.0 TB/s; 32 ragged
+// sequences of 378 MB in all 72 us, 5.2 TB/s: the cache's bytes bound these, with 3 to 7 us of it the join.  8 x 32K int8 cells
+// 76.5 us, 3.6 TB/s: the conversion of every code to fp16 bounds it.  1,000 cells 11.4 us: two kernels' latencies.
 //
 // Precision.  fp16 queries and cache values meet in exact products, summed in 32 bits.  A bfloat16 query row is scaled by a
 // power of two to below 2 and becomes fp16 without loss, up to values 2^-24 of its largest.  Weights are rounded to fp16
@@ -65,7 +71,7 @@ struct Geo {
     static constexpr int kQueryStride = kDim + 8;     // halves
     static constexpr int kQueryBytes = kInt8 ? kRows * kQueryStride * 2 : 0;
     static constexpr int kSmem = 3 * kSlotBytes + kWeightBytes + kQueryBytes;   // K, and V twice
-    static constexpr int kPerSm = kPlane > 24000 ? 2 : kPlane > 12000 ? 3 : 4;   // CTAs: enough copies in flight
+    static constexpr int kPerSm = kPlane > 24000 ? 2 : kPlane > 12000 ? 3 : 4;   // CTAs: as many as shared memory holds
     static constexpr int kCols = kDim / kWarps;       // of the output, per warp
     static constexpr int kOutTiles = kCols / 8;
 };

@@ -6,7 +6,8 @@
 // kSlice of them (128 threads, 8 rows x 4 columns each at head_dim 128, in registers from its first token to its last).
 // One pass over the slice gives both k^T S and q^T S; the new output is q^T S + (q . k) d, so a token costs one
 // reduction over the rows: two shuffles and one exchange between the four warps.  A single token is bound by the
-// bytes of S, read and written once; 32 columns are 128 bytes of a row, whole lines.
+// bytes of S, read and written once; 32 columns are 128 bytes of a row, whole lines.  64 sequences of 32 heads of 128, a
+// token each: 44 us in a graph, 6.1 TB/s; one sequence 2.2 us.
 #include "skv_ops.h"
 
 #include <algorithm>
@@ -150,23 +151,28 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 //     S <- e^(G_63) S + K^T (e^(G_63 - G) V')
 // What needs no state, P and T = (I + A)^-1 with the decays, is worked out first, for all chunks at once: prepare_kernel
 // writes a record per chunk and head into the workspace.  Then chunk_kernel takes one head's slice of 16 kGroupsOf value
-// columns through all chunks of its sequence: four loader warps stay a chunk ahead, and a pair of consumer warps holds
-// the transposed state of 16 columns in accumulators, each warp one half of the keys.  What a product leaves in
-// accumulators is the left operand of the next (S^T K^T, then V'^T = R^T T^T, then S^T += V'^T K), so the chain from
-// chunk to chunk passes through memory once, where the halves' sums over the keys meet.  That chain, not the flops,
-// bounds a long sequence: hence the halves, and narrow slices where few CTAs would run (2 groups: 128 CTAs for 32
-// heads of one sequence), wider ones where there are more than fill the GPU (4).
+// columns through all chunks of its sequence.  Four loader warps stay a chunk ahead.  State warps hold the transposed state of
+// 16 columns each in accumulators, alone or as a pair with a half of the keys each (kSplit).  Output warps turn the states
+// and V' that those leave in shared memory into O.  What a product leaves in accumulators is the left operand of the next
+// (S^T K^T, then V'^T = R^T T^T, then S^T += V'^T K), so the chain from chunk to chunk passes through memory once, where a
+// pair's sums over the keys meet, or not at all.  That chain's latency, not the flops, bounds a long sequence: hence the pairs
+// and slices of 32 columns where few CTAs would run, 4 state warps with a scheduler each; a whole head per CTA, whose
+// 8 state warps share the copies and records, where there are more than fill the GPU.
+//
+// Measured, 32 heads of 128 on 16 key heads: one bfloat16 sequence of 32K tokens 1,627 us, 230 of them prepare_kernel (the
+// chain takes 2.7 us a chunk; the bytes alone would take 125); 12 ragged fp16 sequences of 15,943 tokens in all 568 us.
 //
 // Precision.  Every product is fp16 with 32-bit sums.  A 32-bit operand (S, R, V', T, A) enters as the sum of two fp16
 // values after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least; the
-// state therefore keeps 32-bit quality.  Only what goes to the 16-bit output alone (Q S, P V') takes the first of the
-// two.  K and Q are exact: fp16 as they are, bfloat16 scaled by a power of two (K by one per chunk, Q by one per row), up
-// to values 2^-24 of the largest.  The sums G are taken in 64 bits and kept as two 32-bit parts, so that a decay of
-// e^-200 in a chunk (deeper ones are as good as that) leaves the others' differences exact.
+// state therefore keeps 32-bit quality.  What goes to the output alone (Q S, P V') takes the first of the two where that
+// is bfloat16, eight times coarser; for fp16 outputs P and V' take both.  K and Q are exact: fp16 as they are, bfloat16
+// scaled by a power of two (K by one per chunk, Q by one per row), up to values 2^-24 of the largest.  The sums G are taken
+// in 64 bits and kept as two 32-bit parts, so that a decay of e^-200 in a chunk (deeper ones are as good as that) leaves the
+// others' differences exact.
 
 constexpr int kChunk = 64;
-constexpr int kProducers = 4;
-constexpr int kProducerThreads = kProducers * 32;
+constexpr int kLoaders = 4;
+constexpr int kLoaderThreads = kLoaders * 32;
 constexpr int kScratch = 68;          // floats between rows of the 32-bit scratch matrices
 // T's entries are about 1 at most for keys of about unit length: 2^5 of them leaves their two fp16 parts 30 bits below 1,
 // and room for entries of 2,000 where keys differ in length.
@@ -396,10 +402,10 @@ __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, con
 /// One chunk of one key head, for all of its value heads: K, Q and their products serve them all.  Four warps; four CTAs
 /// an SM hide the short phases' latencies.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __grid_constant__ DeltaDev p) {
+__global__ void __launch_bounds__(kLoaderThreads, 4) prepare_kernel(const __grid_constant__ DeltaDev p) {
     extern __shared__ __align__(128) uint8_t smem[];
     auto& room = *reinterpret_cast<PrepareRoom<kDim>*>(smem);
-    constexpr int kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
+    constexpr int kChunks = kDim / 8, kMine = kChunk * kChunks / kLoaderThreads;
     constexpr bool kFine = std::is_same<T, __half>::value;
     const skv_gdn_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -426,7 +432,7 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
     uint4 k[kMine], q[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-        const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+        const int at = i * kLoaderThreads + tid, r = at / kChunks, chunk = at % kChunks;
         const bool on = t0 + r < end;
         k[i] = on ? __ldg(reinterpret_cast<const uint4*>(kh + (int64_t) (t0 + r) * a.k_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
         q[i] = on ? __ldg(reinterpret_cast<const uint4*>(qh + (int64_t) (t0 + r) * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
     }
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-        const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+        const int at = i * kLoaderThreads + tid, r = at / kChunks, chunk = at % kChunks;
         int power = 0;
         if constexpr (!std::is_same<T, __half>::value) {
             float x[8], most = 0.0f;
@@ -610,7 +616,7 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
         }
         __syncthreads();
         // ---- T in two fp16 parts, and P
-        for (int at = tid; at < kTriangleBytes / 16; at += kProducerThreads) {
+        for (int at = tid; at < kTriangleBytes / 16; at += kLoaderThreads) {
             const int block = at / 32, r = at % 32 / 2, chunk = at % 2;
             const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3, j = block - block_of(i, 0);
             const float4* x = reinterpret_cast<const float4*>(&work.t[(i * 16 + r) * kScratch + j * 16 + chunk * 8]);
@@ -637,7 +643,7 @@ __global__ void __launch_bounds__(kProducerThreads, 4) prepare_kernel(const __gr
 template <int kDim, int kGroupsOf, int kSplit, int kTogether, bool kFine>
 struct ChunkRoom {
     static constexpr int kStates = kGroupsOf * kSplit, kOutputs = kGroupsOf / kTogether;
-    static constexpr int kThreadsOf = (kProducers + kStates + kOutputs) * 32;   // loaders, state warps, output warps
+    static constexpr int kThreadsOf = (kLoaders + kStates + kOutputs) * 32;   // loaders, state warps, output warps
     static constexpr int kMeeting = (kSplit * kTogether + 1) * 32;              // the state warps of an output warp, and it
     static constexpr int kSlices = kDim / (kGroupsOf * 16);
     struct Buffer {
@@ -661,7 +667,7 @@ enum : int { kFull = 0, kEmpty = 2, kPair = 4, kValueFree = 4, kStateReady = 8, 
 
 template <typename T, int kDim, typename Room>
 __device__ __forceinline__ void load_chunks(const DeltaDev& p, Room& room, int begin, int end, int seq, int head, int slice) {
-    constexpr int kAll = Room::kThreadsOf, kChunks = kDim / 8, kMine = kChunk * kChunks / kProducerThreads;
+    constexpr int kAll = Room::kThreadsOf, kChunks = kDim / 8, kMine = kChunk * kChunks / kLoaderThreads;
     constexpr int kValueChunks = sizeof(Room::Buffer::v) / (kChunk * 16);
     const skv_gdn_args& a = p.a;
     const int tid = threadIdx.x;
@@ -675,19 +681,19 @@ __device__ __forceinline__ void load_chunks(const DeltaDev& p, Room& room, int b
         if (n >= 2) meet<kAll>(kEmpty + b);
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
-            const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+            const int at = i * kLoaderThreads + tid, r = at / kChunks, chunk = at % kChunks;
             const uint32_t to = chunk_at<kChunks>(r, chunk);
             const bool on = t0 + r < end;
             const int64_t t = on ? t0 + r : begin;
             copy_async16(smem_at(buf.k) + to, kh + t * a.k_stride + chunk * 8, on);
             copy_async16(smem_at(buf.q) + to, qh + t * a.q_stride + chunk * 8, on);
         }
-        for (int at = tid; at < kChunk * kValueChunks; at += kProducerThreads) {
+        for (int at = tid; at < kChunk * kValueChunks; at += kLoaderThreads) {
             const int r = at / kValueChunks, chunk = at % kValueChunks;
             const bool on = t0 + r < end;
             copy_async16(smem_at(buf.v) + chunk_at<kValueChunks>(r, chunk), vh + (int64_t) (on ? t0 + r : begin) * a.v_stride + chunk * 8, on);
         }
-        for (int at = tid; at < (int) ((Room::kRest ? sizeof(Record) : offsetof(Record, mix_low)) / 16); at += kProducerThreads)
+        for (int at = tid; at < (int) ((Room::kRest ? sizeof(Record) : offsetof(Record, mix_low)) / 16); at += kLoaderThreads)
             copy_async16(smem_at(&buf.record) + at * 16, reinterpret_cast<const uint8_t*>(record) + at * 16, true);
         asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
         if constexpr (!std::is_same<T, __half>::value) {
@@ -695,7 +701,7 @@ __device__ __forceinline__ void load_chunks(const DeltaDev& p, Room& room, int b
             const float key_down = __ldg(&record->f.key_down);
 #pragma unroll 4
             for (int i = 0; i < kMine; ++i) {
-                const int at = i * kProducerThreads + tid, r = at / kChunks, chunk = at % kChunks;
+                const int at = i * kLoaderThreads + tid, r = at / kChunks, chunk = at % kChunks;
                 const uint32_t to = chunk_at<kChunks>(r, chunk);
                 const float down = __ldg(&record->f.down[r]);
                 float x[8];
@@ -719,7 +725,7 @@ __device__ __forceinline__ void advance(Room& room, int begin, int end, int slic
     constexpr int kAll = Room::kThreadsOf, kMeeting = Room::kMeeting, kChunks = kDim / 8;
     constexpr int kValueChunks = sizeof(Room::Buffer::v) / (kChunk * 16);
     constexpr int kKeys = kDim / kSplit;
-    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kProducers, g = lane >> 2, c = lane & 3;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kLoaders, g = lane >> 2, c = lane & 3;
     const int part = kSplit == 1 ? 0 : warp & 1, group = kSplit == 1 ? warp : warp >> 1, key0 = part * kKeys;
     const int output = group / kTogether;
     const int col0 = slice * kValueChunks * 8 + group * 16;   // the group's value columns
@@ -909,7 +915,7 @@ __device__ __forceinline__ void put_out(const DeltaDev& p, Room& room, int begin
     constexpr int kAll = Room::kThreadsOf, kMeeting = Room::kMeeting, kChunks = kDim / 8, kDeep = kDim / kSplit / 16;
     constexpr int kValueChunks = sizeof(Room::Buffer::v) / (kChunk * 16);
     const skv_gdn_args& a = p.a;
-    const int lane = threadIdx.x & 31, output = (threadIdx.x >> 5) - kProducers - Room::kStates, g = lane >> 2, c = lane & 3;
+    const int lane = threadIdx.x & 31, output = (threadIdx.x >> 5) - kLoaders - Room::kStates, g = lane >> 2, c = lane & 3;
     T* const out = static_cast<T*>(a.out) + head * kDim + slice * kValueChunks * 8 + output * kTogether * 16 + 2 * c;
     int b = 0;
     for (int t0 = begin; t0 < end; t0 += kChunk, b ^= 1) {
@@ -1053,10 +1059,10 @@ __global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, 
     float* const state = state_of(p, seq, head, kDim);
     if (!state) return;
     const int warp = threadIdx.x >> 5;
-    if (warp < kProducers) {
+    if (warp < kLoaders) {
         if constexpr (kShares) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegisters));
         load_chunks<T, kDim>(p, room, begin, end, seq, head, slice);
-    } else if (warp < kProducers + Room::kStates) {
+    } else if (warp < kLoaders + Room::kStates) {
         if constexpr (kShares) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kStateRegisters));
         advance<T, kDim, kSplit, kTogether>(room, begin, end, slice, state);
     } else {
@@ -1089,7 +1095,7 @@ cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(prepare_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepare);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    e = launch_early(prepare_kernel<T, kDim>, dim3((unsigned) (record_slots(p.a.n_tokens, p.a.n_seqs) * p.a.n_k_heads)), kProducerThreads, kPrepare, stream, p);
+    e = launch_early(prepare_kernel<T, kDim>, dim3((unsigned) (record_slots(p.a.n_tokens, p.a.n_seqs) * p.a.n_k_heads)), kLoaderThreads, kPrepare, stream, p);
     if (e != cudaSuccess) return e;
     return launch_early(kKernel, dim3((unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * Room::kSlices)), Room::kThreadsOf, kSmem, stream, p);
 }

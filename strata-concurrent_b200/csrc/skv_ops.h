@@ -87,8 +87,8 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 /// A kernel launched with launch_early begins with this: whatever ran before on the stream has then ended.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-/// A launch that may be set up while the kernel before it on the stream ends; the kernel waits for that one itself.  Back to
-/// back calls that end in 3 us each are then 1 us nearer to each other.
+/// A launch that may be set up while the kernel before it on the stream ends; the kernel waits for that one itself.  One
+/// step of the delta rule in a graph of them takes 2.2 us so, 2.7 without; attention over 1,000 cells, two kernels, 11.4 and 14.4.
 template <typename... Parameters, typename... Arguments>
 cudaError_t launch_early(void (*kernel)(Parameters...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Arguments&... arguments) {
     cudaLaunchConfig_t config{};

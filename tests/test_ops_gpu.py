@@ -503,6 +503,24 @@ def test_delta_of_keys_and_queries_of_other_lengths(torch_cuda, count):
     check_delta(torch, (q, k, v, g, beta), first, state, out, starts, [0])
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("vh", [4, 160])
+def test_delta_keeps_a_bad_token_to_its_heads(torch_cuda, bad, vh):
+    """A NaN or an infinity in a key: other sequences, other key heads and the chunks before it as without it."""
+    torch = torch_cuda
+    counts = [100, 200, 70]
+    x = list(delta_inputs(torch, 98, sum(counts), 2, vh, 128, torch.float16))
+    state = normal(torch, 99, 3, vh, 128, 128, scale=0.1)
+    clean = state.clone()
+    want = run_delta(torch, x, clean, counts)[0]
+    x[1] = x[1].clone()
+    x[1][100 + 130, 1, 5] = bad
+    got = run_delta(torch, x, state, counts)[0]
+    assert torch.equal(got[:, : vh // 2], want[:, : vh // 2]) and torch.equal(state[:, : vh // 2], clean[:, : vh // 2])
+    assert torch.equal(got[:228], want[:228]) and torch.equal(got[300:], want[300:])
+    assert torch.equal(state[::2], clean[::2]) and not got[230, vh // 2 :].isfinite().any()
+
+
 def test_delta_on_two_streams_at_once(torch_cuda):
     """Two prompts side by side, a workspace each: the bits of one after the other."""
     torch = torch_cuda
