@@ -1,16 +1,17 @@
 // skv_append.cu - skv_kv_append: K and V of new tokens into their cells of a paged cache, rotated on the way, and q
 // beside them.
 //
-// Pure streaming: every value is read once and written once, so the bytes bound it.  A CTA takes kTokens tokens and
-// a share of their rows (a row is one head of q, K or V of one token).  It computes the cosines and sines of its tokens
-// once (the angle cell * inv_freq in 64 bits, reduced by whole turns, then a 32-bit sincos of at most pi) and every row
-// uses them from shared memory; head_dim / 8 lanes hold a row, 16 bytes each, so a warp's loads and stores are whole
-// lines.  The half-style pair of a lane's values lies in another lane of the same row: one shuffle.
+// Pure streaming: every value is read once and written once, so the bytes bound it, where the instructions beside them stay
+// few.  A CTA takes kTokens tokens and a share of their rows (a row is one head of q, K or V of one token).  It computes the
+// cosines and sines of its tokens once (the angle cell * inv_freq in 64 bits, reduced by whole turns, then a 32-bit sincos of
+// at most pi) and every row uses them from shared memory.  Of K and V, head_dim / 8 lanes hold a row, 16 bytes each; the
+// half-style pair of a lane's values lies in another lane of the same row: one shuffle.  Of q, by far the most rows, what is
+// not turned is copied as it lies (or left, in place), and what is turned goes 16 values a thread, both of a pair, in full
+// warps: 32K tokens 155 us, 166 with q's rows treated like K's, at 80 % of all issue slots.
 //
-// Measured (24 + 4 heads of 256, 64 turned, in a graph): 32K tokens into an fp16 cache 166 us, 5.7 TB/s; into an int8 cache
-// 190 us, 4.7 TB/s, where finding the codes costs issue slots.  A ragged batch of 7,948 tokens into an int8 cache 52 us: its
-// 994 CTAs are 1.3 times what runs at once, and cutting them finer repeats the angles (47 to 57 us more or less at two, eight
-// and 48 CTAs per SM).  One token 2.8 us: a launch.
+// Measured (24 + 4 heads of 256, 64 turned, in a graph): 32K tokens into an fp16 cache 155 us, 6.1 TB/s; into an int8 cache
+// 155 us, 5.9 TB/s.  A ragged batch of 7,948 tokens into an int8 cache 45 us, 4.9 TB/s: its 994 CTAs are 1.7 times what runs at
+// once, and cutting them finer repeats the angles.  One token 3 us: a launch.
 #include "skv_ops.h"
 
 #include <string>
@@ -57,10 +58,12 @@ namespace {
 
 constexpr int kTokens = 8;      // tokens per CTA
 constexpr int kThreads = 256;
-// Rows a thread has on their way at once, beside those it works on.  With 8 tokens per CTA, 32K tokens of 24 + 4 heads of
-// 256 take 167 us at 2 and at 4, 188 at 7 (registers cost CTAs); 8K tokens 57 at 2, 66 at 4.  4 or 16 tokens per CTA: 170, 167
-// and, for 64 single tokens, 3.1 and 4.2 against 3.3.
+// 16-byte pieces a thread has on their way at once: of K and V, beside those it works on; of q's copies; and of q's turned
+// pieces, two each.  32K tokens of 24 + 4 heads of 256, fp16 and int8 caches, and a ragged int8 batch: 8 copies and 2 turns
+// 155, 155 and 45 us; 4 and 2 158, 162 and 46; 2 and 1 164, 169 and 51; 4 and 4 172, 222 and 67 (registers cost CTAs).  One of K
+// and V ahead in place of two: 159, 157 and 45.  4 or 16 tokens per CTA: 162 and 163, 166 and 171, 48 and 49.
 constexpr int kAhead = 2;
+constexpr int kCopies = 8, kTurns = 2;
 constexpr int kMaxPairs = 128;  // n_rot / 2 of the widest head
 
 struct AppendDev {
@@ -68,8 +71,16 @@ struct AppendDev {
     skv_append_args a;
     uint32_t* status;
     int share;        // rows (over all of the CTA's tokens) per CTA in y
-    float per_row;    // 1 / rows of a token
+    float per_kv, per_q, per_turn;   // 1 / rows of K and V a token, 1 / rows of q a token, 1 / groups of eight pairs a row
 };
+
+/// r / d of small numbers (below 2^20 here), by = 1 / d: exact, as r + 1/2 is half a part away from the next quotient.
+__device__ __forceinline__ int quotient_of(int r, float by) { return (int) (((float) r + 0.5f) * by); }
+__device__ __forceinline__ void turn_pair(float& x, float& y, float2 c) {
+    const float u = x;
+    x = u * c.x - y * c.y;
+    y = y * c.x + u * c.y;
+}
 
 /// The sequence of packed row `row`, the last s with starts[s] <= row, found by a whole warp, 32 places at a time; -1
 /// outside of [starts[0], starts[n]).
@@ -134,24 +145,24 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     const skv_append_args& a = p.a;
     const int tid = threadIdx.x, first = blockIdx.x * kTokens;
     const int pairs = a.n_rot >> 1;
-    const int kv = p.layer.n_head_kv, rows = (a.q ? a.n_head : 0) + 2 * kv;
+    const int kv = p.layer.n_head_kv, kv_rows = 2 * kv * kTokens;
     const int lane = tid % kLanes, at = lane * 8;
-    const int lo = blockIdx.y * p.share, hi = min(lo + p.share, rows * kTokens);
+    const int lo = blockIdx.y * p.share, hi = min(lo + p.share, kv_rows + (a.q ? a.n_head * kTokens : 0));
+    const int kv_hi = min(hi, kv_rows);
     constexpr int kTrip = kThreads / kLanes;
     uint4 ahead[kAhead];
-    // row r of the CTA's tokens: K's heads, V's, q's of the first token, then the next one's.  Only rows of the call's
-    // arrays are touched, whether or not a sequence has them: what no sequence has is not used.
+    // the CTA's rows: K's heads and V's of its first token, of the next one ...; then q's in the same way.  Only rows of the
+    // call's arrays are touched, whether or not a sequence has them: what no sequence has is not used.
     const auto fetch = [&](int base) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int r = base + i * kTrip + tid / kLanes;
-            const int t = (int) (((float) r + 0.5f) * p.per_row), row = r - t * rows;   // exact: r < 2^17
+            const int t = quotient_of(r, p.per_kv), row = r - t * 2 * kv;
             ahead[i] = make_uint4(0, 0, 0, 0);
-            if (r < hi && first + t < a.n_tokens) {
+            if (r < kv_hi && first + t < a.n_tokens) {
                 const int64_t token = first + t;
                 const T* src = row < kv ? static_cast<const T*>(a.k) + token * a.k_stride + row * kDim
-                             : row < 2 * kv ? static_cast<const T*>(a.v) + token * a.v_stride + (row - kv) * kDim
-                                            : static_cast<const T*>(a.q) + token * a.q_stride + (row - 2 * kv) * kDim;
+                                        : static_cast<const T*>(a.v) + token * a.v_stride + (row - kv) * kDim;
                 ahead[i] = *reinterpret_cast<const uint4*>(src + at);
             }
         }
@@ -202,72 +213,133 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     }
     __syncthreads();
 
-    // every lane of a row makes the same trips, and a warp's lanes meet at the shuffles: rows past the end are idle
-    for (int base = lo; base < hi; base += kAhead * kTrip) {
+    // ---- K and V.  Every lane of a row makes the same trips, and a warp's lanes meet at the shuffles: rows past the end are idle
+    for (int base = lo; base < kv_hi; base += kAhead * kTrip) {
         uint4 now[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) now[i] = ahead[i];
-        if (base + kAhead * kTrip < hi) fetch(base + kAhead * kTrip);
+        if (base + kAhead * kTrip < kv_hi) fetch(base + kAhead * kTrip);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int r = base + i * kTrip + tid / kLanes;
-        if (base + i * kTrip >= hi) break;   // the same for the whole CTA
-        const int t = min((int) (((float) r + 0.5f) * p.per_row), kTokens - 1), row = r - t * rows;
-        const bool on = r < hi && s_held[t];
-        const int64_t token = first + t;
-        const bool is_k = row < kv, is_v = !is_k && row < 2 * kv;
-        const int head = is_k ? row : is_v ? row - kv : row - 2 * kv;
-        const uint4 raw = now[i];
-        float x[8];
-        unpack8<T>(raw, x);
-        if (pairs) {
-            if (a.rope_style == SKV_ROPE_HALF) {
-                const int hop = pairs / 8;   // lanes between the two values of a pair
-                const bool low = at < pairs;
-                const int other = (tid & 31) + (low ? hop : -hop);
-                uint4 o;
-                o.x = __shfl_sync(0xffffffffu, raw.x, other & 31);
-                o.y = __shfl_sync(0xffffffffu, raw.y, other & 31);
-                o.z = __shfl_sync(0xffffffffu, raw.z, other & 31);
-                o.w = __shfl_sync(0xffffffffu, raw.w, other & 31);
-                if (on && !is_v && at < a.n_rot) {
-                    float y[8];
-                    unpack8<T>(o, y);
-                    const int j = low ? at : at - pairs;
+        for (int i = 0; i < kAhead; ++i) {
+            const int r = base + i * kTrip + tid / kLanes;
+            if (base + i * kTrip >= kv_hi) break;   // the same for the whole CTA
+            const int t = min(quotient_of(r, p.per_kv), kTokens - 1), row = r - t * 2 * kv;
+            const bool on = r < kv_hi && s_held[t], is_k = row < kv;
+            const uint4 raw = now[i];
+            float x[8];
+            unpack8<T>(raw, x);
+            if (pairs) {
+                if (a.rope_style == SKV_ROPE_HALF) {
+                    const int hop = pairs / 8;   // lanes between the two values of a pair
+                    const bool low = at < pairs;
+                    const int other = (tid & 31) + (low ? hop : -hop);
+                    uint4 o;
+                    o.x = __shfl_sync(0xffffffffu, raw.x, other & 31);
+                    o.y = __shfl_sync(0xffffffffu, raw.y, other & 31);
+                    o.z = __shfl_sync(0xffffffffu, raw.z, other & 31);
+                    o.w = __shfl_sync(0xffffffffu, raw.w, other & 31);
+                    if (on && is_k && at < a.n_rot) {
+                        float y[8];
+                        unpack8<T>(o, y);
+                        const int j = low ? at : at - pairs;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float2 c = turn[t][j + i];
-                        x[i] = low ? x[i] * c.x - y[i] * c.y : x[i] * c.x + y[i] * c.y;
+                        for (int m = 0; m < 8; ++m) {
+                            const float2 c = turn[t][j + m];
+                            x[m] = low ? x[m] * c.x - y[m] * c.y : x[m] * c.x + y[m] * c.y;
+                        }
+                    }
+                } else if (on && is_k && at < a.n_rot) {
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const float2 c = turn[t][at / 2 + m];
+                        const float u = x[2 * m], w = x[2 * m + 1];
+                        x[2 * m] = u * c.x - w * c.y;
+                        x[2 * m + 1] = w * c.x + u * c.y;
                     }
                 }
-            } else if (on && !is_v && at < a.n_rot) {
+            }
+            const int64_t to = on && s_row[t] >= 0 ? s_row[t] + ((int64_t) (is_k ? row : row - kv) << p.layer.page_shift) : -1;
+            if (kInt8) {
+                __half scale;
+                const uint2 codes = quantize(x, scale);
+                if (to >= 0) {
+                    uint8_t* pool = is_k ? p.layer.k : p.layer.v;
+                    *reinterpret_cast<uint2*>(pool + to * kDim + at) = codes;
+                    if ((lane & 7) == 0) (is_k ? p.layer.k_scale : p.layer.v_scale)[to * (kDim / kInt8Group) + lane / 8] = scale;
+                }
+            } else if (to >= 0) {
+                // rounded to the cache's fp16, once; a bf16 value past its range becomes infinite
+                *reinterpret_cast<uint4*>((is_k ? p.layer.k : p.layer.v) + (to * kDim + at) * 2) = pack8<__half>(x);
+            }
+        }
+    }
+    if (hi <= kv_rows) return;
+
+    // ---- q.  What is not turned is copied as it lies, unless it lies there already
+    const int q_lo = max(lo - kv_rows, 0), q_hi = hi - kv_rows;
+    const T* const q = static_cast<const T*>(a.q);
+    T* const q_out = static_cast<T*>(a.q_out);
+    if (a.n_rot < kDim && q != q_out) {
+        for (int base = q_lo + tid / kLanes; base < q_hi; base += kCopies * kTrip) {
+            uint4 w[kCopies];
+            int64_t to[kCopies];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 c = turn[t][at / 2 + i];
-                    const float u = x[2 * i], w = x[2 * i + 1];
-                    x[2 * i] = u * c.x - w * c.y;
-                    x[2 * i + 1] = w * c.x + u * c.y;
+            for (int i = 0; i < kCopies; ++i) {
+                const int r = base + i * kTrip, t = quotient_of(r, p.per_q);
+                to[i] = -1;
+                if (r < q_hi && at >= a.n_rot && s_held[t]) {
+                    const int64_t token = first + t, in = (r - t * a.n_head) * kDim + at;
+                    to[i] = token * a.q_out_stride + in;
+                    w[i] = *reinterpret_cast<const uint4*>(q + token * a.q_stride + in);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i)
+                if (to[i] >= 0) *reinterpret_cast<uint4*>(q_out + to[i]) = w[i];
         }
-        int64_t to = -1;
-        if (on && (is_k || is_v) && s_row[t] >= 0) to = s_row[t] + ((int64_t) head << p.layer.page_shift);
-        if (kInt8) {
-            __half scale;
-            uint2 codes;
-            if (__any_sync(0xffffffffu, to >= 0)) codes = quantize(x, scale);   // not for a warp of query rows
-            if (to >= 0) {
-                uint8_t* pool = is_k ? p.layer.k : p.layer.v;
-                *reinterpret_cast<uint2*>(pool + to * kDim + at) = codes;
-                if ((lane & 7) == 0) (is_k ? p.layer.k_scale : p.layer.v_scale)[to * (kDim / kInt8Group) + lane / 8] = scale;
+    }
+    // ... and eight pairs a thread are turned, in whole warps whatever part of a row that is: 16 bytes at one place and 16 at
+    // another, half a rotation or 16 bytes away
+    if (pairs) {
+        const bool halves = a.rope_style == SKV_ROPE_HALF;
+        const int per = a.n_rot >> 4, apart = halves ? pairs : 8;
+        const int end = q_hi * per;
+        for (int base = q_lo * per + tid; base < end; base += kTurns * kThreads) {
+            uint4 v[kTurns], w[kTurns];
+            int64_t to[kTurns];
+            const float2* by[kTurns];
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const int e = base + i * kThreads, r = quotient_of(e, p.per_turn), j = e - r * per, t = quotient_of(r, p.per_q);
+                to[i] = -1;
+                if (e < end && s_held[t]) {
+                    const int64_t token = first + t, in = (r - t * a.n_head) * kDim + j * (halves ? 8 : 16);
+                    to[i] = token * a.q_out_stride + in;
+                    by[i] = &turn[t][j * 8];
+                    v[i] = *reinterpret_cast<const uint4*>(q + token * a.q_stride + in);
+                    w[i] = *reinterpret_cast<const uint4*>(q + token * a.q_stride + in + apart);
+                }
             }
-        } else if (to >= 0) {
-            // rounded to the cache's fp16, once; a bf16 value past its range becomes infinite
-            *reinterpret_cast<uint4*>((is_k ? p.layer.k : p.layer.v) + (to * kDim + at) * 2) = pack8<__half>(x);
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                if (to[i] < 0) continue;
+                float x[8], y[8];
+                unpack8<T>(v[i], x);
+                unpack8<T>(w[i], y);
+                if (halves) {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) turn_pair(x[m], y[m], by[i][m]);
+                } else {
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        turn_pair(x[2 * m], x[2 * m + 1], by[i][m]);
+                        turn_pair(y[2 * m], y[2 * m + 1], by[i][m + 4]);
+                    }
+                }
+                *reinterpret_cast<uint4*>(q_out + to[i]) = pack8<T>(x);
+                *reinterpret_cast<uint4*>(q_out + to[i] + apart) = pack8<T>(y);
+            }
         }
-        if (on && !is_k && !is_v)
-            *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + token * a.q_out_stride + head * kDim + at) = pack8<T>(x);
-      }
     }
 }
 
@@ -330,7 +402,9 @@ extern "C" int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* a
     const int trips = (rows + trip - 1) / trip;
     if (split > trips) split = trips;
     p.share = (trips + split - 1) / split * trip;
-    p.per_row = 1.0f / (float) (rows / kTokens > 0 ? rows / kTokens : 1);
+    p.per_kv = 1.0f / (float) (2 * layer->n_head_kv);
+    p.per_q = a.q ? 1.0f / (float) a.n_head : 1.0f;
+    p.per_turn = a.n_rot ? 16.0f / (float) a.n_rot : 1.0f;
     const dim3 grid((unsigned) blocks, (unsigned) ((rows + p.share - 1) / p.share));
     const auto s = static_cast<cudaStream_t>(stream);
     const bool int8 = layer->format == SKV_KV_INT8;
