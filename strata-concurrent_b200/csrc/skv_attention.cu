@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) join_kernel(const __grid_cons
 template <typename T, int kDim, bool kInt8>
 cudaError_t launch(const AttnDev& p, int sms, cudaStream_t stream) {
     constexpr int kSmem = Geo<kDim, kInt8>::kSmem, kPerSm = Geo<kDim, kInt8>::kPerSm;
-    static_assert((kSmem + 3072) * kPerSm <= (int) kSmemPerSm && kPerSm <= 4, "the CTAs fit an SM");
+    static_assert((kSmem + 3 * 1024) * kPerSm <= (int) kSmemPerSm && kPerSm <= 4, "the CTAs fit an SM");
     const int ctas = sms * kPerSm;
     cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kDim, kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
