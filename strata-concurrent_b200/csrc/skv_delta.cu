@@ -34,6 +34,7 @@ struct DeltaDev {
     uint32_t* status;
     Record* records;   // [slot][value head], when the call runs in chunks
     int ratio;         // value heads per key head
+    int ranked;        // longest sequences first
 };
 
 /// The tokens [begin, end) of a sequence; false when it has none.
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 // 8 state warps share the copies and records, where there are more than fill the GPU.
 //
 // Measured, 32 heads of 128 on 16 key heads: one bfloat16 sequence of 32K tokens 1,627 us, 230 of them prepare_kernel (the
-// chain takes 2.7 us a chunk; the bytes alone would take 125); 12 ragged fp16 sequences of 15,943 tokens in all 568 us.
+// chain takes 2.7 us a chunk; the bytes alone would take 125); 12 ragged fp16 sequences of 15,943 tokens in all 522 us.
 //
 // Precision.  Every product is fp16 with 32-bit sums.  A 32-bit operand (S, R, V', T, A) enters as the sum of two fp16
 // values after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least; the
@@ -1043,6 +1044,10 @@ __device__ __forceinline__ void put_out(const DeltaDev& p, Room& room, int begin
 constexpr int kLoaderRegisters = 48, kStateRegisters = 176, kOutputRegisters = 112;
 static_assert(kLoaderRegisters * 128 + kStateRegisters * 256 + kOutputRegisters * 128 == 128 * 512, "the shares of 512 threads launched with 128 each");
 
+/// Up to so many sequences are taken longest first, so that no long one begins when the others end: 12 ragged prompts of
+/// 15,943 tokens 522 us (570 in their order), four of 1K and then one of 4K 344 (476); fp16, 32 heads of 128.
+constexpr int kRanked = 128;   // chunks times this stay below 2^32
+
 template <typename T, int kDim, int kGroupsOf, int kSplit, int kTogether>
 __global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, std::is_same<T, __half>::value>::kThreadsOf, 1) chunk_kernel(const __grid_constant__ DeltaDev p) {
     using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, std::is_same<T, __half>::value>;
@@ -1052,9 +1057,31 @@ __global__ void __launch_bounds__(ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, 
     const skv_gdn_args& a = p.a;
     const int slice = blockIdx.x % Room::kSlices;
     const int64_t item = blockIdx.x / Room::kSlices;
-    const int head = (int) (item % a.n_v_heads), seq = (int) (item / a.n_v_heads);
+    const int head = (int) (item % a.n_v_heads);
+    int seq = (int) (item / a.n_v_heads);
     wait_for_previous();
     int begin, end;
+    if (p.ranked) {
+        // a key per sequence: its chunks, then its place; the rank of a sequence is the number of greater keys, two threads each
+        __shared__ alignas(16) uint32_t s_keys[kRanked];
+        __shared__ int s_seq;
+        const int tid = threadIdx.x;
+        if (tid < kRanked)
+            s_keys[tid] = tid >= a.n_seqs ? 0u : (tokens_of(a, tid, begin, end) ? (uint32_t) (end - begin + kChunk - 1) / kChunk * kRanked : 0u) + kRanked - 1 - tid;
+        __syncthreads();
+        if (tid < 2 * kRanked) {
+            const uint32_t mine = s_keys[tid >> 1];
+            int rank = 0;
+            for (int i = (tid & 1) * 4; i < a.n_seqs; i += 8) {
+                const uint4 x = *reinterpret_cast<const uint4*>(s_keys + i);
+                rank += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+            }
+            rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+            if ((tid >> 1) < a.n_seqs && rank == seq) s_seq = tid >> 1;
+        }
+        __syncthreads();
+        seq = s_seq;
+    }
     if (!tokens_of(a, seq, begin, end)) return;
     float* const state = state_of(p, seq, head, kDim);
     if (!state) return;
@@ -1079,7 +1106,7 @@ cudaError_t launch_tokens(const DeltaDev& p, cudaStream_t stream) {
 }
 
 template <typename T, int kDim, int kGroupsOf, int kSplit, int kTogether>
-cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
+cudaError_t launch_chunks(const DeltaDev& p, int sms, cudaStream_t stream) {
     using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, std::is_same<T, __half>::value>;
     constexpr auto kKernel = chunk_kernel<T, kDim, kGroupsOf, kSplit, kTogether>;
     constexpr int kSmem = sizeof(Room), kPrepare = sizeof(PrepareRoom<kDim>);
@@ -1095,9 +1122,14 @@ cudaError_t launch_chunks(const DeltaDev& p, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(prepare_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepare);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
+    // finding the rank costs a CTA about 0.5 us, a long sequence that begins late some 6 us a chunk: 100 sequences of 64 tokens
+    // 314 us in their order, 328 by rank
+    DeltaDev to = p;
+    const int64_t ctas = (int64_t) p.a.n_seqs * p.a.n_v_heads * Room::kSlices;
+    to.ranked = p.a.n_seqs > 1 && p.a.n_seqs <= kRanked && (int64_t) (std::min(p.a.max_tokens, p.a.n_tokens) / kChunk + 1) * 4 * sms > ctas;
     e = launch_early(prepare_kernel<T, kDim>, dim3((unsigned) (record_slots(p.a.n_tokens, p.a.n_seqs) * p.a.n_k_heads)), kLoaderThreads, kPrepare, stream, p);
     if (e != cudaSuccess) return e;
-    return launch_early(kKernel, dim3((unsigned) ((int64_t) p.a.n_seqs * p.a.n_v_heads * Room::kSlices)), Room::kThreadsOf, kSmem, stream, p);
+    return launch_early(kKernel, dim3((unsigned) ctas), Room::kThreadsOf, kSmem, stream, to);
 }
 
 /// How long a launch of so many CTAs per sequence and head takes, one CTA per SM, in tokens of one CTA: the longest sequence
@@ -1119,10 +1151,10 @@ cudaError_t launch(const DeltaDev& p, int sms, cudaStream_t stream) {
     // 234; eight of 32 736, 658, 486.  One of 8K and 15 of 100 tokens, 32 heads: 482, 622, 797; 64 heads: 919, 747, 845.
     const int64_t narrow = span_of(p.a, sms, p.a.head_dim / 32);
     if (p.a.head_dim == 64)
-        return narrow * 3 <= span_of(p.a, sms, 1) * 4 ? launch_chunks<T, 64, 2, 2, 1>(p, stream) : launch_chunks<T, 64, 4, 1, 2>(p, stream);
+        return narrow * 3 <= span_of(p.a, sms, 1) * 4 ? launch_chunks<T, 64, 2, 2, 1>(p, sms, stream) : launch_chunks<T, 64, 4, 1, 2>(p, sms, stream);
     const int64_t middle = span_of(p.a, sms, 2) * 3, wide = span_of(p.a, sms, 1) * 4;
-    if (narrow * 2 <= std::min(middle, wide)) return launch_chunks<T, 128, 2, 2, 1>(p, stream);
-    return middle <= wide ? launch_chunks<T, 128, 4, 2, 1>(p, stream) : launch_chunks<T, 128, 8, 1, 2>(p, stream);
+    if (narrow * 2 <= std::min(middle, wide)) return launch_chunks<T, 128, 2, 2, 1>(p, sms, stream);
+    return middle <= wide ? launch_chunks<T, 128, 4, 2, 1>(p, sms, stream) : launch_chunks<T, 128, 8, 1, 2>(p, sms, stream);
 }
 
 }  // namespace

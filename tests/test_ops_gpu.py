@@ -486,6 +486,20 @@ def test_delta_of_each_width(torch_cuda, kind, vh, d, counts):
     check_delta(torch, x, first, state, out, starts, list(range(len(counts))))
 
 
+@pytest.mark.parametrize("n,vh", [(128, 4), (129, 4), (70, 48)])
+def test_delta_of_many_short_sequences(torch_cuda, n, vh):
+    """By rank, too many for ranks, too short to be worth ranks; equal lengths and none among them."""
+    torch = torch_cuda
+    counts = [int(x) for x in np.random.default_rng(n).integers(0, 71, n)]
+    counts[3], counts[5], counts[7], counts[-1] = 0, 70, 70, 64
+    x = delta_inputs(torch, 87, sum(counts), 2, vh, 128, torch.bfloat16)
+    state = normal(torch, 88, n, vh, 128, 128, scale=0.1)
+    first = state.clone()
+    out, starts = run_delta(torch, x, state, counts)
+    assert status(torch) == 0
+    check_delta(torch, x, first, state, out, starts, list(range(n)))
+
+
 @pytest.mark.parametrize("count", [5, 200])
 def test_delta_of_keys_and_queries_of_other_lengths(torch_cuda, count):
     """Keys of a tenth to twice the unit length, queries 2^20 and 2^-30 of it, large values."""
