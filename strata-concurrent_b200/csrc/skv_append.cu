@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     fetch(lo);   // on their way while the angles are worked out
 
     if (blockIdx.y == 0 && a.lengths_out) {
-        for (int s = blockIdx.x * kThreads + tid; s < a.n_seqs; s += gridDim.x * kThreads) {
+        for (int64_t s = (int64_t) blockIdx.x * kThreads + tid; s < a.n_seqs; s += (int64_t) gridDim.x * kThreads) {
             const int n = a.seq_starts ? max(0, __ldg(a.seq_starts + s + 1) - __ldg(a.seq_starts + s)) : 1;
             a.lengths_out[s] = max(0, __ldg(a.lengths + s)) + n;
         }

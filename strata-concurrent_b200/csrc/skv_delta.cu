@@ -1110,7 +1110,8 @@ cudaError_t launch_chunks(const DeltaDev& p, int sms, cudaStream_t stream) {
     using Room = ChunkRoom<kDim, kGroupsOf, kSplit, kTogether, std::is_same<T, __half>::value>;
     constexpr auto kKernel = chunk_kernel<T, kDim, kGroupsOf, kSplit, kTogether>;
     constexpr int kSmem = sizeof(Room), kPrepare = sizeof(PrepareRoom<kDim>);
-    static_assert(kSmem <= 227 * 1024, "the buffers fit an SM");
+    static_assert(kSmem + 4 * kRanked + 64 <= 227 * 1024, "the buffers fit an SM");
+    static_assert(Room::kThreadsOf >= 2 * kRanked, "two threads per ranked sequence");
     if constexpr (Room::kThreadsOf == 512) {
         // the roles' shares add up only if the CTA was launched with the registers they were made for
         static const int registers = [] {

@@ -190,6 +190,23 @@ def test_append_of_nothing(torch_cuda):
     assert torch.equal(layer.tensors[0], before[0]) and torch.equal(layer.tensors[1], before[1])
 
 
+def test_append_of_very_many_padding_rows(torch_cuda):
+    """70 million rows, five of them a sequence's: more CTAs than 2^31 threads' worth, and only those five go anywhere."""
+    torch = torch_cuda
+    n = 70_000_000
+    x = torch.zeros(n, 1, 64, dtype=torch.float16, device="cuda")
+    x[:5] = normal(torch, 9, 5, 1, 64, dtype=torch.float16)
+    k_pool, v_pool = (torch.full((4, 1, 4, 64), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    layer = skv.KvLayer(k_pool, v_pool, torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device="cuda"))
+    after = torch.full((64,), -5, dtype=torch.int32, device="cuda")
+    skv.kv_append(layer, x, x, ints(torch, [3, 0]), seq_starts=ints(torch, [0, 3, 5]), lengths_out=after[31:33])
+    assert status(torch) == 0 and after.tolist() == [-5] * 31 + [6, 2] + [-5] * 31
+    want = torch.full_like(k_pool, 7.0)
+    for row, (page, cell) in enumerate(((2, 3), (0, 0), (0, 1), (1, 0), (1, 1))):
+        want[page, 0, cell] = x[row, 0]
+    assert torch.equal(k_pool, want) and torch.equal(v_pool, want)
+
+
 def test_memory_of_another_place_is_refused(torch_cuda):
     """A pool or a state in pinned host memory never reaches a kernel."""
     torch = torch_cuda
