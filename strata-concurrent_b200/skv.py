@@ -769,7 +769,7 @@ def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=No
                 scale: float | None = None, workspace=None, stream=None) -> None:
     """The gated delta rule over packed sequences (skv_gated_delta): q, k [token][k_head][dim], v, out
     [token][v_head][dim], g, beta float32 [token][v_head], state float32 [row][v_head][dim key][dim value], updated in
-    place.  max_tokens bounds the tokens of one sequence (all of them when None).  scale: dim ** -0.5 when None."""
+    place.  max_tokens bounds the tokens of one sequence (all of them when None; a close bound splits the work better).  scale: dim ** -0.5 when None."""
     dev = q.get_device()
     qp, n, kh, dim, qs = _rows(q, "q", dev)
     kind = q.dtype
