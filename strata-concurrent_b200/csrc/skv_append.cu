@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     wait_for_previous();
     fetch(lo);   // on their way while the angles are worked out
 
-    if (blockIdx.y == 0 && a.lengths_out) {
-        for (int64_t s = (int64_t) blockIdx.x * kThreads + tid; s < a.n_seqs; s += (int64_t) gridDim.x * kThreads) {
+    if (blockIdx.y == 0 && a.lengths_out && blockIdx.x < 65536) {   // as many CTAs as keep the steps within 32 bits
+        for (uint32_t s = blockIdx.x * kThreads + tid; s < (uint32_t) a.n_seqs; s += min(gridDim.x, 65536u) * kThreads) {
             const int n = a.seq_starts ? max(0, __ldg(a.seq_starts + s + 1) - __ldg(a.seq_starts + s)) : 1;
             a.lengths_out[s] = max(0, __ldg(a.lengths + s)) + n;
         }
