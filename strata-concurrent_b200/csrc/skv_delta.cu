@@ -167,7 +167,9 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 // values after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least; the
 // state therefore keeps 32-bit quality.  What goes to the output alone (Q S, P V') takes the first of the two where that
 // is bfloat16, eight times coarser; for fp16 outputs P and V' take both.  K and Q are exact: fp16 as they are, bfloat16
-// scaled by a power of two (K by one per chunk, Q by one per row), up to values 2^-24 of the largest.  The sums G are taken
+// scaled by a power of two (K by one per chunk, Q by one per row), up to values 2^-24 of the largest.  A row of P is scaled by
+// a power of two that follows from the largest values of its query and of the chunk's keys: it neither overflows nor loses
+// more than what lies 2^-39 below what its products could reach.  The sums G are taken
 // in 64 bits and kept as two 32-bit parts, so that a decay of e^-200 in a chunk (deeper ones are as good as that) leaves the
 // others' differences exact.
 
@@ -260,8 +262,8 @@ __device__ __forceinline__ int right_half() { return (threadIdx.x >> 3) & 1; }
 struct Factors {
     float value[kChunk];    // 2^F beta
     float key[kChunk];      // 2^2F beta e^G
-    float query[kChunk];    // e^G
-    float out[kChunk];      // scale 2^(the query row's power)
+    float query[kChunk];    // e^G 2^-(the power of P's row)
+    float out[kChunk];      // scale 2^(the query row's power and that of P's row)
     float update[kChunk];   // e^(G_63 - G)
     float down[kChunk];     // 2^-(the query row's power)
     float whole;            // e^(G_63)
@@ -330,6 +332,7 @@ struct PrepareRoom {
     double carry[2];          // the first 32 tokens' sum, and all
     float beta[kChunk];
     int power[kChunk];        // of the query rows
+    int mix_power[kChunk];    // of P's rows, beyond that of the query's
     float largest[4];
 };
 
@@ -367,7 +370,7 @@ __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, con
     for (int h = 0; h < 2; ++h) {
         const int in = g + h * 8, row = kRow * 16 + in;
         const float2 sum = room.sums[row];
-        const float by = fit2 * room.beta[row];
+        const float by = fit2 * room.beta[row], down = power_of_two(-room.mix_power[row]);
 #pragma unroll
         for (int u = 0; u < kBlocks; ++u) {
             const bool below = kFrom + u < kRow;
@@ -391,7 +394,7 @@ __device__ __forceinline__ void decayed(PrepareRoom<kDim>& room, float fit2, con
                 *reinterpret_cast<float2*>(&room.work.a[row * kScratch + col]) =
                     make_float2(k0 ? by * d0 * kk[kAt + t][2 * h] : 0.0f, k1 ? by * d1 * kk[kAt + t][2 * h + 1] : 0.0f);
                 uint32_t high, low;
-                split(q0 ? d0 * qk[kAt + t][2 * h] : 0.0f, q1 ? d1 * qk[kAt + t][2 * h + 1] : 0.0f, high, low);
+                split(q0 ? d0 * (down * qk[kAt + t][2 * h]) : 0.0f, q1 ? d1 * (down * qk[kAt + t][2 * h + 1]) : 0.0f, high, low);
                 const uint32_t to = block_of(kRow, kFrom + u) * kBlockBytes + half_row_at(in, t & 1) + c * 4;
                 *reinterpret_cast<uint32_t*>(room.mix + to) = high;
                 if constexpr (kFine) *reinterpret_cast<uint32_t*>(room.mix_low + to) = low;
@@ -438,46 +441,52 @@ __global__ void __launch_bounds__(kLoaderThreads, 4) prepare_kernel(const __grid
         k[i] = on ? __ldg(reinterpret_cast<const uint4*>(kh + (int64_t) (t0 + r) * a.k_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
         q[i] = on ? __ldg(reinterpret_cast<const uint4*>(qh + (int64_t) (t0 + r) * a.q_stride + chunk * 8)) : make_uint4(0, 0, 0, 0);
     }
-    int key_power = 0;
-    if constexpr (!std::is_same<T, __half>::value) {
-        float top = 0.0f;
+    float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            float x[8];
-            unpack8<T>(k[i], x);
+    for (int i = 0; i < kMine; ++i) {
+        float x[8];
+        unpack8<T>(k[i], x);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
-        }
-        top = warp_largest(top);
-        if (lane == 0) room.largest[warp] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(room.largest[0], room.largest[1]), fmaxf(room.largest[2], room.largest[3]));
-        key_power = top > 0.0f && top < INFINITY ? min(max(exponent_of(top), -60), 60) : 0;
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
     }
+    top = warp_largest(top);
+    if (lane == 0) room.largest[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(room.largest[0], room.largest[1]), fmaxf(room.largest[2], room.largest[3]));
+    const int key_exponent = top > 0.0f && top < INFINITY ? exponent_of(top) : 0;
+    const int key_power = std::is_same<T, __half>::value ? 0 : min(max(key_exponent, -60), 60);
+    // A product of a query row and a key, as the tensor cores have them, is below kDim 2^(their largest values' exponents + 2);
+    // divided by this and by 2^(the query's exponent) it is below 2^14, whatever their sizes, and small ones keep their bits.
+    constexpr int kLogDim = kDim == 64 ? 6 : 7;
+    const int mix_base = max(key_exponent - key_power, -24) + kLogDim + 2 - 14;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
         const int at = i * kLoaderThreads + tid, r = at / kChunks, chunk = at % kChunks;
         int power = 0;
+        float x[8], most = 0.0f;
+        unpack8<T>(q[i], x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+#pragma unroll
+        for (int m = 1; m < kChunks; m <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
+        const int query_exponent = most > 0.0f && most < INFINITY ? exponent_of(most) : 0;
         if constexpr (!std::is_same<T, __half>::value) {
-            float x[8], most = 0.0f;
-            unpack8<T>(k[i], x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= power_of_two(-key_power);
-            k[i] = pack8<__half>(x);
-            unpack8<T>(q[i], x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-#pragma unroll
-            for (int m = 1; m < kChunks; m <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-            power = most > 0.0f && most < INFINITY ? min(max(exponent_of(most), -126), 126) : 0;
+            power = min(max(query_exponent, -126), 126);
             const float down = power_of_two(-power);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] *= down;
             q[i] = pack8<__half>(x);
+            unpack8<T>(k[i], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= power_of_two(-key_power);
+            k[i] = pack8<__half>(x);
         }
         *reinterpret_cast<uint4*>(room.in.k + chunk_at<kChunks>(r, chunk)) = k[i];
         *reinterpret_cast<uint4*>(room.in.q + chunk_at<kChunks>(r, chunk)) = q[i];
-        if (chunk == 0) room.power[r] = power;
+        if (chunk == 0) {
+            room.power[r] = power;
+            room.mix_power[r] = mix_base + query_exponent - power;
+        }
     }
     __syncthreads();
     // ---- K K^T and Q K^T on and below the diagonal: ten blocks of 16 x 16, at most three a warp
@@ -528,9 +537,9 @@ __global__ void __launch_bounds__(kLoaderThreads, 4) prepare_kernel(const __grid
             const float into = expf((float) sum);
             record.f.value[tid] = fit * beta;
             record.f.key[tid] = fit2 * beta * into;
-            record.f.query[tid] = into;
+            record.f.query[tid] = into * power_of_two(-room.mix_power[tid]);
             record.f.update[tid] = expf((float) (all - sum));
-            record.f.out[tid] = a.scale * power_of_two(room.power[tid]);
+            record.f.out[tid] = a.scale * power_of_two(room.power[tid]) * power_of_two(room.mix_power[tid]);
             record.f.down[tid] = power_of_two(-room.power[tid]);
             if (tid == 0) {
                 record.f.whole = expf((float) all);

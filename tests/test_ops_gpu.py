@@ -534,6 +534,46 @@ def test_delta_of_keys_and_queries_of_other_lengths(torch_cuda, count):
     check_delta(torch, (q, k, v, g, beta), first, state, out, starts, [0])
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("decay", [-1.0, -16.0])
+@pytest.mark.parametrize("size,strength", [(60000.0, 0.5), (1.0, 0.5), (2.0 ** -14, 0.5), (2.0 ** -20, 0.5), (30000.0, 512.0), (2.0 ** -7, 2.0 ** -7)])
+@pytest.mark.parametrize("count", [12, 16])
+def test_delta_of_queries_of_any_size(torch_cuda, kind, d, decay, size, strength, count):
+    """Keys of four equal values each, orthogonal to each other; a token asks for the key before its own.  So what it reads
+    is e^decay (q . k) v of that token and nothing else, whatever the sizes of q and k.  The sizes and the write strength
+    beta = 1 / |k|^2 are powers of two or exact in both types, and scale undoes them: every output is about v.
+
+    Bound.  The output's rounding; the decay, 2^-20 (an exponential of a difference within 2^-21 of it); two 16-bit operands
+    of 2^-11 each for bfloat16 outputs, of 2^-22 for float16 ones; sums of one term, whose other terms are exact zeros; values
+    of V' below 2^-39 of the largest are not kept, at most 8 here, nor decayed products of q and k below 2^-37 of d times
+    the largest values of the two (2^-39 of a power of two that is at most four times that)."""
+    torch = torch_cuda
+    dt = getattr(torch, kind)
+    if kind == "bfloat16":
+        size = 2.0 ** round(math.log2(size))
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    kh, vh = 1, 2
+    q, k = (torch.zeros(count, kh, d, dtype=dt, device="cuda") for _ in "qk")
+    for t in range(count):
+        k[t, 0, 4 * t:4 * t + 4] = strength
+        if t:
+            q[t, 0, 4 * t - 4:4 * t] = size
+    v = torch.randn(count, vh, d, generator=gen, device="cuda").clamp(-8, 8).to(dt)
+    g = torch.full((count, vh), decay, device="cuda")
+    beta = torch.full((count, vh), 0.25 / strength ** 2, device="cuda")
+    state = torch.zeros(1, vh, d, d, device="cuda")
+    # k beta v is read: |q . k| beta = 4 size strength / (4 strength^2)
+    scale = strength / size * math.exp(-decay)
+    out, _ = run_delta(torch, (q, k, v, g, beta), state, [count], scale=scale)
+    assert status(torch) == 0
+    assert (out[0] == 0).all()
+    want = v[:-1].double() * (float(np.float32(scale)) * math.exp(decay) * size / strength)
+    off = want.abs() * (R.half(dt) * (1 + 2.0 ** -7) + 2.0 ** -20 + (2.0 ** -10 if kind == "bfloat16" else 2.0 ** -21)) + 2.0 ** -36 + R.tiny(dt)
+    off = off + 2.0 ** -37 * d * size * strength * (0.25 / strength ** 2) * scale * v[:-1].double().abs()
+    assert ((out[1:].double() - want).abs() <= off).all()
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("vh", [4, 160])
 def test_delta_keeps_a_bad_token_to_its_heads(torch_cuda, bad, vh):
