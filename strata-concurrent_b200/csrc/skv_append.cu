@@ -122,6 +122,7 @@ __device__ __forceinline__ uint2 quantize(const float (&x)[8], __half& scale) {
             w[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040), __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410);
         return make_uint2(w[0], w[1]);
     }
+    if (step == 0.0f) return make_uint2(0, 0);   // a group too small for a scale
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         // ties, codes off by one, and values far past the scale

@@ -246,6 +246,29 @@ def test_append_int8_edges(torch_cuda):
             assert scale[row, g] == layer.tensors[3][page, 0, row, g]
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_append_int8_of_groups_too_small_for_a_scale(torch_cuda, kind):
+    """A group whose largest value / 127 rounds to a float16 zero (below 127 * 2^-25) has scale and codes of zero, both signs,
+    with and without a NaN; one just above has the smallest scale and codes of its own."""
+    torch = torch_cuda
+    layer = make_layer(torch, 2, [4], kv=1, dim=256, int8=True)
+    sign = torch.tensor([1.0, -1.0], device="cuda").repeat(32)
+    small = torch.zeros(4, 1, 256, dtype=torch.float64, device="cuda")
+    for row in range(4):
+        for group, size in enumerate((2.0 ** -19, 2.0 ** -24, 3e-6, 2.0 ** -18 * 1.5)):
+            small[row, 0, group * 64:group * 64 + 64] = size * sign * torch.linspace(1, 0, 64, device="cuda") ** (row + 1)
+    small = small.to(getattr(torch, kind))
+    small[3, 0, 5] = math.nan
+    skv.kv_append(layer, small, -small, ints(torch, [0]), seq_starts=ints(torch, [0, 4]))
+    assert status(torch) == 0
+    page = int(layer.tensors[4][0, 0])
+    for codes, scale, x in ((layer.tensors[0], layer.tensors[2], small), (layer.tensors[1], layer.tensors[3], -small)):
+        codes, scale = codes[page, 0].double(), scale[page, 0].double()
+        assert (scale[:, :3] == 0).all() and (codes[:, :192] == 0).all()
+        assert (scale[:, 3] == 2.0 ** -24).all()
+        assert torch.equal(codes[:, 192:], (x[:, 0, 192:].double() / 2.0 ** -24).round().clamp(-127, 127))
+
+
 # ------------------------------------------------------------------------------------------------ attention
 
 def run_attention(torch, layer, q, lengths, scale, stream=None, workspace=None):
