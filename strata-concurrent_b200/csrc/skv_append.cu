@@ -40,6 +40,13 @@ int check_layer(const skv_kv_layer* l, int n_seqs, const char* what) {
     return SKV_OK;
 }
 
+int check_layer_memory(const skv_kv_layer& l, int device, const char* what) {
+    const bool scales = l.format == SKV_KV_INT8;
+    for (const void* p : {l.k_pool, l.v_pool, scales ? l.k_scale : nullptr, scales ? l.v_scale : nullptr})
+        if (p && !ops_own_memory(p, device)) return fail(SKV_EINVAL, std::string(what) + ": the pool is not memory of the current device");
+    return SKV_OK;
+}
+
 LayerDev to_device(const skv_kv_layer& l) {
     LayerDev d{};
     d.k = static_cast<uint8_t*>(l.k_pool);
@@ -391,7 +398,7 @@ extern "C" int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* a
     }
     DeviceCtx* ctx = current_ctx();
     if (!ctx) return SKV_ECUDA;
-    if (!ops_own_memory(layer->k_pool, ctx->device)) return no("the pool is not memory of the current device");
+    if (const int rc = check_layer_memory(*layer, ctx->device, "skv_kv_append")) return rc;
     AppendDev p{};
     p.layer = to_device(*layer);
     p.a = a;

@@ -880,7 +880,7 @@ int skv_decode_attention(const skv_kv_layer* layer, const skv_attention_args* ar
         return no("the workspace must be 256-byte aligned and as large as skv_decode_attention_workspace says");
     DeviceCtx* ctx = current_ctx();
     if (!ctx) return SKV_ECUDA;
-    if (!ops_own_memory(layer->k_pool, ctx->device)) return no("the pool is not memory of the current device");
+    if (const int rc = check_layer_memory(*layer, ctx->device, "skv_decode_attention")) return rc;
     const Room room(*layer);
     AttnDev p{};
     p.layer = to_device(*layer);

@@ -25,6 +25,8 @@ inline bool ops_own_memory(const void* p, int device) {
 
 /// Refuses a layer that the kernels cannot address; SKV_OK otherwise.
 int check_layer(const skv_kv_layer* layer, int n_seqs, const char* what);
+/// Refuses a layer whose pools or scales are not memory of `device`; SKV_OK otherwise.
+int check_layer_memory(const skv_kv_layer& layer, int device, const char* what);
 
 /// A layer as the kernels take it.
 struct LayerDev {

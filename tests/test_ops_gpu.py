@@ -222,6 +222,22 @@ def test_memory_of_another_place_is_refused(torch_cuda):
     assert (host == 0).all()
 
 
+@pytest.mark.parametrize("part", ["k_pool", "v_pool", "k_scale", "v_scale"])
+def test_each_part_of_a_layer_is_looked_at(torch_cuda, part):
+    """A pool or its scales in pinned host memory (which a kernel could reach) is refused by both operators, untouched."""
+    torch = torch_cuda
+    layer = make_layer(torch, 2, [4], int8=True)
+    like = layer.tensors[("k_pool", "v_pool", "k_scale", "v_scale").index(part)]
+    host = torch.zeros(like.shape, dtype=like.dtype).pin_memory()
+    setattr(layer.args, part, host.data_ptr())
+    x = normal(torch, 1, 1, 2, 256, dtype=torch.float16)
+    with pytest.raises(skv.SkvError, match="current device"):
+        skv.kv_append(layer, x, x, ints(torch, [0]))
+    with pytest.raises(skv.SkvError, match="current device"):
+        run_attention(torch, layer, normal(torch, 1, 1, 24, 256, dtype=torch.float16), [4], 0.0625)
+    assert status(torch) == 0 and not host.any()
+
+
 def test_append_int8_edges(torch_cuda):
     """Zeros, one huge group, infinities and NaN: the other groups of the row are as without them."""
     torch = torch_cuda
