@@ -79,13 +79,28 @@ struct Geo {
 // ---------------------------------------------------------------- small pieces
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+/// The first `read` of kBytes bytes are copied, the rest becomes zeros; of none, nothing is read.
 template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool on) {   // off: zeros, nothing is read
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int read) {
     if constexpr (kBytes == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(on ? kBytes : 0) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(read) : "memory");
 }
+/// Where a copy of 4 or 8 bytes that holds the scales of `row` begins (a multiple of its size), in bytes, and how many of them
+/// are read: at head_dim 64 a row has one scale of two bytes; an even row's is the first half of its word, whose second
+/// half may lie behind the last row.
+constexpr __host__ __device__ int64_t scales_at(int64_t row, int groups) { return (row * groups * 2) & ~(int64_t) 3; }
+constexpr __host__ __device__ int scales_read(int64_t row, int groups) { return groups > 1 ? groups * 2 : row & 1 ? 4 : 2; }
+constexpr bool scales_lie_within(int64_t rows, int groups) {
+    for (int64_t row = 0; row < rows; ++row) {
+        const int64_t at = scales_at(row, groups), end = at + scales_read(row, groups);
+        if (at % (groups > 1 ? groups * 2 : 4) || end > rows * groups * 2 || row * groups * 2 < at || (row + 1) * groups * 2 > end) return false;
+    }
+    return true;
+}
+static_assert(scales_lie_within(1, 1) && scales_lie_within(2, 1) && scales_lie_within(7, 1) && scales_lie_within(5, 2) && scales_lie_within(5, 4),
+              "a row's scales are read, and nothing behind the last row's");
 __device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>
 __device__ __forceinline__ void wait_async() {
@@ -290,13 +305,13 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         for (int i = 0; i < G::kCells / kPer; ++i) {
             const int r = i * kPer + lane / G::kChunks, chunk = lane % G::kChunks;
             const int64_t from_byte = __shfl_sync(0xffffffffu, byte, r);
-            copy_async<16>(to + chunk_at<G::kChunks>(r, chunk), pool + (from_byte < 0 ? 0 : from_byte) + chunk * 16, from_byte >= 0);
+            copy_async<16>(to + chunk_at<G::kChunks>(r, chunk), pool + (from_byte < 0 ? 0 : from_byte) + chunk * 16, from_byte < 0 ? 0 : 16);
         }
         if constexpr (kInt8) {
-            // head_dim 64 has one two-byte scale per cell: the aligned word that holds it
             if (lane < G::kCells)
                 copy_async<G::kScaleBytes>(base + G::kPlane + (warp * G::kCells + lane) * G::kScaleBytes,
-                                           reinterpret_cast<const uint8_t*>(scales) + (row < 0 ? 0 : (row * G::kGroups * 2) & ~(int64_t) 3), row >= 0);
+                                           reinterpret_cast<const uint8_t*>(scales) + (row < 0 ? 0 : scales_at(row, G::kGroups)),
+                                           row < 0 ? 0 : scales_read(row, G::kGroups));
         }
     };
     // the next tile's rows and K, and the entries of the tile after it

@@ -319,6 +319,29 @@ def test_attention_ragged(torch_cuda, kind, int8, kv, heads, dim, page):
     check_attention(torch, layer, q, lengths, dim ** -0.5, got)
 
 
+@pytest.mark.parametrize("kv,page,spare", [(1, 1, 0), (1, 1, 1), (3, 1, 0), (1, 2, 0)])
+def test_attention_int8_to_the_last_scale_of_a_pool(torch_cuda, kv, page, spare):
+    """head_dim 64 has one two-byte scale a cell, copied with the word around it: odd and even numbers of rows, the last
+    page in use, what lies behind the scales full of NaN."""
+    torch = torch_cuda
+    lengths = [33, 70]
+    layer = make_layer(torch, 13, lengths, kv, 64, page, True, spare)
+    pages = layer.tensors[0].shape[0]
+    if not spare:
+        assert (layer.tensors[4] == pages - 1).any()
+    held = []
+    for i, name in ((2, "k_scale"), (3, "v_scale")):
+        n = layer.tensors[i].numel()
+        room = torch.full((n + 8,), math.nan, dtype=torch.float16, device="cuda")
+        room[:n] = layer.tensors[i].flatten()
+        setattr(layer.args, name, room.data_ptr())
+        held.append(room)
+    q = normal(torch, 14, 2, 3 * kv, 64, dtype=torch.float16)
+    got = run_attention(torch, layer, q, lengths, 0.125)
+    assert status(torch) == 0
+    check_attention(torch, layer, q, lengths, 0.125, got)
+
+
 @pytest.mark.parametrize("lengths", [[1], [37], [700], [5000], [40000], [20001, 3], [30] * 200, [0, 0, 0], [9000] + [1] * 40])
 @pytest.mark.parametrize("int8", [False, True])
 def test_attention_few_and_many(torch_cuda, lengths, int8):
