@@ -334,7 +334,9 @@ typedef struct skv_append_args {
 SKV_API int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* args, void* stream);
 
 /* skv_decode_attention - softmax(scale * q K^T) V of one new token per sequence over the first lengths[s] cells of its
- * cache.  Query head h reads K/V head h / (n_head / n_head_kv).  lse, when given, gets the natural logarithm of the
+ * cache.  Query head h reads K/V head h / (n_head / n_head_kv).  n_head is at most 4096; a sequence counts
+ * as many items as K/V heads, twice or more where more than 16 query heads share one, and a call has 2^30 items at most.
+ * lse, when given, gets the natural logarithm of the
  * sum of the exponentials per (sequence, head), so parts of one cache held apart can be joined.  A sequence of length
  * 0 (or one whose every cell was skipped, or scored minus infinity) gives zeros and lse -inf.  A length past the table
  * attends what the table holds and sets SKV_STATUS_BAD_SRC_PAGE; so does a negative one, which attends nothing.

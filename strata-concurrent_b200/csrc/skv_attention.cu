@@ -845,6 +845,12 @@ cudaError_t launch(const AttnDev& p, int dim, bool int8, int sms, cudaStream_t s
     return int8 ? launch<T, 256, true>(p, sms, stream) : launch<T, 256, false>(p, sms, stream);
 }
 
+/// A call's items and sequences are counted in 32 bits, in steps of up to a grid's CTAs.
+bool too_many_items(const skv_kv_layer& l, int n_seqs, int n_head) {
+    const int blocks = (n_head / l.n_head_kv + kRows - 1) / kRows;
+    return (int64_t) n_seqs * l.n_head_kv * blocks > (1 << 30);
+}
+
 /// The workspace: parts, their maxima and sums, the shares' cuts.
 struct Room {
     size_t ml, cut, bytes;
@@ -870,6 +876,9 @@ int skv_decode_attention_workspace(const skv_kv_layer* layer, int n_seqs, int n_
     *out_bytes = 0;
     if (n_seqs < 0 || n_head < 1) return fail(SKV_EINVAL, "skv_decode_attention_workspace: bad counts");
     if (const int rc = check_layer(layer, n_seqs, "skv_decode_attention_workspace")) return rc;
+    if (n_head > 4096 || n_head % layer->n_head_kv)
+        return fail(SKV_EINVAL, "skv_decode_attention_workspace: n_head must be a multiple of n_head_kv, at most 4096");
+    if (too_many_items(*layer, n_seqs, n_head)) return fail(SKV_ERANGE, "skv_decode_attention_workspace: too many sequences and heads");
     *out_bytes = Room(*layer).bytes;
     return SKV_OK;
 }
@@ -878,7 +887,7 @@ int skv_decode_attention(const skv_kv_layer* layer, const skv_attention_args* ar
     const auto no = [](const char* why) { return fail(SKV_EINVAL, std::string("skv_decode_attention: ") + why); };
     if (!args) return no("no arguments");
     const skv_attention_args& a = *args;
-    if (a.n_seqs < 0 || a.n_seqs > 65535) return no("n_seqs must be in [0, 65535]");
+    if (a.n_seqs < 0) return no("n_seqs is negative");
     if (const int rc = check_layer(layer, a.n_seqs, "skv_decode_attention")) return rc;
     if (a.n_head < 1 || a.n_head > 4096 || a.n_head % layer->n_head_kv) return no("n_head must be a multiple of n_head_kv, at most 4096");
     if (a.dtype != SKV_DTYPE_F16 && a.dtype != SKV_DTYPE_BF16) return no("unknown dtype");

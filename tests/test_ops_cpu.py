@@ -112,6 +112,31 @@ def test_workspace_sizes():
     refused(L.skv_gated_delta_workspace(-1, 3, 32, 128, 50, C.byref(out)), "bad sizes")
 
 
+@pytest.mark.parametrize("seqs,kv,heads,fits", [
+    (1 << 16, 2, 24, True), (1 << 29, 2, 24, True), ((1 << 29) + 1, 2, 24, False), (1 << 28, 2, 34, True), ((1 << 28) + 1, 2, 34, False),
+    (1 << 30, 1, 16, True), ((1 << 31) - 1, 1, 16, False), (1 << 30, 1, 17, False)])
+def test_attention_and_its_workspace_take_the_same_number_of_sequences(seqs, kv, heads, fits):
+    """Both refuse above 2^30 items (a sequence's K/V heads, in blocks of 16 query heads), and neither before: the
+    call then gets as far as a refusal of its scale or of its workspace, the last ones on the host."""
+    L, out, big = skv.lib(), C.c_uint64(), layer(n_tables=(1 << 31) - 1, n_head_kv=kv)
+    rc = L.skv_decode_attention_workspace(C.byref(big), seqs, heads, C.byref(out))
+    args = dict(n_seqs=seqs, n_head=heads, q_stride=heads * 256, out_stride=heads * 256, workspace_bytes=0)
+    call = L.skv_decode_attention(C.byref(big), C.byref(attention(**args)), None)
+    if fits:
+        assert rc == skv.OK and out.value % 256 == 0
+        refused(call, "workspace")
+    else:
+        assert (rc, call) == (skv.ERANGE, skv.ERANGE)
+        assert "too many" in L.skv_last_error().decode()
+
+
+@pytest.mark.parametrize("heads", [25, 4098])
+def test_the_attention_workspace_refuses_the_heads_that_attention_refuses(heads):
+    L, out = skv.lib(), C.c_uint64()
+    refused(L.skv_decode_attention_workspace(C.byref(layer()), 4, heads, C.byref(out)), "multiple")
+    refused(L.skv_decode_attention(C.byref(layer()), C.byref(attention(n_head=heads, q_stride=1 << 21, out_stride=1 << 21)), None), "multiple")
+
+
 def test_the_binding_refuses_tensors_that_do_not_fit():
     """CPU tensors, wrong types, shapes and layouts never reach the library."""
     torch = pytest.importorskip("torch")

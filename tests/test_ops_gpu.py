@@ -390,6 +390,28 @@ def test_attention_ignores_what_lies_behind_the_length(torch_cuda):
     assert ((got[0].double() - want[0]).abs() <= want[2]).all()
 
 
+def test_attention_of_70_000_sequences(torch_cuda):
+    """Lengths 0, 1 and 2 over four shared pages: a single cell's value comes back as it is, two equal keys average theirs."""
+    torch = torch_cuda
+    n = 70_000
+    k_pool = torch.zeros(4, 1, 2, 64, dtype=torch.float16, device="cuda")
+    v_pool = normal(torch, 3, 4, 1, 2, 64, dtype=torch.float16)
+    table = (torch.arange(n, device="cuda") % 4).to(torch.int32).view(n, 1)
+    layer = skv.KvLayer(k_pool, v_pool, table)
+    q = normal(torch, 4, n, 1, 64, dtype=torch.float16)
+    lengths = (torch.arange(n, device="cuda") % 3).to(torch.int32)
+    out, lse = run_attention(torch, layer, q, lengths, 0.125)
+    assert status(torch) == 0
+    v = v_pool[table[:, 0].long(), 0].double()
+    two = (lengths == 2)[:, None]
+    want = torch.where(two, v.mean(1), torch.where((lengths == 1)[:, None], v[:, 0], 0.0))
+    # keys of zero: weights of exactly 1, their sum and its reciprocal exact; one rounding
+    assert ((out[:, 0].double() - want).abs() <= want.abs() * 2.0 ** -11 + 2.0 ** -25).all()
+    assert torch.equal(out[:, 0][~two[:, 0]].double(), want[~two[:, 0]])
+    assert (lse[lengths == 0] == -math.inf).all() and (lse[lengths == 1] == 0).all()
+    assert ((lse[lengths == 2].double() - math.log(2)).abs() <= 2.0 ** -22).all()
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_attention_skips_pages_outside_the_pool(torch_cuda, int8):
     """-1 (not resident), past the pool, a whole sequence of them, a length past the table, a negative one."""
