@@ -79,13 +79,13 @@ struct Geo {
 // ---------------------------------------------------------------- small pieces
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-/// The first `read` of kBytes bytes are copied, the rest becomes zeros; of none, nothing is read.
-template <int kBytes>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int read) {
+/// The first kRead of kBytes bytes, and zeros behind them; off: zeros, nothing is read.
+template <int kBytes, int kRead = kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool on) {
     if constexpr (kBytes == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? kRead : 0) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(read) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(on ? kRead : 0) : "memory");
 }
 /// Where a copy of 4 or 8 bytes that holds the scales of `row` begins (a multiple of its size), in bytes, and how many of them
 /// are read: at head_dim 64 a row has one scale of two bytes; an even row's is the first half of its word, whose second
@@ -305,13 +305,15 @@ __global__ void __launch_bounds__(kThreads, Geo<kDim, kInt8>::kPerSm) attention_
         for (int i = 0; i < G::kCells / kPer; ++i) {
             const int r = i * kPer + lane / G::kChunks, chunk = lane % G::kChunks;
             const int64_t from_byte = __shfl_sync(0xffffffffu, byte, r);
-            copy_async<16>(to + chunk_at<G::kChunks>(r, chunk), pool + (from_byte < 0 ? 0 : from_byte) + chunk * 16, from_byte < 0 ? 0 : 16);
+            copy_async<16>(to + chunk_at<G::kChunks>(r, chunk), pool + (from_byte < 0 ? 0 : from_byte) + chunk * 16, from_byte >= 0);
         }
         if constexpr (kInt8) {
-            if (lane < G::kCells)
-                copy_async<G::kScaleBytes>(base + G::kPlane + (warp * G::kCells + lane) * G::kScaleBytes,
-                                           reinterpret_cast<const uint8_t*>(scales) + (row < 0 ? 0 : scales_at(row, G::kGroups)),
-                                           row < 0 ? 0 : scales_read(row, G::kGroups));
+            if (lane < G::kCells) {
+                const uint32_t dst = base + G::kPlane + (warp * G::kCells + lane) * G::kScaleBytes;
+                const uint8_t* src = reinterpret_cast<const uint8_t*>(scales) + (row < 0 ? 0 : scales_at(row, G::kGroups));
+                if (G::kGroups == 1 && !(row & 1)) copy_async<G::kScaleBytes, scales_read(0, G::kGroups)>(dst, src, row >= 0);
+                else copy_async<G::kScaleBytes, scales_read(1, G::kGroups)>(dst, src, row >= 0);
+            }
         }
     };
     // the next tile's rows and K, and the entries of the tile after it
