@@ -260,7 +260,7 @@ SKV_API int skv_slice_segments(const skv_segment* segs, int n_segs, uint64_t lo,
  * device, allocate nothing and can be captured into a CUDA graph (after one call outside of capture has set up the
  * device).  Activations are fp16 or bf16 (`dtype`); sums, softmax statistics, states and angles are held in 32 bits or
  * more.  Row pointers are 16-byte aligned and strides (in elements, between tokens) multiples of 8; the heads of one
- * token lie back to back.  An output may not overlap an input unless an argument says so.  Everything they are given lies
+ * token lie back to back; arrays of 32-bit values are 4-byte aligned.  An output may not overlap an input unless an argument says so.  Everything they are given lies
  * in the current device's own memory; a pool, its scales or a state elsewhere is refused (SKV_EINVAL), the other arrays are
  * not looked at here (skv.py looks at every tensor's device). */
 #define SKV_DTYPE_F16 0

@@ -36,7 +36,7 @@ int check_layer(const skv_kv_layer* l, int n_seqs, const char* what) {
         if ((reinterpret_cast<uintptr_t>(l->k_scale) | reinterpret_cast<uintptr_t>(l->v_scale)) & 7u)
             return no("scales must be 8-byte aligned");
     }
-    if (reinterpret_cast<uintptr_t>(l->page_tables) & 3u) return no("page tables must be 4-byte aligned");
+    if (!ops_aligned4(l->page_tables)) return no("page tables must be 4-byte aligned");
     return SKV_OK;
 }
 
@@ -375,6 +375,7 @@ extern "C" int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* a
     if (a.n_seqs == 0) return SKV_OK;
     if (!a.lengths) return no("no lengths");
     if (!a.seq_starts && a.n_tokens != a.n_seqs) return no("without seq_starts every sequence has one row");
+    if (!ops_aligned4(a.lengths, a.lengths_out, a.seq_starts, a.inv_freq)) return no("lengths, starts and inv_freq must be 4-byte aligned");
     if (a.lengths_out == a.lengths) return no("lengths_out must not be lengths");
     if (a.dtype != SKV_DTYPE_F16 && a.dtype != SKV_DTYPE_BF16) return no("unknown dtype");
     if (a.rope_style != SKV_ROPE_HALF && a.rope_style != SKV_ROPE_PAIRS) return no("unknown rope style");

@@ -896,6 +896,7 @@ int skv_decode_attention(const skv_kv_layer* layer, const skv_attention_args* ar
     if (!(a.scale > -INFINITY && a.scale < INFINITY)) return no("the scale must be finite");
     if (a.n_seqs == 0) return SKV_OK;
     if (!a.q || !a.out || !a.lengths) return no("missing q, out or lengths");
+    if (!ops_aligned4(a.lengths, a.lse)) return no("lengths and lse must be 4-byte aligned");
     if (!ops_aligned16(a.q) || !ops_aligned16(a.out) || a.q_stride % 8 || a.out_stride % 8)
         return no("q and out must be 16-byte aligned, their strides multiples of 8");
     const int64_t row = (int64_t) a.n_head * layer->head_dim;

@@ -1199,6 +1199,7 @@ int skv_gated_delta(const skv_gdn_args* args, void* stream) {
     if (!a.q || !a.k || !a.v || !a.out || !a.g || !a.beta || !a.state) return no("missing buffer");
     if (!ops_aligned16(a.q) || !ops_aligned16(a.k) || !ops_aligned16(a.v) || !ops_aligned16(a.out) || !ops_aligned16(a.state))
         return no("q, k, v, out and state must be 16-byte aligned");
+    if (!ops_aligned4(a.g, a.beta, a.state_index, a.seq_starts)) return no("g, beta, state_index and seq_starts must be 4-byte aligned");
     if (a.q_stride % 8 || a.k_stride % 8 || a.v_stride % 8 || a.out_stride % 8 || a.state_stride % 4)
         return no("strides must be multiples of 8 elements (4 floats for the state)");
     const int64_t kw = (int64_t) a.n_k_heads * a.head_dim, vw = (int64_t) a.n_v_heads * a.head_dim;

@@ -11,6 +11,11 @@ namespace skv {
 /// Values per scale of an int8 cell (KV_Q8_GROUP of the parked format).
 constexpr int kInt8Group = 64;
 
+/// Every one of the arrays of 32-bit values lies on a multiple of their size (none counts as well).
+template <typename... P>
+bool ops_aligned4(const P*... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & 3u) == 0;
+}
 inline bool ops_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 /// True when `p` is memory of `device` itself: a host address or another GPU's memory is refused before a launch.

@@ -89,6 +89,20 @@ def test_delta_refuses(bad, text):
     refused(skv.lib().skv_gated_delta(C.byref(delta(**bad)), None), text)
 
 
+@pytest.mark.parametrize("call,name", [(c, n) for c, names in (
+    ("append", ("lengths", "lengths_out", "seq_starts", "inv_freq")), ("attention", ("lengths", "lse")),
+    ("delta", ("g", "beta", "state_index", "seq_starts"))) for n in names])
+@pytest.mark.parametrize("off", [1, 2])
+def test_arrays_of_32_bits_off_their_alignment_are_refused(call, name, off):
+    L, bad = skv.lib(), {name: P + 0x100 + off}
+    if call == "append":
+        refused(L.skv_kv_append(C.byref(layer()), C.byref(append(**bad)), None), "4-byte")
+    elif call == "attention":
+        refused(L.skv_decode_attention(C.byref(layer()), C.byref(attention(**bad)), None), "4-byte")
+    else:
+        refused(L.skv_gated_delta(C.byref(delta(**bad)), None), "4-byte")
+
+
 def test_no_arguments_and_nothing_to_do():
     L = skv.lib()
     refused(L.skv_kv_append(None, C.byref(append()), None), "no layer")
