@@ -304,7 +304,7 @@ typedef struct skv_kv_layer {
  * value 2j with 2j+1; values from n_rot on pass through; n_rot 0 (inv_freq null) rotates nothing.  q, when given, is rotated the same way into
  * q_out, which may be q itself.  int8: scale = fp16(max |x| / 127) per 64 values, code = x / scale rounded to nearest
  * even, within +-127 (a zero scale gives codes 0; a scale past fp16 saturates; a NaN takes code 0).
- * lengths_out, when given, gets lengths[s] + the number of its rows.
+ * lengths_out, when given, gets lengths[s] + the number of its rows; a negative length counts as 0 there, and 2^31 - 1 is not passed.
  * A cell past the table (table_stride * page_size) or a negative length sets SKV_STATUS_BAD_DST_PAGE; nothing is
  * written for it in the cache (q_out is).  Two rows must not name the same cell. */
 #define SKV_ROPE_HALF 0

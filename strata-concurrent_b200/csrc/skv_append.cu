@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     if (blockIdx.y == 0 && a.lengths_out && blockIdx.x < 65536) {   // as many CTAs as keep the steps within 32 bits
         for (uint32_t s = blockIdx.x * kThreads + tid; s < (uint32_t) a.n_seqs; s += min(gridDim.x, 65536u) * kThreads) {
             const int n = a.seq_starts ? max(0, __ldg(a.seq_starts + s + 1) - __ldg(a.seq_starts + s)) : 1;
-            a.lengths_out[s] = max(0, __ldg(a.lengths + s)) + n;
+            a.lengths_out[s] = (int) min((uint32_t) max(0, __ldg(a.lengths + s)) + (uint32_t) n, 0x7fffffffu);
         }
     }
     // a warp per token: its sequence, its cell, and the cell's row in the pools

@@ -190,6 +190,19 @@ def test_append_of_nothing(torch_cuda):
     assert torch.equal(layer.tensors[0], before[0]) and torch.equal(layer.tensors[1], before[1])
 
 
+def test_append_lengths_at_the_ends_of_their_range(torch_cuda):
+    """lengths_out neither wraps nor starts below zero; cells past the table are flagged and written nowhere."""
+    torch = torch_cuda
+    layer = make_layer(torch, 6, [4, 4, 4, 4])
+    before = [x.clone() for x in layer.tensors[:2]]
+    k = normal(torch, 1, 10, 2, 256, dtype=torch.float16)
+    after = ints(torch, [0] * 4)
+    skv.kv_append(layer, k, k, ints(torch, [2 ** 31 - 1, 2 ** 31 - 3, -2 ** 31, 2 ** 31 - 3]), seq_starts=ints(torch, [0, 1, 6, 8, 10]), lengths_out=after)
+    assert status(torch) == skv.STATUS_BAD_DST_PAGE
+    assert after.tolist() == [2 ** 31 - 1, 2 ** 31 - 1, 2, 2 ** 31 - 1]
+    assert torch.equal(layer.tensors[0], before[0]) and torch.equal(layer.tensors[1], before[1])
+
+
 def test_append_of_very_many_padding_rows(torch_cuda):
     """70 million rows, five of them a sequence's: more CTAs than 2^31 threads' worth, and only those five go anywhere."""
     torch = torch_cuda
