@@ -597,7 +597,8 @@ def unpack_segments(image, dst: PooledSequence) -> list:
 
 # ------------------------------------------------------------------------------------------------ operators
 # On device tensors (torch's, or anything with its data_ptr, shape, stride, dtype and device).  They run on the current
-# device and, like the copies, on `stream` (None: the legacy default stream).
+# device and, like the copies, on `stream` (None: the legacy default stream).  They have no backward pass: a tensor that
+# requires a gradient is refused while gradients are recorded (torch.no_grad, or detach(), says that none is wanted).
 
 _CODES = {"torch.float16": DTYPE_F16, "torch.bfloat16": DTYPE_BF16}
 _KNOWN = {}     # dtype object -> (its name, its code or None), so that a call formats no text
@@ -617,9 +618,18 @@ def _dtype(x) -> tuple:
     return got
 
 
+def _no_gradient(what: str) -> None:
+    """Called for a tensor that requires a gradient."""
+    import torch
+    if torch.is_grad_enabled():
+        raise TypeError(f"{what}: requires a gradient, and the operators have no backward pass (detach it, or use torch.no_grad)")
+
+
 def _rows(x, what: str, device: int, kind=None) -> tuple:
     """(address, rows, heads, values, elements between rows) of a [row][head][value] tensor on GPU `device`, of dtype `kind`
     (None: a float16 or bfloat16 one), whose heads lie back to back."""
+    if x.requires_grad:
+        _no_gradient(what)
     n, heads, dim = x.shape
     if x.is_contiguous():
         step = heads * dim
@@ -638,6 +648,8 @@ def _rows(x, what: str, device: int, kind=None) -> tuple:
 
 def _vector(x, what: str, device: int, name: str, at_least: int) -> int:
     """The address of a contiguous 1-d tensor of at least so many `name` values on GPU `device`."""
+    if x.requires_grad:
+        _no_gradient(what)
     got = _KNOWN.get(x.dtype) or _dtype(x)
     if got[0] != name or x.dim() != 1 or x.get_device() != device or not x.is_contiguous():
         raise TypeError(f"{what}: a contiguous 1-d {name} tensor on the GPU of the others")
@@ -673,6 +685,8 @@ class KvLayer:
                 raise TypeError("KvLayer: scales are float16, [page][kv_head][cell][head_dim / 64]")
         self.device = k_pool.get_device()
         for x in (k_pool, v_pool, *scales):
+            if x.requires_grad:
+                _no_gradient("KvLayer")
             if not x.is_contiguous() or x.get_device() != self.device or self.device < 0:
                 raise ValueError("KvLayer: pools and scales must be contiguous and on the GPU, all on one")
         self._init(k_pool, v_pool, k_scale, v_scale, page_tables, pages, n_head_kv, head_dim, page_size, fmt)
@@ -750,6 +764,8 @@ def decode_attention(layer: KvLayer, q, lengths, out, *, workspace, scale: float
         raise ValueError("decode_attention: q and out are [sequence][head][head_dim] of the layer")
     lp = 0
     if lse is not None:
+        if lse.requires_grad:
+            _no_gradient("lse")
         if _dtype(lse)[0] != "torch.float32" or lse.shape != (n, heads) or not lse.is_contiguous() or lse.get_device() != dev:
             raise TypeError("decode_attention: lse is a contiguous float32 [sequence][head] tensor on the GPU")
         lp = lse.data_ptr()
@@ -779,7 +795,11 @@ def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=No
     if kn != n or kkh != kh or kd != dim or vn != n or vd != dim or on != n or oh != vh or od != dim:
         raise ValueError("gated_delta: q and k are [token][k_head][dim], v and out [token][v_head][dim]")
     steps = []
+    if state.requires_grad:
+        _no_gradient("state")
     for x, what in ((g, "g"), (beta, "beta")):
+        if x.requires_grad:
+            _no_gradient(what)
         if _dtype(x)[0] != "torch.float32" or x.shape != (n, vh) or x.get_device() != dev:
             raise TypeError(f"gated_delta: {what} is a float32 [token][v_head] tensor on the GPU")
         if x.is_contiguous():

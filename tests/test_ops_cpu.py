@@ -151,6 +151,25 @@ def test_the_attention_workspace_refuses_the_heads_that_attention_refuses(heads)
     refused(L.skv_decode_attention(C.byref(layer()), C.byref(attention(n_head=heads, q_stride=1 << 21, out_stride=1 << 21)), None), "multiple")
 
 
+def test_the_binding_refuses_tensors_that_want_a_gradient():
+    """There is no backward pass; where no gradient is recorded such a tensor is as good as any."""
+    torch = pytest.importorskip("torch")
+    x, vector = (torch.zeros(*shape, dtype=dt, requires_grad=True) for shape, dt in (((1, 2, 256), torch.float16), ((8,), torch.float32)))
+    pool, table = torch.zeros(8, 2, 4, 256, dtype=torch.float16, requires_grad=True), torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(TypeError, match="q: requires a gradient"):
+        skv._rows(x, "q", 0)
+    with pytest.raises(TypeError, match="inv_freq: requires a gradient"):
+        skv._vector(vector, "inv_freq", -1, "torch.float32", 0)
+    with pytest.raises(TypeError, match="requires a gradient"):
+        skv.KvLayer(pool, pool, table)
+    with torch.no_grad():
+        assert skv._vector(vector, "inv_freq", -1, "torch.float32", 0) == vector.data_ptr()
+        with pytest.raises(ValueError, match="not on the GPU"):
+            skv._rows(x, "q", 0)
+        with pytest.raises(ValueError, match="on the GPU"):
+            skv.KvLayer(pool, pool, table)
+
+
 def test_the_binding_refuses_tensors_that_do_not_fit():
     """CPU tensors, wrong types, shapes and layouts never reach the library."""
     torch = pytest.importorskip("torch")

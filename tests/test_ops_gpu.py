@@ -831,6 +831,29 @@ def test_delta_in_a_graph(torch_cuda):
             check_delta(torch, x, first, state, out, starts.tolist(), [0, 1, 2])
 
 
+def test_a_gradient_that_would_be_lost_is_refused(torch_cuda):
+    """Each activation, gate and state of each call; without recording the results are those of plain tensors."""
+    torch = torch_cuda
+    layer = make_layer(torch, 2, [4])
+    for name in ("q", "k", "v", "g", "beta", "state", "out"):
+        x = dict(zip(("q", "k", "v", "g", "beta"), delta_inputs(torch, 3, 2, 1, 2, 64, torch.float16)))
+        x["state"], x["out"] = torch.zeros(2, 2, 64, 64, device="cuda"), torch.zeros(2, 2, 64, dtype=torch.float16, device="cuda")
+        x[name].requires_grad_()
+        with pytest.raises(TypeError, match=f"{name}: requires a gradient"):
+            skv.gated_delta(**x)
+        with torch.no_grad():
+            skv.gated_delta(**x)
+        assert x["state"].any() and x["out"].any()
+    row, q = normal(torch, 4, 1, 2, 256, dtype=torch.float16), normal(torch, 5, 1, 24, 256, dtype=torch.float16)
+    with pytest.raises(TypeError, match="v: requires a gradient"):
+        skv.kv_append(layer, row, row.clone().requires_grad_(), ints(torch, [0]))
+    with pytest.raises(TypeError, match="q: requires a gradient"):
+        run_attention(torch, layer, q.clone().requires_grad_(), [4], 0.0625)
+    with torch.no_grad():
+        got = run_attention(torch, layer, q.clone().requires_grad_(), [4], 0.0625)
+    assert torch.equal(got[0], run_attention(torch, layer, q, [4], 0.0625)[0])
+
+
 # ------------------------------------------------------------------------------------------------ all of them, as a serving step uses them
 
 def test_a_conversation_is_prefilled_handed_over_and_continued(torch_cuda):
