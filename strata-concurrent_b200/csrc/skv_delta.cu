@@ -11,6 +11,7 @@
 #include "skv_ops.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstddef>
 #include <string>
@@ -1123,10 +1124,13 @@ cudaError_t launch_chunks(const DeltaDev& p, int sms, cudaStream_t stream) {
     static_assert(Room::kThreadsOf >= 2 * kRanked, "two threads per ranked sequence");
     if constexpr (Room::kThreadsOf == 512) {
         // the roles' shares add up only if the CTA was launched with the registers they were made for
-        static const int registers = [] {
+        static std::atomic<int> registers{0};   // the answer is kept, a failure to get one is not
+        if (registers == 0) {
             cudaFuncAttributes f{};
-            return cudaFuncGetAttributes(&f, kKernel) == cudaSuccess ? f.numRegs : 0;
-        }();
+            const cudaError_t e = cudaFuncGetAttributes(&f, kKernel);
+            if (e != cudaSuccess) return e;
+            registers = f.numRegs;
+        }
         if (registers != 128) return cudaErrorInvalidConfiguration;
     }
     cudaError_t e = cudaFuncSetAttribute(prepare_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepare);
