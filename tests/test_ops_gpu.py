@@ -122,6 +122,41 @@ def test_append_ragged(torch_cuda, kind, int8, kv, heads, dim, page, rot, style)
     assert (q_out[:lead] == 7).all() and (q_out[starts[-1]:] == 7).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("style", ["half", "pairs"])
+@pytest.mark.parametrize("scale", [1.1386294, 0.5, 0.0])
+def test_append_scales_what_it_turns(torch_cuda, kind, int8, style, scale):
+    """rope_scale multiplies the turned values of K and q alone: those from n_rot on and V are as without it."""
+    torch = torch_cuda
+    dt, n, rot, cell = getattr(torch, kind), 19, 64, 77
+    layer = make_layer(torch, 5, [cell + n], 2, 128, 16, int8)
+    k, v, q = (normal(torch, 70 + i, n, h, 128, dtype=dt) for i, h in enumerate((2, 2, 6)))
+    q_out, inv = torch.empty_like(q), 1e4 ** (-torch.arange(rot // 2, device="cuda") / (rot // 2))
+    skv.kv_append(layer, k, v, ints(torch, [cell]), seq_starts=ints(torch, [0, n]), q=q, q_out=q_out, inv_freq=inv, rope_style=style, rope_scale=scale)
+    assert status(torch) == 0
+    by = float(np.float32(scale))
+    for t in range(n):
+        at = cell + t
+        page, slot = int(layer.tensors[4][0, at // 16]), at % 16
+        for x, got in ((k, layer.tensors[0][page, :, slot]), (q, q_out[t]), (v, layer.tensors[1][page, :, slot])):
+            want, mag = x[t].double(), x[t].double().abs()
+            if x is not v:
+                want, mag = R.rotated(torch, want, at, inv, style)
+                want[:, :rot] *= by
+                mag[:, :rot] *= by
+            # cos and sin times the scale: one rounding more than a turn alone
+            off = 7 * 2.0 ** -24 * mag
+            if int8 and x is not q:
+                steps = (layer.tensors[2] if x is k else layer.tensors[3])[page, :, slot].double().repeat_interleave(64, -1)
+                got, off = got.double() * steps, off + steps * (0.5 + 127 * 2.0 ** -11 + 127 * 2.0 ** -22) + 127 * 2.0 ** -25
+            else:
+                # the cache holds float16, q_out its own type
+                to = dt if x is q else torch.float16
+                off = off + want.abs() * R.half(to) * (1 + 2.0 ** -7) + R.tiny(to)
+            assert ((got.double() - want).abs() <= off).all(), (t, x is k)
+
+
 @pytest.mark.parametrize("n", [1, 2, 9, 64, 300])
 def test_append_one_row_each_q_in_place(torch_cuda, n):
     torch = torch_cuda
