@@ -6,13 +6,14 @@ With G the sums of g from a chunk's first token on, and S the state before it:
 
 What a kernel may be off (u v: products of magnitudes; c a value column; `top` the largest magnitude in the 16 columns c is one of):
   * Each product stage is off by W = 2^-18 of the sum of its magnitudes: sums of up to 128 products in 32 bits that round or
-    cut 16 times by 2^-23 (2^-19), operands of two 16-bit parts (2^-22 each), factors with a few 2^-22.
+    cut 16 times by 2^-23 (2^-19), operands of two 16-bit parts (2^-22 each), factors with a few 2^-22.  K K^T and Q K^T are such
+    stages: where q_i . k_j nearly cancels, P_ij is off by W of |q_i| . |k_j| all the same.
   * An operand's parts end 2^-39 below its largest value (here 2^-38), T's at 2^-30 (2^-29), P's 2^-37 d below the largest values of
     its query and the chunk's keys, bfloat16 q and k 2^-24 below the largest.
   * Q S takes one part of S: 2^-11 of each product.  P V' of bfloat16 outputs takes one part of each: 2^-11 twice.
   * What was off in S before the chunk grows no more, as a step is a contraction (beta |k|^2 <= 2): E_c bounds |dS_c|, and moves
     an output by at most |q| E_c.  What is new in R and V' is followed through |T|, |P| and |K|.
-  * The output is rounded once.
+  * The output is rounded once, from a value that is off already: half a step of |O| and of what it is off by.
 Token by token (chunk 1) the same holds without the 16-bit parts.
 
 `far` bounds every element.  `square` is the mean square of the 16-bit roundings as if each were evenly spread over its step
@@ -51,7 +52,7 @@ def chunks(torch, q, k, v, g, beta, state, first, last, chunk):
         rest = write * (V - into * (K @ S))
         value = T @ rest
         after = whole * S + (K * left).transpose(1, 2) @ value
-        yield dict(a=a, b=b, Q=Q, K=K, V=V, write=write, A=A, T=T, P=P, into=into, left=left, whole=whole, R=rest, value=value, S=S, after=after)
+        yield dict(decay=decay, a=a, b=b, Q=Q, K=K, V=V, write=write, A=A, T=T, P=P, into=into, left=left, whole=whole, R=rest, value=value, S=S, after=after)
         S = after
 
 
@@ -73,6 +74,7 @@ def delta(torch, q, k, v, g, beta, state, starts, rows, scale, chunk=64):
         for c in chunks(torch, q, k, v, g, beta, state[r], starts[s], starts[s + 1], chunk):
             S, K, Q, P, T, into = c["S"].abs(), c["K"].abs(), c["Q"].abs(), c["P"].abs(), c["T"].abs(), c["into"]
             value, wrong, write = c["value"].abs(), c["R"].abs(), c["write"]
+            d_mix, d_solve = (W * c["decay"] * (x @ K.transpose(1, 2)) for x in (Q, write * K))    # of P, of A
             columns = S.sum(1, keepdim=True)
             key_floor = 2.0 ** -24 * K.amax((1, 2), keepdim=True) * columns * narrow
             query_floor = 2.0 ** -24 * Q.amax(2, keepdim=True) * columns * narrow
@@ -80,9 +82,9 @@ def delta(torch, q, k, v, g, beta, state, starts, rows, scale, chunk=64):
             d_rest = d_rest + 2.0 ** -38 * _top(wrong)
             eye = torch.eye(T.shape[1], dtype=torch.float64, device=q.device)
             ones = torch.ones_like(eye).tril()
-            d_value = T @ d_rest + (W * (T @ (eye + c["A"].abs()) @ T) + 2.0 ** -29 * (T @ ones @ T)) @ wrong
+            d_value = T @ d_rest + (T @ (W * eye + d_solve) @ T + 2.0 ** -29 * (T @ ones @ T)) @ wrong
             qs, pv = Q @ S, P @ value
-            small = W * into * qs + into * (2.0 ** -38 * _top(S) * Q.sum(2, keepdim=True) + query_floor) + W * pv
+            small = W * into * qs + into * (2.0 ** -38 * _top(S) * Q.sum(2, keepdim=True) + query_floor) + W * pv + d_mix @ value
             small = small + 2.0 ** -38 * _top(value) * P.sum(2, keepdim=True)
             small = small + 2.0 ** -37 * d * Q.amax(2, keepdim=True) * K.amax((1, 2), keepdim=True) * value.sum(1, keepdim=True)
             small = scale * (small + Q.norm(dim=2, keepdim=True) * E + P @ d_value)
@@ -97,12 +99,12 @@ def delta(torch, q, k, v, g, beta, state, starts, rows, scale, chunk=64):
             final[r] = c["after"]
             floors = write * into * (2.0 ** -38 * _top(S) * K.sum(2, keepdim=True) + key_floor) + 2.0 ** -38 * _top(wrong)
             d_rest2 = (write * W) ** 2 * (into ** 2 * (K ** 2 @ S ** 2) + c["V"] ** 2) + floors ** 2
-            d_value2 = T ** 2 @ d_rest2 + (W * (T @ (eye + c["A"].abs()) @ T)) ** 2 @ wrong ** 2 + ((2.0 ** -29 * (T @ ones @ T)) @ wrong) ** 2
+            d_value2 = T ** 2 @ d_rest2 + (T @ (W * eye + d_solve) @ T) ** 2 @ wrong ** 2 + ((2.0 ** -29 * (T @ ones @ T)) @ wrong) ** 2
             square_sum = square_sum + ((K.norm(dim=2, keepdim=True) * left) ** 2 * (d_value2 + (W * value) ** 2)).sum(1, keepdim=True)
             square_sum = square_sum + (W * S.norm(dim=1, keepdim=True)) ** 2 + (2.0 ** -38 * _top(left * value) * K.norm(dim=2).sum(1)[:, None, None]) ** 2
         off[r], spread[r] = E[:, 0], square_sum.sum((1, 2)).sqrt()
     tiny = R.tiny(kind)
-    return (out, final, far + out.abs() * half * (1 + 2.0 ** -8) + tiny, square + (out * half) ** 2 / 3, rest + tiny, off, spread)
+    return (out, final, far * (1 + half) + out.abs() * half + tiny, square + (out * half) ** 2 / 3, rest + tiny, off, spread)
 
 
 def wrong_outputs(torch, got, bounds, tokens=slice(None)):
