@@ -335,12 +335,14 @@ SKV_API int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* args
 
 /* skv_decode_attention - softmax(scale * q K^T) V of one new token per sequence over the first lengths[s] cells of its
  * cache.  Query head h reads K/V head h / (n_head / n_head_kv).  n_head is at most 4096; a sequence counts
- * as many items as K/V heads, twice or more where more than 16 query heads share one, and a call has 2^30 items at most.
- * lse, when given, gets the natural logarithm of the
- * sum of the exponentials per (sequence, head), so parts of one cache held apart can be joined.  A sequence of length
+ * as many items as K/V heads, twice or more where more than 16 query heads share one, and a call has 2^30 items at most
+ * (SKV_ERANGE).  lse, when given, gets the natural logarithm of the sum of the exponentials per (sequence, head), so parts of one cache held apart can be joined.  A sequence of length
  * 0 (or one whose every cell was skipped, or scored minus infinity) gives zeros and lse -inf.  A length past the table
  * attends what the table holds and sets SKV_STATUS_BAD_SRC_PAGE; so does a negative one, which attends nothing.
- * Results do not depend on timing: the same inputs give the same bits.
+ * Results do not depend on timing: the same inputs give the same bits.  Scores are sums of exact products in 32 bits (a bf16
+ * query counts down to 2^-24 of its row's largest value).  For its product with V a weight, of an int8 cache a weight times
+ * V's scale, is rounded to 11 bits, and counts down to 2^-39 of the largest; the sum of the weights and lse are in 32 bits.
+ * Up to 16 query heads of a K/V head share one reading of its cells; more read them once for every 16.
  * workspace: skv_decode_attention_workspace bytes of device memory, 256-byte aligned.  Its content is nobody's between
  * calls; two calls that may overlap on the GPU (two streams, two graphs) need one each. */
 typedef struct skv_attention_args {
@@ -370,8 +372,13 @@ SKV_API int skv_decode_attention_workspace(const skv_kv_layer* layer, int n_seqs
  * seq_starts as in skv_kv_append; max_tokens bounds the tokens of one sequence (a longer one is cut there), and the closer
  * it is to the longest one's, the better the work is split (eight sequences of 2,048 tokens: 486 us, 736 for a bound of
  * 16,384).  Calls of few tokens a sequence (max_tokens below 16, or seq_starts null) run token by token, the others in
- * chunks of 64 through the tensor cores; both hold S in 32 bits.  In chunks a value counts down to 2^-39 of the largest it
- * is summed with, and an infinity or a NaN in a token or a state leaves nothing to rely on of the output and state of the
+ * chunks of 64 through the tensor cores; both hold S in 32 bits.  Token by token everything is in 32 bits.  In chunks the
+ * operands of products are 16-bit values under shared powers of two: S, the tokens' corrections beta (v - k^T S) and what comes
+ * of them as two such values (22 bits, down to 2^-39 of the largest of their head among the same 16 value columns and, but for
+ * S, the same 64 tokens: a column much smaller than its neighbours keeps fewer bits); the tokens' effects on each other
+ * down to 2^-30; q . k down to 2^-37 head_dim times the largest values of the query and of the chunk's keys.  S^T q takes one
+ * value of 11 bits of S; for bf16 outputs the chunk's own part of an output takes one of both of its operands.  An infinity
+ * or a NaN in a token or a state leaves nothing to rely on of the output and state of the
  * value heads that use it, from the first token of its chunk on; other heads and sequences are as without it.
  * workspace: skv_gated_delta_workspace bytes of device memory, 256-byte aligned; as for skv_decode_attention. */
 typedef struct skv_gdn_args {

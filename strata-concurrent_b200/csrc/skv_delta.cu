@@ -165,8 +165,10 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 // chain takes 2.7 us a chunk; the bytes alone would take 125); 12 ragged fp16 sequences of 15,943 tokens in all 522 us.
 //
 // Precision.  Every product is fp16 with 32-bit sums.  A 32-bit operand (S, R, V', T, A) enters as the sum of two fp16
-// values after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least; the
-// state therefore keeps 32-bit quality.  What goes to the output alone (Q S, P V') takes the first of the two where that
+// values after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least (T:
+// 2^-30 of 1); the state therefore keeps 32-bit quality.  The largest is that of a warp's 16 value columns, of S over its keys, of
+// R and V' over the chunk's tokens: a power per column would keep a small column's bits beside large ones, but put four
+// shuffles in place of one reduction into each of four searches on the chain.  What goes to the output alone (Q S, P V') takes the first of the two where that
 // is bfloat16, eight times coarser; for fp16 outputs P and V' take both.  K and Q are exact: fp16 as they are, bfloat16
 // scaled by a power of two (K by one per chunk, Q by one per row), up to values 2^-24 of the largest.  A row of P is scaled by
 // a power of two that follows from the largest values of its query and of the chunk's keys: it neither overflows nor loses
