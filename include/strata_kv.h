@@ -336,12 +336,14 @@ SKV_API int skv_kv_append(const skv_kv_layer* layer, const skv_append_args* args
 /* skv_decode_attention - softmax(scale * q K^T) V of one new token per sequence over the first lengths[s] cells of its
  * cache.  Query head h reads K/V head h / (n_head / n_head_kv).  n_head is at most 4096; a sequence counts
  * as many items as K/V heads, twice or more where more than 16 query heads share one, and a call has 2^30 items at most
- * (SKV_ERANGE).  lse, when given, gets the natural logarithm of the sum of the exponentials per (sequence, head), so parts of one cache held apart can be joined.  A sequence of length
- * 0 (or one whose every cell was skipped, or scored minus infinity) gives zeros and lse -inf.  A length past the table
+ * (SKV_ERANGE).  lse, when given, gets the natural logarithm of the sum of the exponentials per (sequence, head), so parts
+ * of one cache held apart can be joined.  A sequence of length 0 (or one whose every cell was skipped, or scored minus infinity) gives zeros and lse -inf.  A length past the table
  * attends what the table holds and sets SKV_STATUS_BAD_SRC_PAGE; so does a negative one, which attends nothing.
  * Results do not depend on timing: the same inputs give the same bits.  Scores are sums of exact products in 32 bits (a bf16
  * query counts down to 2^-24 of its row's largest value).  For its product with V a weight, of an int8 cache a weight times
  * V's scale, is rounded to 11 bits, and counts down to 2^-39 of the largest; the sum of the weights and lse are in 32 bits.
+ * The table need not be a whole conversation's: a row of some of its pages, the partly filled one last, attends to those, and
+ * several rows of one conversation's pages with growing lengths are several new tokens of it (each reads the cells again).
  * Up to 16 query heads of a K/V head share one reading of its cells; more read them once for every 16.
  * workspace: skv_decode_attention_workspace bytes of device memory, 256-byte aligned.  Its content is nobody's between
  * calls; two calls that may overlap on the GPU (two streams, two graphs) need one each. */

@@ -19,9 +19,10 @@
 // multiplies all weights with its own quarter of V's columns.  So no warp holds an output that another has to add, and a
 // tile costs two barriers.
 //
-// Measured (24 heads on 2 K/V heads of 256, both kernels, in a graph): 131,072 fp16 cells 53 us, 5.0 TB/s; 32 ragged
-// sequences of 378 MB in all 72 us, 5.2 TB/s: the cache's bytes bound these, with 3 to 7 us of it the join.  8 x 32K int8 cells
-// 76.5 us, 3.6 TB/s: the conversion of every code to fp16 bounds it.  1,000 cells 11.4 us: two kernels' latencies.
+// Measured (24 heads on 2 K/V heads of 256, both kernels, in a graph): 131,072 fp16 cells 54 us, 5.0 TB/s; 32 ragged
+// sequences of 378 MB in all 73 us, 5.2 TB/s: the cache's bytes bound these, with 3 to 7 us of it the join.  8 x 32K int8 cells
+// 76.8 us, 3.6 TB/s: the latency of converting every code to fp16 in front of its product, with three warps a scheduler.  1,000
+// cells 11.5 us: two kernels' latencies.
 //
 // Precision.  fp16 queries and cache values meet in exact products, summed in 32 bits.  A bfloat16 query row is scaled by a
 // power of two to below 2 and becomes fp16 without loss, up to values 2^-24 of its largest.  Weights are rounded to fp16

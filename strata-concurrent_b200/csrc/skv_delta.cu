@@ -161,8 +161,9 @@ __global__ void __launch_bounds__(kThreads) token_kernel(const __grid_constant__
 // and slices of 32 columns where few CTAs would run, 4 state warps with a scheduler each; a whole head per CTA, whose
 // 8 state warps share the copies and records, where there are more than fill the GPU.
 //
-// Measured, 32 heads of 128 on 16 key heads: one bfloat16 sequence of 32K tokens 1,627 us, 230 of them prepare_kernel (the
-// chain takes 2.7 us a chunk; the bytes alone would take 125); 12 ragged fp16 sequences of 15,943 tokens in all 522 us.
+// Measured, 32 heads of 128 on 16 key heads: one bfloat16 sequence of 32K tokens 1,623 us, 230 of them prepare_kernel (the
+// chain takes 2.7 us a chunk; the bytes alone would take 125); 12 ragged fp16 sequences of 15,943 tokens in all 529 us (521
+// before rows of P had powers of their own).
 //
 // Precision.  Every product is fp16 with 32-bit sums.  A 32-bit operand (S, R, V', T, A) enters as the sum of two fp16
 // values after scaling by a power of two that puts the largest near 2^14: 22 bits, and 2^-39 of the largest at least (T:
@@ -1057,7 +1058,7 @@ constexpr int kLoaderRegisters = 48, kStateRegisters = 176, kOutputRegisters = 1
 static_assert(kLoaderRegisters * 128 + kStateRegisters * 256 + kOutputRegisters * 128 == 128 * 512, "the shares of 512 threads launched with 128 each");
 
 /// Up to so many sequences are taken longest first, so that no long one begins when the others end: 12 ragged prompts of
-/// 15,943 tokens 522 us (570 in their order), four of 1K and then one of 4K 344 (476); fp16, 32 heads of 128.
+/// 15,943 tokens 522 us (570 in their order; 529 now), four of 1K and then one of 4K 344 (476); fp16, 32 heads of 128.
 constexpr int kRanked = 128;   // chunks times this stay below 2^32
 
 template <typename T, int kDim, int kGroupsOf, int kSplit, int kTogether>

@@ -517,6 +517,32 @@ def test_attention_of_large_and_small_queries(torch_cuda):
         assert ((got[0][s].double() - want[0][s]).abs() <= want[2][s]).all()
 
 
+@pytest.mark.parametrize("int8", [False, True])
+def test_attention_through_tables_of_their_own(torch_cuda, int8):
+    """A table of some of a sequence's pages, in any order, attends to their cells (the last, partly filled one at the end);
+    several rows with one sequence's pages and growing lengths are several new tokens of it."""
+    torch = torch_cuda
+    full = make_layer(torch, 35, [333], int8=int8)
+    k_pool, v_pool, k_scale, v_scale, table = full.tensors
+    q = normal(torch, 36, 5, 24, 256, dtype=torch.float16)
+    some = torch.from_numpy(np.random.default_rng(3).permutation(83)[:41]).cuda()    # of the 83 full pages
+    picked = torch.cat([table[0][some], table[0, 83:84]])[None]
+    layer = skv.KvLayer(k_pool, v_pool, picked, k_scale=k_scale, v_scale=v_scale)
+    got = run_attention(torch, layer, q[:1], [41 * 4 + 1], 0.0625)
+    k, v, _ = R.cells_of(torch, full, 0, 333)
+    cells = torch.cat([(some[:, None] * 4 + torch.arange(4, device="cuda")).flatten(), torch.tensor([332], device="cuda")])
+    k, v = (z.repeat_interleave(12, 0)[:, cells] for z in (k, v))
+    score = torch.einsum("hd,hnd->hn", q[0].double(), k) * 0.0625
+    want = torch.einsum("hn,hnd->hd", torch.softmax(score, -1), v)
+    _, _, far, far_lse = R.attention(torch, layer, q[:1], [41 * 4 + 1], 0.0625)
+    assert ((got[0][0].double() - want).abs() <= far[0]).all()
+    assert ((got[1][0].double() - torch.logsumexp(score, -1)).abs() <= far_lse[0]).all()
+    rows = skv.KvLayer(k_pool, v_pool, table.expand(5, -1).contiguous(), k_scale=k_scale, v_scale=v_scale)
+    lengths = [329, 330, 331, 332, 333]
+    check_attention(torch, rows, q, lengths, 0.0625, run_attention(torch, rows, q, lengths, 0.0625))
+    assert status(torch) == 0
+
+
 def test_attention_past_4_gib(torch_cuda):
     torch = torch_cuda
     pages, page, n = 16500, 256, 300
