@@ -628,7 +628,7 @@ def _no_gradient(what: str) -> None:
 def _rows(x, what: str, device: int, kind=None) -> tuple:
     """(address, rows, heads, values, elements between rows) of a [row][head][value] tensor on GPU `device`, of dtype `kind`
     (None: a float16 or bfloat16 one), whose heads lie back to back."""
-    if x.requires_grad:
+    if getattr(x, "requires_grad", False):
         _no_gradient(what)
     n, heads, dim = x.shape
     if x.is_contiguous():
@@ -648,7 +648,7 @@ def _rows(x, what: str, device: int, kind=None) -> tuple:
 
 def _vector(x, what: str, device: int, name: str, at_least: int) -> int:
     """The address of a contiguous 1-d tensor of at least so many `name` values on GPU `device`."""
-    if x.requires_grad:
+    if getattr(x, "requires_grad", False):
         _no_gradient(what)
     got = _KNOWN.get(x.dtype) or _dtype(x)
     if got[0] != name or x.dim() != 1 or x.get_device() != device or not x.is_contiguous():
@@ -685,7 +685,7 @@ class KvLayer:
                 raise TypeError("KvLayer: scales are float16, [page][kv_head][cell][head_dim / 64]")
         self.device = k_pool.get_device()
         for x in (k_pool, v_pool, *scales):
-            if x.requires_grad:
+            if getattr(x, "requires_grad", False):
                 _no_gradient("KvLayer")
             if not x.is_contiguous() or x.get_device() != self.device or self.device < 0:
                 raise ValueError("KvLayer: pools and scales must be contiguous and on the GPU, all on one")
@@ -765,7 +765,7 @@ def decode_attention(layer: KvLayer, q, lengths, out, *, workspace, scale: float
         raise ValueError("decode_attention: q and out are [sequence][head][head_dim] of the layer")
     lp = 0
     if lse is not None:
-        if lse.requires_grad:
+        if getattr(lse, "requires_grad", False):
             _no_gradient("lse")
         if _dtype(lse)[0] != "torch.float32" or lse.shape != (n, heads) or not lse.is_contiguous() or lse.get_device() != dev:
             raise TypeError("decode_attention: lse is a contiguous float32 [sequence][head] tensor on the GPU")
@@ -797,10 +797,10 @@ def gated_delta(q, k, v, g, beta, state, out, *, seq_starts=None, state_index=No
     if kn != n or kkh != kh or kd != dim or vn != n or vd != dim or on != n or oh != vh or od != dim:
         raise ValueError("gated_delta: q and k are [token][k_head][dim], v and out [token][v_head][dim]")
     steps = []
-    if state.requires_grad:
+    if getattr(state, "requires_grad", False):
         _no_gradient("state")
     for x, what in ((g, "g"), (beta, "beta")):
-        if x.requires_grad:
+        if getattr(x, "requires_grad", False):
             _no_gradient(what)
         if _dtype(x)[0] != "torch.float32" or x.shape != (n, vh) or x.get_device() != dev:
             raise TypeError(f"gated_delta: {what} is a float32 [token][v_head] tensor on the GPU")

@@ -170,6 +170,24 @@ def test_the_binding_refuses_tensors_that_want_a_gradient():
             skv.KvLayer(pool, pool, table)
 
 
+def test_the_binding_takes_what_has_a_tensors_methods():
+    """Without a requires_grad of its own, too: it gets as far as the look at its device."""
+    torch = pytest.importorskip("torch")
+
+    class Like:
+        def __init__(self, x):
+            self.x = x
+
+        def __getattr__(self, name):
+            if name == "requires_grad":
+                raise AttributeError(name)
+            return getattr(self.x, name)
+
+    with pytest.raises(ValueError, match="not on the GPU"):
+        skv._rows(Like(torch.zeros(1, 2, 256, dtype=torch.float16)), "q", 0)
+    assert skv._vector(Like(torch.zeros(4, dtype=torch.int32)), "lengths", -1, "torch.int32", 4)
+
+
 def test_the_binding_refuses_tensors_that_do_not_fit():
     """CPU tensors, wrong types, shapes and layouts never reach the library."""
     torch = pytest.importorskip("torch")
